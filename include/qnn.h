@@ -455,6 +455,72 @@ int qnn_qconv2d_generic_fwd(const float* x, int n, int c, int h, int w, float ne
 int qnn_chain_epilogue(const uint8_t* bncode, int n, int ho, int wo, int c, const qnn_epilogue* epi,
                        qnn_stream_t stream);
 
+/* ---------------------------------------------------------- float operators
+ *
+ * The operators of a student's training step that are not quantized (qnn/functional.py).  Matrices
+ * are row-major with a row stride ("ld", in elements, at least the row's length); the last index is
+ * dense.  Sums, statistics and states are held in fp32 whatever the type; each output is rounded
+ * once.  Nothing is kept between calls: `work` is scratch of at least the size that the matching
+ * *_work call gives (16-byte aligned), free for other use once the call's kernels have run.  Every
+ * result is the same from run to run (no floating-point atomics). */
+enum { QNN_F32 = 0, QNN_BF16 = 1, QNN_F16 = 2 };
+enum { QNN_ACT_NONE = 0, QNN_ACT_RELU = 1, QNN_ACT_GELU = 2 };
+
+/* y[m][n] = act(z), z = x[m][k] w[n][k]^T + bias[n] + res[m][n] (bias, res nullable), in the order of
+ * the int8 epilogue: the residual first, then the activation.  GELU is z Phi(z).  All of one type.
+ * slope (nullable): act'(z) for qnn_linear_act_bwd --
+ *   ReLU  [m][ceil(n / 8)] bytes, bit c & 7 of byte c / 8: z is not <= 0;
+ *   GELU  [m][n], fp32 for QNN_F32, else int16 fixed point of 1 / 28672 (-32768: NaN).
+ * 1 <= n, k < 2^31 and m < 2^31; m == 0 is a no-op.  Replaces nothing of the reference (its layers are
+ * F.linear on fake-quantized operands, quantize.py:423-430); stands beside qnn_qconv2d_fwd. */
+int qnn_linear_act_fwd_work(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes);
+int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res,
+                       int64_t ldr, void* y, void* slope, int64_t m, int64_t n, int64_t k, int dtype, int act,
+                       void* work, int64_t work_bytes, qnn_stream_t stream);
+/* dz = dy * act'(z); dx[m][k] = dz w; dw[n][k] = dz^T x; db[n] = sum over m of dz; each of dx, dw, db is
+ * nullable.  dz [m][n] (it is the residual's gradient too): required unless act is QNN_ACT_NONE, for
+ * which dz == dy and it is not written.  slope: what the forward wrote.  dz, rounded to the type, is
+ * what the products take. */
+int qnn_linear_act_bwd_work(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes);
+int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const void* x, int64_t ldx, const void* w,
+                       int64_t ldw, void* dz, void* dx, void* dw, void* db, int64_t m, int64_t n, int64_t k,
+                       int dtype, int act, void* work, int64_t work_bytes, qnn_stream_t stream);
+
+/* y = (x - mean) rstd w + b over the last dim, mean and the biased variance of each row in two steps
+ * (the deviations, not the squares' difference), rstd = 1 / sqrt(var + eps).  w, b nullable (1, 0), of
+ * type wdtype: dtype or QNN_F32.  mean, rstd [rows] fp32, nullable: what the backward takes. */
+int qnn_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, float* mean, float* rstd,
+                       int64_t rows, int64_t dim, float eps, int dtype, int wdtype, qnn_stream_t stream);
+/* g = dy w, xh = (x - mean) rstd: dx = rstd (g - mean(g) - xh mean(g xh)), dw = sum over rows of dy xh,
+ * db = sum over rows of dy; dx, dw, db nullable. */
+int qnn_layer_norm_bwd_work(int64_t rows, int64_t dim, int dtype, int64_t* bytes);
+int qnn_layer_norm_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* w, const float* mean,
+                       const float* rstd, void* dx, void* dw, void* db, int64_t rows, int64_t dim, int dtype,
+                       int wdtype, void* work, int64_t work_bytes, qnn_stream_t stream);
+
+/* Distillation from a teacher's top logits.  Row r has `top` entries: teacher logits t[r][e] at the
+ * student's classes index[r][e] (int64 when index_bytes is 8, int32 when 4); an entry with a negative
+ * index is absent, one with index >= vocab makes the row's loss and gradient NaN.  With p the softmax
+ * of t / temp over the entries that are there, q the softmax of s / temp over the vocabulary:
+ *   row_loss[r] = temp^2 sum_e p_e (log p_e - log q_index[e])      (an entry with p_e = 0 adds 0)
+ *   ds[r][j]    = g temp (q_j - sum over e with index[e] == j of p_e)
+ * A row without entries, or whose teacher logits are all -inf, is not counted: loss 0, gradient 0.
+ * row_loss [rows]; stats [4 rows + 4] fp32, what the backward takes; loss (nullable): one fp32,
+ * the sum of the counted rows' losses, over their number when mean != 0 (0 rows counted: 0).
+ * 1 <= top <= 1024, vocab < 2^31.  Replaces the soft-target loss of the distillation trainer
+ * (qdistiler_main.py) for teachers of whom only the top logits are kept. */
+int qnn_topk_distill_fwd_work(int64_t rows, int64_t vocab, int dtype, int64_t* bytes);
+int qnn_topk_distill_fwd(const void* s, int64_t lds, const void* t, int64_t ldt, const void* index, int64_t ldi,
+                         int64_t rows, int64_t vocab, int64_t top, float temp, int mean, int dtype, int tdtype,
+                         int index_bytes, float* row_loss, float* stats, float* loss, void* work,
+                         int64_t work_bytes, qnn_stream_t stream);
+/* grad: the loss's gradient, fp32 on the device: one value (grad_rows == 0, for `loss`; mean as in the
+ * forward) or one for each row (grad_rows != 0, for `row_loss`).  stats: what the forward wrote. */
+int qnn_topk_distill_bwd(const void* s, int64_t lds, const void* t, int64_t ldt, const void* index, int64_t ldi,
+                         const float* stats, const float* grad, int grad_rows, void* ds, int64_t rows,
+                         int64_t vocab, int64_t top, float temp, int mean, int dtype, int tdtype, int index_bytes,
+                         qnn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,130 @@
+// Shared by the float operators (matmul.hip, layer_norm.hip, distill.hip): element types,
+// 16-byte groups of a row, reductions over a wave, the activations.
+#pragma once
+#include <math.h>
+
+#include <type_traits>
+
+#include "qnn_internal.h"
+
+namespace qnn {
+namespace fl {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+// Elements of a type in one 16-byte load: the group in which rows are read and written.
+template <class T>
+constexpr int GROUP = 16 / (int)sizeof(T);
+
+template <class T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+// N consecutive elements at p as floats; `whole` (uniform over the launch): p is aligned for one
+// wide load and all N are there, else those at or past `left` read as `fill`.
+template <class T, int N>
+__device__ __forceinline__ void load_n(float (&o)[N], const T* p, int64_t left, bool whole, float fill = 0.0f) {
+  if (whole) {
+    if constexpr (sizeof(T) * N <= 16) {
+      const Vec<T, N> t = *reinterpret_cast<const Vec<T, N>*>(p);
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = (float)t.v[i];
+    } else {
+      constexpr int G = GROUP<T>;
+#pragma unroll
+      for (int g = 0; g < N / G; ++g) {
+        const Vec<T, G> t = reinterpret_cast<const Vec<T, G>*>(p)[g];
+#pragma unroll
+        for (int i = 0; i < G; ++i) o[g * G + i] = (float)t.v[i];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = i < left ? (float)p[i] : fill;
+  }
+}
+
+template <class T, int N>
+__device__ __forceinline__ void store_n(T* p, const float (&o)[N], int64_t left, bool whole) {
+  if (whole) {
+    constexpr int G = sizeof(T) * N <= 16 ? N : GROUP<T>;
+#pragma unroll
+    for (int g = 0; g < N / G; ++g) {
+      Vec<T, G> t;
+#pragma unroll
+      for (int i = 0; i < G; ++i) t.v[i] = (T)o[g * G + i];
+      reinterpret_cast<Vec<T, G>*>(p)[g] = t;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < left) p[i] = (T)o[i];
+  }
+}
+
+__device__ __forceinline__ float wave_sum_f(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// e^x by the hardware's 2^x; the product's rounding costs |x| 2^-24 of relative error.
+__device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+
+// GELU z Phi(z) and its derivative Phi(z) + z phi(z) together, from one exponential:
+// Phi(-a) = erfc(a / sqrt 2) / 2 and erfc(u) = e^(-u^2) t P(t), t = 1 / (1 + 0.36 u), with P fitted
+// here to the scaled complement e^(u^2) erfc(u) (relative error 3.6e-8 for all u), so that the
+// far negative side keeps its relative precision too.  z^2 is carried with its rounding error.
+// The limits at the infinities are 0 and 0 below, z and 1 above; a NaN stays one.
+__device__ __forceinline__ void gelu_f(float z, float& y, float& slope) {
+  const float a = fminf(fabsf(z), 20.0f);  // phi and erfc are 0 in 32 bits long before
+  const float s = a * a, sl = fmaf(a, a, -s);
+  const float e = exp_f(-0.5f * s) * fmaf(-0.5f, sl, 1.0f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.36f * 0.70710678118654752f, a, 1.0f));
+  float p = 0.03754199f;
+  p = fmaf(p, t, -0.14138553f);
+  p = fmaf(p, t, 0.14222577f);
+  p = fmaf(p, t, -0.02727648f);
+  p = fmaf(p, t, 0.10558839f);
+  p = fmaf(p, t, 0.12331503f);
+  p = fmaf(p, t, 0.16381756f);
+  p = fmaf(p, t, 0.18995832f);
+  p = fmaf(p, t, 0.20310671f);
+  p = fmaf(p, t, 0.20310828f);
+  const float tail = 0.5f * e * p * t;
+  const float cdf = z < 0.0f ? tail : 1.0f - tail;
+  const float zc = z < 0.0f ? -a : a;
+  y = z <= -20.0f ? -0.0f : z * cdf;
+  const float d = fmaf(zc * 0.39894228040143268f, e, cdf);
+  slope = z != z ? z : d;
+}
+
+// The derivative of GELU between the passes, for 16-bit types: fixed point of 2^-15 1.75 (it lies in
+// [-0.13, 1.13]), off by at most 1.8e-5 -- a fourteenth of fp16's half step at 1, where z itself
+// rounded to the type would add an error as large as that of the gradient's own rounding.
+constexpr float SLOPE_STEPS = 28672.0f;
+__device__ __forceinline__ int16_t slope_pack(float d) {
+  return d != d ? (int16_t)-32768 : (int16_t)(int)rintf(d * SLOPE_STEPS);
+}
+__device__ __forceinline__ float slope_unpack(int16_t q) {
+  return q == -32768 ? __builtin_nanf("") : (float)q * (1.0f / SLOPE_STEPS);
+}
+
+template <class F>
+static inline int with_type(int dtype, F&& f) {
+  switch (dtype) {
+    case QNN_F32: return f((float)0);
+    case QNN_BF16: return f((bf16)0.0f);
+    case QNN_F16: return f((f16)0.0f);
+  }
+  return arg_error("dtype: QNN_F32, QNN_BF16 or QNN_F16");
+}
+
+static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+static inline int type_bytes(int dtype) { return dtype == QNN_F32 ? 4 : 2; }
+
+}  // namespace fl
+}  // namespace qnn

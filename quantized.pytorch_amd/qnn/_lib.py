@@ -112,6 +112,22 @@ SIGNATURES = {
     "qnn_debug_set_spin_limit": [c_int],
     "qnn_rangebn_f32": [c_ptr, c_ptr, c_int, c_int, c_int, c_float, c_float, c_float, c_float, c_ptr, c_ptr, c_ptr,
                         c_ptr, c_ptr, c_int, c_ptr],
+    "qnn_linear_act_fwd_work": [c_i64, c_i64, c_i64, c_int, c_ptr],
+    "qnn_linear_act_fwd": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_int,
+                           c_int, c_ptr, c_i64, c_ptr],
+    "qnn_linear_act_bwd_work": [c_i64, c_i64, c_i64, c_int, c_ptr],
+    "qnn_linear_act_bwd": [c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64,
+                           c_i64, c_int, c_int, c_ptr, c_i64, c_ptr],
+    "qnn_layer_norm_fwd": [c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_float, c_int, c_int,
+                           c_ptr],
+    "qnn_layer_norm_bwd_work": [c_i64, c_i64, c_int, c_ptr],
+    "qnn_layer_norm_bwd": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int,
+                           c_int, c_ptr, c_i64, c_ptr],
+    "qnn_topk_distill_fwd_work": [c_i64, c_i64, c_int, c_ptr],
+    "qnn_topk_distill_fwd": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_i64, c_float, c_int, c_int,
+                             c_int, c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr],
+    "qnn_topk_distill_bwd": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_int, c_ptr, c_i64, c_i64,
+                             c_i64, c_float, c_int, c_int, c_int, c_int, c_ptr],
 }
 
 
