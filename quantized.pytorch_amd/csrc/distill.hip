@@ -1,10 +1,18 @@
 // Distillation from a teacher's top logits (include/qnn.h: qnn_topk_distill_fwd, qnn_topk_distill_bwd).
 //   p = softmax(t / T) over a row's entries that are there, q = softmax(s / T) over the vocabulary
 //   row_loss = T^2 sum_e p_e (log p_e - log q_{i_e});  ds_j = g T (q_j - sum over i_e == j of p_e)
+//
+// Bound by HBM: forward reads the logits once (largest logit and sum of exponentials together, the sum
+// rescaled when the maximum grows), backward reads them and writes their gradient.  A wave takes a row
+// of up to 16 KiB, a workgroup a longer one; where there are few long rows the forward pass cuts them
+// into pieces whose (maximum, sum) pairs a second launch joins.  The gradient is dense but for the
+// teacher's classes: a workgroup writes its piece of the row as if there were none, and then the
+// classes that lie in it again, the first entry of a class with the sum of all of them.
+//
 // stats, four floats a row: the largest student logit, 1 / sum of e^((s - largest) / T), the largest
 // teacher logit, 1 / the teacher's sum (0: the row is not counted); then the number of counted rows.
 // A row whose statistics are not numbers (an index past the vocabulary, all of its logits -inf, a
-// NaN) carries a NaN in the second, which makes its whole gradient NaN.
+// NaN, the teacher's too) carries a NaN in the second, which makes its whole gradient NaN.
 #include "float_common.h"
 
 namespace qnn {
@@ -13,26 +21,10 @@ using namespace fl;
 
 constexpr int NT = 256;
 constexpr int MAX_TOP = 1024;
-
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-  v = wave_sum_f(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = sh[0];
-  for (int w = 1; w < NT / 64; ++w) r += sh[w];
-  return r;
-}
-
-__device__ __forceinline__ float block_max(float v, float* sh) {
-  v = wave_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = sh[0];
-  for (int w = 1; w < NT / 64; ++w) r = fmaxf(r, sh[w]);
-  return r;
-}
+constexpr int WIDE = 512;        // lanes for a row or a piece that is longer than a wave's
+constexpr int WAVE_BYTES = 16384;  // the longest row that a wave takes
+constexpr int MAX_SPLITS = 64;   // pieces of a row: a lane each when they are joined
+constexpr float LOG2E = 1.44269504088896341f;
 
 struct Entries {
   const void* t;
@@ -51,51 +43,152 @@ struct Entries {
   }
 };
 
-// one block per row
-template <class T>
-__global__ __launch_bounds__(NT) void distill_rows_kernel(const T* s, int64_t lds, Entries en, int64_t vocab,
-                                                          float temp, float* row_loss, float* stats) {
-  __shared__ float sh[NT / 64];
-  const int64_t r = blockIdx.x;
-  const T* sr = s + r * lds;
-  const float it = 1.0f / temp;
-  float m = -INFINITY;
-  for (int64_t c = threadIdx.x; c < vocab; c += NT) m = fmaxf(m, (float)sr[c]);
-  m = block_max(m, sh);
-  float sum = 0.0f;
-  for (int64_t c = threadIdx.x; c < vocab; c += NT) sum += exp_f(((float)sr[c] - m) * it);
-  sum = block_sum(sum, sh);
-  float tm = -INFINITY, bad = 0.0f;
-  for (int e = threadIdx.x; e < en.top; e += NT) {
-    const int64_t i = en.klass(r, e);
-    if (i >= 0) tm = fmaxf(tm, en.logit(r, e));
-    if (i >= vocab) bad = 1.0f;
+// A running (maximum, sum of e^((x - maximum) / T)); k = log2(e) / T.  While the maximum is -inf the
+// sum is taken from 0 instead, so that logits of -inf add 0 and not NaN.
+struct Run {
+  float m, s;
+};
+__device__ __forceinline__ float from(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// This lane's run over s[lo, hi): groups (lo + lane GROUP), L GROUP apart, U of them in flight.
+template <class T, int L>
+__device__ __forceinline__ Run run_over(const T* s, int64_t lo, int64_t hi, int lane, float k) {
+  constexpr int GR = GROUP<T>, U = 4;
+  Run a = {-INFINITY, 0.0f};
+  auto add = [&](const float* v, int n) {
+    float m = a.m;
+#pragma unroll
+    for (int i = 0; i < n; ++i) m = fmaxf(m, v[i]);
+    const float f = from(m);
+    float t = a.s * __builtin_amdgcn_exp2f((a.m - f) * k);
+#pragma unroll
+    for (int i = 0; i < n; ++i) t += __builtin_amdgcn_exp2f((v[i] - f) * k);
+    a = {m, t};
+  };
+  int64_t c = lo + lane * GR;
+  for (; c + (U - 1) * L * GR + GR <= hi; c += U * L * GR) {
+    Vec<T, GR> raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = load_group(s + c + u * L * GR, GR);
+#pragma unroll
+    for (int u = 0; u < U; u += 2) {
+      float v[2 * GR];
+#pragma unroll
+      for (int i = 0; i < GR; ++i) v[i] = (float)raw[u].v[i], v[GR + i] = (float)raw[u + 1].v[i];
+      add(v, 2 * GR);
+    }
   }
-  tm = block_max(tm, sh);
-  bad = block_max(bad, sh);
-  const bool counted = tm > -INFINITY || bad > 0.0f;
+  for (; c < hi; c += L * GR) {
+    const Vec<T, GR> raw = load_group(s + c, hi - c);
+    float v[GR];
+#pragma unroll
+    for (int i = 0; i < GR; ++i) v[i] = c + i < hi ? (float)raw.v[i] : -INFINITY;
+    add(v, GR);
+  }
+  return a;
+}
+
+// ---- reductions over the L lanes of a row (L 64, or a workgroup)
+template <int L, class V, class Op>
+__device__ __forceinline__ V over_lanes(V v, Op op) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+  if constexpr (L > 64) {
+    __shared__ V sh[L / 64];
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < L / 64; ++w) v = op(v, sh[w]);
+  }
+  return v;
+}
+template <int L>
+__device__ __forceinline__ Run over_lanes_run(Run a, float k) {
+  const float m = over_lanes<L>(a.m, [](float x, float y) { return fmaxf(x, y); });
+  const float s = a.s * __builtin_amdgcn_exp2f((a.m - from(m)) * k);
+  return {m, over_lanes<L>(s, [](float x, float y) { return x + y; })};
+}
+
+// The row's statistics and loss from its lanes' runs.
+template <class T, int L>
+__device__ __forceinline__ void finish_row(const T* sr, Run a, const Entries& en, int64_t r, int64_t vocab, float temp,
+                                           int lane, float* row_loss, float* stats) {
+  auto add = [](float x, float y) { return x + y; };
+  auto most = [](float x, float y) { return fmaxf(x, y); };
+  const float k = LOG2E / temp, it = 1.0f / temp;
+  a = over_lanes_run<L>(a, k);
+  if (a.m == -INFINITY) a.s = __builtin_nanf("");  // all of the row's logits are -inf
+  float tm = -INFINITY, bad = 0.0f;
+  for (int e = lane; e < en.top; e += L) {
+    const int64_t i = en.klass(r, e);
+    const float t = i >= 0 ? en.logit(r, e) : -INFINITY;
+    tm = fmaxf(tm, t);
+    if (i >= vocab || t != t) bad = 1.0f;
+  }
+  tm = over_lanes<L>(tm, most);
+  bad = over_lanes<L>(bad, most);
+  const bool some = tm > -INFINITY;
+  // sum of the teacher's exponentials, and of e_e (u_e - log q_e): the loss is their quotient less log
+  // of the sum, since the p_e add up to 1
   float ts = 0.0f;
-  if (tm > -INFINITY)
-    for (int e = threadIdx.x; e < en.top; e += NT)
-      if (en.klass(r, e) >= 0) ts += exp_f((en.logit(r, e) - tm) * it);
-  ts = block_sum(ts, sh);
+  if (some)
+    for (int e = lane; e < en.top; e += L)
+      if (en.klass(r, e) >= 0) ts += __builtin_amdgcn_exp2f((en.logit(r, e) - tm) * k);
+  ts = over_lanes<L>(ts, add);
+  const float lts = logf(ts), ls = logf(a.s);
   float l = 0.0f;
-  if (tm > -INFINITY && bad == 0.0f)
-    for (int e = threadIdx.x; e < en.top; e += NT) {
+  if (some && bad == 0.0f)
+    for (int e = lane; e < en.top; e += L) {
       const int64_t i = en.klass(r, e);
       if (i < 0) continue;
-      const float u = (en.logit(r, e) - tm) * it, p = exp_f(u) / ts;
-      if (p != 0.0f) l += p * ((u - logf(ts)) - (((float)sr[i] - m) * it - logf(sum)));
+      const float u = (en.logit(r, e) - tm) * it, p = __builtin_amdgcn_exp2f(u * LOG2E) / ts;
+      if (p != 0.0f) l += p * ((u - lts) - (((float)sr[i] - a.m) * it - ls));
     }
-  l = block_sum(l, sh);
-  if (threadIdx.x == 0) {
-    if (bad > 0.0f) l = sum = __builtin_nanf("");
+  l = over_lanes<L>(l, add);
+  if (lane == 0) {
+    if (bad > 0.0f) l = a.s = __builtin_nanf("");
+    const bool counted = some || bad > 0.0f;
     row_loss[r] = counted ? temp * temp * l : 0.0f;
-    stats[4 * r] = m;
-    stats[4 * r + 1] = 1.0f / sum;
-    stats[4 * r + 2] = tm;
-    stats[4 * r + 3] = counted ? (bad > 0.0f ? 1.0f : 1.0f / ts) : 0.0f;
+    float4 st = {a.m, 1.0f / a.s, tm, counted ? (bad > 0.0f ? 1.0f : 1.0f / ts) : 0.0f};
+    *reinterpret_cast<float4*>(stats + 4 * r) = st;
   }
+}
+
+// L lanes a row
+template <class T, int L>
+__global__ __launch_bounds__(L > NT ? L : NT) void distill_rows_kernel(const T* s, int64_t lds, Entries en, int64_t rows,
+                                                                       int64_t vocab, float temp, float* row_loss,
+                                                                       float* stats) {
+  constexpr int ROWS = L > NT ? 1 : NT / L;
+  const int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / L;
+  if (r >= rows) return;  // a whole wave: L > 64 has a row for every workgroup
+  const int lane = threadIdx.x % L;
+  const Run a = run_over<T, L>(s + r * lds, 0, vocab, lane, LOG2E / temp);
+  finish_row<T, L>(s + r * lds, a, en, r, vocab, temp, lane, row_loss, stats);
+}
+
+// piece (row, split) of long rows: its run into part[row][split]
+template <class T>
+__global__ __launch_bounds__(WIDE) void distill_part_kernel(const T* s, int64_t lds, int64_t vocab, float temp,
+                                                            int splits, int64_t piece, Run* part) {
+  const int64_t r = blockIdx.x / splits;
+  const int64_t lo = blockIdx.x % splits * piece, hi = lo + piece < vocab ? lo + piece : vocab;
+  const float k = LOG2E / temp;
+  const Run a = over_lanes_run<WIDE>(run_over<T, WIDE>(s + r * lds, lo, hi, threadIdx.x, k), k);
+  if (threadIdx.x == 0) part[(int64_t)blockIdx.x] = a;
+}
+
+template <class T>
+__global__ __launch_bounds__(NT) void distill_split_rows_kernel(const T* s, int64_t lds, Entries en, int64_t rows,
+                                                                int64_t vocab, float temp, int splits,
+                                                                const Run* part, float* row_loss, float* stats) {
+  const int64_t r = (int64_t)blockIdx.x * (NT / 64) + threadIdx.x / 64;
+  if (r >= rows) return;
+  const int lane = threadIdx.x % 64;
+  const Run a = lane < splits ? part[r * splits + lane] : Run{-INFINITY, 0.0f};
+  finish_row<T, 64>(s + r * lds, a, en, r, vocab, temp, lane, row_loss, stats);
 }
 
 __global__ __launch_bounds__(NT) void distill_join_kernel(const float* row_loss, float* stats, float* loss,
@@ -117,34 +210,97 @@ __global__ __launch_bounds__(NT) void distill_join_kernel(const float* row_loss,
   }
 }
 
-template <class T>
-__global__ __launch_bounds__(NT) void distill_grad_kernel(const T* s, int64_t lds, Entries en, const float* stats,
-                                                          const float* grad, int grad_rows, T* ds, int64_t rows,
-                                                          int64_t vocab, float temp, int mean) {
-  __shared__ int64_t cls[MAX_TOP];
-  const int64_t r = blockIdx.x;
+// The gradient of a row's piece [lo, lo + PIECE), L lanes.
+template <class T, int L>
+struct Grad {
+  static constexpr int THREADS = L > NT ? L : NT, ROWS = THREADS / L;
+  static constexpr int64_t PIECE = L > 64 ? (int64_t)L * 4 * GROUP<T> : WAVE_BYTES / (int)sizeof(T);
+};
+
+template <class T, int L>
+__global__ __launch_bounds__((Grad<T, L>::THREADS)) void distill_grad_kernel(const T* s, int64_t lds, Entries en,
+                                                                             const float* stats, const float* grad,
+                                                                             int grad_rows, T* ds, int64_t rows,
+                                                                             int64_t vocab, int pieces, float temp,
+                                                                             int mean) {
+  constexpr int GR = GROUP<T>, ROWS = Grad<T, L>::ROWS;
+  __shared__ int cls[ROWS][MAX_TOP];
+  __shared__ float mass[ROWS][MAX_TOP];
+  __shared__ int found[ROWS];
+  const int sub = threadIdx.x / L, lane = threadIdx.x % L;
+  const int64_t r = (int64_t)(blockIdx.x / pieces) * ROWS + sub;
+  const int64_t lo = blockIdx.x % pieces * Grad<T, L>::PIECE;
+  const int64_t hi = lo + Grad<T, L>::PIECE < vocab ? lo + Grad<T, L>::PIECE : vocab;
+  const float k = LOG2E / temp;
   const T* sr = s + r * lds;
   T* dr = ds + r * vocab;
-  const float it = 1.0f / temp;
-  const float m = stats[4 * r], inv = stats[4 * r + 1], tm = stats[4 * r + 2], ti = stats[4 * r + 3];
-  float g = temp * (grad_rows ? grad[r] : grad[0]);
-  if (mean) g /= fmaxf(stats[4 * rows], 1.0f);
-  for (int e = threadIdx.x; e < en.top; e += NT) cls[e] = en.klass(r, e);
-  for (int64_t c = threadIdx.x; c < vocab; c += NT)
-    dr[c] = ti == 0.0f ? (T)0.0f : (T)(g * (exp_f(((float)sr[c] - m) * it) * inv));
-  __syncthreads();  // the entries' classes are written again, by the first entry of each class
-  if (ti == 0.0f) return;
-  for (int e = threadIdx.x; e < en.top; e += NT) {
-    const int64_t i = cls[e];
-    if (i < 0 || i >= vocab) continue;
-    bool first = true;
-    for (int f = 0; f < e; ++f) first = first && cls[f] != i;
-    if (!first) continue;
-    float p = 0.0f;
-    for (int f = e; f < en.top; ++f)
-      if (cls[f] == i) p += exp_f((en.logit(r, f) - tm) * it) * ti;
-    dr[i] = (T)(g * (exp_f(((float)sr[i] - m) * it) * inv - p));
+  float m = 0.0f, inv = 0.0f, ti = 0.0f, g = 0.0f;
+  if (r < rows) {
+    const float4 st = *reinterpret_cast<const float4*>(stats + 4 * r);
+    m = st.x, inv = st.y, ti = st.w;
+    g = temp * (grad_rows ? grad[r] : grad[0]);
+    if (mean) g /= fmaxf(stats[4 * rows], 1.0f);
+    if (lane < 64) {  // the row's first wave picks the entries of this piece, in their order
+      int n = 0;
+      for (int e0 = 0; e0 < en.top; e0 += 64) {
+        const int e = e0 + lane;
+        const int64_t i = e < en.top && ti != 0.0f ? en.klass(r, e) : -1;
+        const bool in = i >= lo && i < hi;
+        const unsigned long long all = __ballot(in);
+        if (in) {
+          const int at = n + __popcll(all & ((1ull << lane) - 1));
+          cls[sub][at] = (int)i;
+          mass[sub][at] = __builtin_amdgcn_exp2f((en.logit(r, e) - st.z) * k) * ti;
+        }
+        n += __popcll(all);
+      }
+      if (lane == 0) found[sub] = n;
+    }
+    auto value = [&](float v) { return ti == 0.0f ? 0.0f : g * (__builtin_amdgcn_exp2f((v - m) * k) * inv); };
+    constexpr int U = 4;
+    int64_t c = lo + lane * GR;
+    for (; c + (U - 1) * L * GR + GR <= hi; c += U * L * GR) {
+      Vec<T, GR> raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = load_group(sr + c + u * L * GR, GR);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < GR; ++i) raw[u].v[i] = (T)value((float)raw[u].v[i]);
+        store_group(dr + c + u * L * GR, raw[u], GR);
+      }
+    }
+    for (; c < hi; c += L * GR) {
+      Vec<T, GR> raw = load_group(sr + c, hi - c);
+#pragma unroll
+      for (int i = 0; i < GR; ++i) raw.v[i] = (T)value((float)raw.v[i]);
+      store_group(dr + c, raw, hi - c);
+    }
   }
+  __syncthreads();  // the lists, and the piece as it is without the teacher
+  if (r >= rows) return;
+  const int n = found[sub];
+  for (int e = lane; e < n; e += L) {
+    const int i = cls[sub][e];
+    bool first = true;
+    for (int f = 0; f < e; ++f) first = first && cls[sub][f] != i;
+    if (!first) continue;
+    float p = mass[sub][e];
+    for (int f = e + 1; f < n; ++f)
+      if (cls[sub][f] == i) p += mass[sub][f];
+    dr[i] = (T)(g * (__builtin_amdgcn_exp2f(((float)sr[i] - m) * k) * inv - p));
+  }
+}
+
+// Pieces of a row in the forward pass: none for rows that a wave takes; else as many as fill the chip
+// with four workgroups a CU, each with two rounds of loads at least.
+int splits_of(int64_t rows, int64_t vocab, int dtype) {
+  const int64_t size = type_bytes(dtype);
+  if (rows == 0 || vocab * size <= WAVE_BYTES) return 1;
+  int64_t n = cdiv(1024, rows);
+  const int64_t most = cdiv(vocab * size, WIDE * 16 * 2);
+  if (n > most) n = most;
+  return (int)(n > MAX_SPLITS ? MAX_SPLITS : n);
 }
 
 int check(const void* s, int64_t lds, const void* t, int64_t ldt, const void* index, int64_t ldi, int64_t rows,
@@ -157,6 +313,7 @@ int check(const void* s, int64_t lds, const void* t, int64_t ldt, const void* in
   QNN_REQUIRE(tdtype == QNN_F32 || tdtype == QNN_BF16 || tdtype == QNN_F16, "tdtype: QNN_F32, QNN_BF16 or QNN_F16");
   QNN_REQUIRE(index_bytes == 4 || index_bytes == 8, "index_bytes: 4 or 8");
   QNN_REQUIRE(stats && (rows == 0 || (s && t && index)), "null pointer");
+  QNN_REQUIRE(aligned16(stats), "stats: on a 16-byte boundary");
   return QNN_OK;
 }
 
@@ -170,7 +327,9 @@ extern "C" {
 
 int qnn_topk_distill_fwd_work(int64_t rows, int64_t vocab, int dtype, int64_t* bytes) {
   QNN_REQUIRE(rows >= 0 && vocab >= 1 && bytes, "bad shape or null pointer");
-  *bytes = 0;
+  QNN_REQUIRE(dtype == QNN_F32 || dtype == QNN_BF16 || dtype == QNN_F16, "dtype: QNN_F32, QNN_BF16 or QNN_F16");
+  const int n = splits_of(rows, vocab, dtype);
+  *bytes = n > 1 ? rows * n * (int64_t)sizeof(Run) : 0;
   return QNN_OK;
 }
 
@@ -184,9 +343,25 @@ int qnn_topk_distill_fwd(const void* s, int64_t lds, const void* t, int64_t ldt,
   hipStream_t st = (hipStream_t)stream;
   const int rc = with_type(dtype, [&](auto z) {
     using T = decltype(z);
-    if (rows > 0)
-      hipLaunchKernelGGL((distill_rows_kernel<T>), dim3((unsigned)rows), dim3(NT), 0, st, (const T*)s, lds, en, vocab,
-                         temp, row_loss, stats);
+    const int splits = splits_of(rows, vocab, dtype);
+    if (rows == 0) return (int)QNN_OK;
+    if (splits > 1) {
+      QNN_REQUIRE(work && work_bytes >= rows * splits * (int64_t)sizeof(Run),
+                  "work: at least what qnn_topk_distill_fwd_work says");
+      // a whole number of groups, so that pieces begin where a lane's loads do
+      const int64_t piece = cdiv(cdiv(vocab, splits), GROUP<T>) * GROUP<T>;
+      hipLaunchKernelGGL((distill_part_kernel<T>), dim3((unsigned)(rows * splits)), dim3(WIDE), 0, st, (const T*)s, lds,
+                         vocab, temp, splits, piece, (Run*)work);
+      QNN_LAUNCH_CHECK("qnn_topk_distill_fwd");
+      hipLaunchKernelGGL((distill_split_rows_kernel<T>), dim3((unsigned)cdiv(rows, NT / 64)), dim3(NT), 0, st,
+                         (const T*)s, lds, en, rows, vocab, temp, splits, (const Run*)work, row_loss, stats);
+    } else if (vocab * (int64_t)sizeof(T) <= WAVE_BYTES) {
+      hipLaunchKernelGGL((distill_rows_kernel<T, 64>), dim3((unsigned)cdiv(rows, NT / 64)), dim3(NT), 0, st,
+                         (const T*)s, lds, en, rows, vocab, temp, row_loss, stats);
+    } else {
+      hipLaunchKernelGGL((distill_rows_kernel<T, WIDE>), dim3((unsigned)rows), dim3(WIDE), 0, st, (const T*)s, lds, en,
+                         rows, vocab, temp, row_loss, stats);
+    }
     QNN_LAUNCH_CHECK("qnn_topk_distill_fwd");
     return (int)QNN_OK;
   });
@@ -206,8 +381,18 @@ int qnn_topk_distill_bwd(const void* s, int64_t lds, const void* t, int64_t ldt,
   const Entries en = {t, ldt, index, ldi, (int)top, tdtype, index_bytes};
   return with_type(dtype, [&](auto z) {
     using T = decltype(z);
-    hipLaunchKernelGGL((distill_grad_kernel<T>), dim3((unsigned)rows), dim3(NT), 0, (hipStream_t)stream, (const T*)s,
-                       lds, en, stats, grad, grad_rows, (T*)ds, rows, vocab, temp, mean);
+    auto launch = [&](auto lanes) {
+      constexpr int L = decltype(lanes)::value;
+      using G = Grad<T, L>;
+      const int64_t pieces = cdiv(vocab, G::PIECE), blocks = cdiv(rows, G::ROWS) * pieces;
+      QNN_REQUIRE(blocks < (1LL << 31), "too many logits for one call");
+      hipLaunchKernelGGL((distill_grad_kernel<T, L>), dim3((unsigned)blocks), dim3(G::THREADS), 0, (hipStream_t)stream,
+                         (const T*)s, lds, en, stats, grad, grad_rows, (T*)ds, rows, vocab, (int)pieces, temp, mean);
+      return (int)QNN_OK;
+    };
+    const int rc = vocab * (int64_t)sizeof(T) <= WAVE_BYTES ? launch(std::integral_constant<int, 64>{})
+                                                            : launch(std::integral_constant<int, WIDE>{});
+    if (rc) return rc;
     QNN_LAUNCH_CHECK("qnn_topk_distill_bwd");
     return (int)QNN_OK;
   });

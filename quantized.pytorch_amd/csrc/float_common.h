@@ -18,45 +18,71 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 template <class T>
 constexpr int GROUP = 16 / (int)sizeof(T);
 
+// N elements that may begin at any element: the type's alignment is all that the compiler assumes, and
+// the card's loads and stores of 16 bytes take any address.
 template <class T, int N>
-struct alignas(sizeof(T) * N) Vec {
+struct Vec {
   T v[N];
 };
+struct __attribute__((packed, aligned(2))) Bytes16 {
+  uint32_t v[4];
+};
 
-// N consecutive elements at p as floats; `whole` (uniform over the launch): p is aligned for one
-// wide load and all N are there, else those at or past `left` read as `fill`.
+// The group of elements at p, raw: 16 bytes in one load if all of it is there, else those at or past
+// `left` as 0.
+template <class T>
+__device__ __forceinline__ Vec<T, GROUP<T>> load_group(const T* p, int64_t left) {
+  Vec<T, GROUP<T>> o;
+  if (left >= GROUP<T>) {
+    const Bytes16 t = *reinterpret_cast<const Bytes16*>(p);
+    __builtin_memcpy(&o, &t, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < GROUP<T>; ++i) o.v[i] = i < left ? p[i] : (T)0.0f;
+  }
+  return o;
+}
+
+template <class T>
+__device__ __forceinline__ void store_group(T* p, const Vec<T, GROUP<T>>& o, int64_t left) {
+  if (left >= GROUP<T>) {
+    Bytes16 t;
+    __builtin_memcpy(&t, &o, 16);
+    *reinterpret_cast<Bytes16*>(p) = t;
+  } else {
+#pragma unroll
+    for (int i = 0; i < GROUP<T>; ++i)
+      if (i < left) p[i] = o.v[i];
+  }
+}
+
+// N consecutive elements at p as floats, those at or past `left` as 0 (N a whole number of groups).
 template <class T, int N>
-__device__ __forceinline__ void load_n(float (&o)[N], const T* p, int64_t left, bool whole, float fill = 0.0f) {
-  if (whole) {
-    if constexpr (sizeof(T) * N <= 16) {
-      const Vec<T, N> t = *reinterpret_cast<const Vec<T, N>*>(p);
+__device__ __forceinline__ void load_n(float (&o)[N], const T* p, int64_t left) {
+  constexpr int G = GROUP<T>;
+  if (left >= N) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = (float)t.v[i];
-    } else {
-      constexpr int G = GROUP<T>;
+    for (int g = 0; g < N / G; ++g) {
+      const Vec<T, G> t = load_group(p + g * G, G);
 #pragma unroll
-      for (int g = 0; g < N / G; ++g) {
-        const Vec<T, G> t = reinterpret_cast<const Vec<T, G>*>(p)[g];
-#pragma unroll
-        for (int i = 0; i < G; ++i) o[g * G + i] = (float)t.v[i];
-      }
+      for (int i = 0; i < G; ++i) o[g * G + i] = (float)t.v[i];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = i < left ? (float)p[i] : fill;
+    for (int i = 0; i < N; ++i) o[i] = i < left ? (float)p[i] : 0.0f;
   }
 }
 
 template <class T, int N>
-__device__ __forceinline__ void store_n(T* p, const float (&o)[N], int64_t left, bool whole) {
-  if (whole) {
-    constexpr int G = sizeof(T) * N <= 16 ? N : GROUP<T>;
+__device__ __forceinline__ void store_n(T* p, const float (&o)[N], int64_t left) {
+  constexpr int G = GROUP<T>;
+  if (left >= N) {
 #pragma unroll
     for (int g = 0; g < N / G; ++g) {
       Vec<T, G> t;
 #pragma unroll
       for (int i = 0; i < G; ++i) t.v[i] = (T)o[g * G + i];
-      reinterpret_cast<Vec<T, G>*>(p)[g] = t;
+      store_group(p + g * G, t, G);
     }
   } else {
 #pragma unroll

@@ -2,44 +2,289 @@
 //   mean = sum(x) / d, var = sum((x - mean)^2) / d, rstd = 1 / sqrt(var + eps), xh = (x - mean) rstd
 //   y = xh w + b;  g = dy w;  dx = rstd (g - mean(g) - xh mean(g xh))
 //   dw = sum over rows of dy xh;  db = sum over rows of dy
+//
+// Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx, each once.  A row
+// lives in the registers of L lanes (G groups of 16 bytes a lane), so the two-step variance and the two
+// means of the backward pass cost no second read.  A workgroup takes rows in strides of the grid and
+// loads its next row before it works on the present one; the weights stay in registers from row to
+// row.  The backward pass sums dw and db on the way: a lane has the same columns in every row, so they
+// are sums in its registers, joined over a workgroup's rows in LDS, written as one partial row a
+// workgroup and added up by a second, small launch in a fixed order.
 #include "float_common.h"
 
 namespace qnn {
 namespace {
 using namespace fl;
 
-constexpr int NT = 256;
-
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-  v = wave_sum_f(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = sh[0];
-  for (int w = 1; w < NT / 64; ++w) r += sh[w];
-  return r;
+// Sums over the L lanes that share a row: shuffles, then (L > 64) the waves' results through LDS,
+// two slots used in turn so that one barrier a sum is enough.
+template <int L, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float* sh, int& turn) {
+#pragma unroll
+  for (int o = (L < 64 ? L : 64) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
+  if constexpr (L > 64) {
+    constexpr int W = L / 64;
+    float* at = sh + turn * 2 * W;
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) at[i * W + threadIdx.x / 64] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s = at[i * W];
+#pragma unroll
+      for (int w = 1; w < W; ++w) s += at[i * W + w];
+      v[i] = s;
+    }
+  }
 }
 
-// one block per row
+// L lanes a row, G groups of 16 bytes a lane: lane l has columns (j L + l) GROUP + i, j < G, i < GROUP.
+template <int L_, int G_>
+struct Shape {
+  static constexpr int L = L_, G = G_, NT = L > 256 ? L : 256, ROWS = NT / L;
+};
+
+template <class T, class W, class S>
+__global__ __launch_bounds__(S::NT) void layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx,
+                                                               const W* __restrict__ w, const W* __restrict__ b,
+                                                               T* __restrict__ y, float* __restrict__ mean,
+                                                               float* __restrict__ rstd, int64_t rows, int dim,
+                                                               float eps) {
+  constexpr int L = S::L, G = S::G, GR = GROUP<T>;
+  __shared__ float sh[4 * (L > 64 ? L / 64 : 1)];
+  const int lane = threadIdx.x % L, sub = threadIdx.x / L;
+  int turn = 0;
+  const float inv = 1.0f / (float)dim;
+  float wv[G][GR], bv[G][GR];
+#pragma unroll
+  for (int j = 0; j < G; ++j) {
+    const int c = (j * L + lane) * GR;
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+      wv[j][i] = 1.0f;
+      bv[j][i] = 0.0f;
+    }
+    if (w) load_n<W, GR>(wv[j], w + c, dim - c);
+    if (b) load_n<W, GR>(bv[j], b + c, dim - c);
+  }
+  Vec<T, GR> next[G];
+  int64_t r = (int64_t)blockIdx.x * S::ROWS + sub;
+  const int64_t step = (int64_t)gridDim.x * S::ROWS;
+  auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int c = (j * L + lane) * GR;
+      next[j] = load_group(x + row * ldx + c, row < rows ? dim - c : 0);
+    }
+  };
+  fetch(r);
+  // every lane of a workgroup takes part in every round, for the barriers in its sums
+  for (int64_t r0 = (int64_t)blockIdx.x * S::ROWS; r0 < rows; r0 += step, r += step) {
+    float v[G][GR];
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+      for (int i = 0; i < GR; ++i) {
+        v[j][i] = (float)next[j].v[i];
+        s[0] += v[j][i];
+      }
+    fetch(r + step);
+    row_sums<L>(s, sh, turn);
+    const float mu = s[0] * inv;
+    float q[1] = {0.0f};
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+      for (int i = 0; i < GR; ++i) {
+        v[j][i] = (j * L + lane) * GR + i < dim ? v[j][i] - mu : 0.0f;
+        q[0] = fmaf(v[j][i], v[j][i], q[0]);
+      }
+    row_sums<L>(q, sh, turn);
+    const float rs = 1.0f / sqrtf(fmaf(q[0], inv, eps));
+    if (r < rows) {
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        const int c = (j * L + lane) * GR;
+        Vec<T, GR> o;
+#pragma unroll
+        for (int i = 0; i < GR; ++i) o.v[i] = (T)fmaf(v[j][i] * rs, wv[j][i], bv[j][i]);
+        store_group(y + r * dim + c, o, dim - c);
+      }
+      if (lane == 0 && mean) mean[r] = mu;
+      if (lane == 0 && rstd) rstd[r] = rs;
+    }
+  }
+}
+
+// part: [gridDim.x][2][dim], this workgroup's sums of dw and db (null: not wanted)
+template <class T, class W, class S>
+__global__ __launch_bounds__(S::NT) void layer_norm_bwd_kernel(const T* __restrict__ dy, int64_t ldy,
+                                                               const T* __restrict__ x, int64_t ldx,
+                                                               const W* __restrict__ w,
+                                                               const float* __restrict__ mean,
+                                                               const float* __restrict__ rstd, T* __restrict__ dx,
+                                                               float* __restrict__ part, int64_t rows, int dim) {
+  constexpr int L = S::L, G = S::G, GR = GROUP<T>;
+  __shared__ float sh[4 * (L > 64 ? L / 64 : 1)];
+  const int lane = threadIdx.x % L, sub = threadIdx.x / L;
+  int turn = 0;
+  const float inv = 1.0f / (float)dim;
+  float wv[G][GR], aw[G][GR] = {}, ab[G][GR] = {};
+#pragma unroll
+  for (int j = 0; j < G; ++j) {
+    const int c = (j * L + lane) * GR;
+#pragma unroll
+    for (int i = 0; i < GR; ++i) wv[j][i] = 1.0f;
+    if (w) load_n<W, GR>(wv[j], w + c, dim - c);
+  }
+  Vec<T, GR> nx[G], ny[G];
+  float nmu, nrs;
+  int64_t r = (int64_t)blockIdx.x * S::ROWS + sub;
+  const int64_t step = (int64_t)gridDim.x * S::ROWS;
+  auto fetch = [&](int64_t row) {
+    const bool there = row < rows;
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int c = (j * L + lane) * GR;
+      nx[j] = load_group(x + row * ldx + c, there ? dim - c : 0);
+      ny[j] = load_group(dy + row * ldy + c, there ? dim - c : 0);
+    }
+    nmu = there ? mean[row] : 0.0f;
+    nrs = there ? rstd[row] : 0.0f;
+  };
+  fetch(r);
+  for (int64_t r0 = (int64_t)blockIdx.x * S::ROWS; r0 < rows; r0 += step, r += step) {
+    float h[G][GR], g[G][GR];
+    float s[2] = {0.0f, 0.0f};
+    const float mu = nmu, rs = nrs;
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+#pragma unroll
+      for (int i = 0; i < GR; ++i) {
+        // past the row's end x and dy are 0 here: xh is off, but dy xh and g xh are 0 and so no sum is
+        // (a mean that is no number makes them NaN; they are not written)
+        h[j][i] = ((float)nx[j].v[i] - mu) * rs;
+        const float d = (float)ny[j].v[i];
+        const float dh = d * h[j][i];
+        g[j][i] = d * wv[j][i];
+        aw[j][i] += dh;
+        ab[j][i] += d;
+        s[0] += g[j][i];
+        s[1] = fmaf(g[j][i], h[j][i], s[1]);
+      }
+    fetch(r + step);
+    if (dx) {
+      row_sums<L>(s, sh, turn);
+      const float sg = s[0] * inv, sx = s[1] * inv;
+      if (r < rows) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          const int c = (j * L + lane) * GR;
+          Vec<T, GR> o;
+#pragma unroll
+          for (int i = 0; i < GR; ++i) o.v[i] = (T)(rs * (g[j][i] - sg - h[j][i] * sx));
+          store_group(dx + r * dim + c, o, dim - c);
+        }
+      }
+    }
+  }
+  if (!part) return;
+  if constexpr (S::ROWS > 1) {  // the workgroup's rows, in their order
+    __shared__ float all[S::ROWS][L * G * GR];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < G; ++j)
+#pragma unroll
+        for (int i = 0; i < GR; ++i) all[sub][(j * L + lane) * GR + i] = which ? ab[j][i] : aw[j][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < dim; c += S::NT) {
+        float s = all[0][c];
+#pragma unroll
+        for (int k = 1; k < S::ROWS; ++k) s += all[k][c];
+        part[((int64_t)blockIdx.x * 2 + which) * dim + c] = s;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      const int c = (j * L + lane) * GR;
+      float* p = part + (int64_t)blockIdx.x * 2 * dim + c;
+      store_n<float, GR>(p, aw[j], dim - c);
+      store_n<float, GR>(p + dim, ab[j], dim - c);
+    }
+  }
+}
+
+// dw and db from `parts` partial rows: 64 columns a workgroup, 16 threads a column
+template <class W>
+__global__ __launch_bounds__(1024) void layer_norm_join_kernel(const float* __restrict__ part, int parts, int dim,
+                                                               W* dw, W* db) {
+  __shared__ float sh[16][64];
+  const int lane = threadIdx.x & 63, k = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;  // over dw's columns, then db's
+  float s = 0.0f;
+  if (c < 2 * (int64_t)dim) {
+#pragma unroll 8
+    for (int p = k; p < parts; p += 16) s += part[(int64_t)p * 2 * dim + c];
+  }
+  sh[k][lane] = s;
+  __syncthreads();
+  if (k == 0 && c < 2 * (int64_t)dim) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += sh[i][lane];
+    if (c < dim) {
+      if (dw) dw[c] = (W)s;
+    } else if (db) {
+      db[c - dim] = (W)s;
+    }
+  }
+}
+
+// ---- rows too long for registers: a workgroup a row, read again (from L2) for each step
+constexpr int LONG = 1024;
+
 template <class T, class W>
-__global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* x, int64_t ldx, const W* w, const W* b, T* y,
-                                                            float* mean, float* rstd, int64_t dim, float eps) {
-  __shared__ float sh[NT / 64];
+__global__ __launch_bounds__(LONG) void layer_norm_fwd_long_kernel(const T* x, int64_t ldx, const W* w, const W* b,
+                                                                   T* y, float* mean, float* rstd, int64_t dim,
+                                                                   float eps) {
+  constexpr int GR = GROUP<T>;
+  __shared__ float sh[4 * (LONG / 64)];
   const int64_t r = blockIdx.x;
   const T* xr = x + r * ldx;
-  T* yr = y + r * dim;
-  float s = 0.0f;
-  for (int64_t c = threadIdx.x; c < dim; c += NT) s += (float)xr[c];
-  const float mu = block_sum(s, sh) / (float)dim;
-  float q = 0.0f;
-  for (int64_t c = threadIdx.x; c < dim; c += NT) {
-    const float d = (float)xr[c] - mu;
-    q = fmaf(d, d, q);
+  int turn = 0;
+  float s[1] = {0.0f}, q[1] = {0.0f}, v[GR];
+  for (int64_t c = threadIdx.x * GR; c < dim; c += LONG * GR) {
+    load_n<T, GR>(v, xr + c, dim - c);
+#pragma unroll
+    for (int i = 0; i < GR; ++i) s[0] += v[i];
   }
-  const float rs = 1.0f / sqrtf(block_sum(q, sh) / (float)dim + eps);
-  for (int64_t c = threadIdx.x; c < dim; c += NT) {
-    const float xh = ((float)xr[c] - mu) * rs;
-    yr[c] = (T)fmaf(xh, w ? (float)w[c] : 1.0f, b ? (float)b[c] : 0.0f);
+  row_sums<LONG>(s, sh, turn);
+  const float mu = s[0] / (float)dim;
+  for (int64_t c = threadIdx.x * GR; c < dim; c += LONG * GR) {
+    load_n<T, GR>(v, xr + c, dim - c);
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+      const float d = c + i < dim ? v[i] - mu : 0.0f;
+      q[0] = fmaf(d, d, q[0]);
+    }
+  }
+  row_sums<LONG>(q, sh, turn);
+  const float rs = 1.0f / sqrtf(q[0] / (float)dim + eps);
+  for (int64_t c = threadIdx.x * GR; c < dim; c += LONG * GR) {
+    float wv[GR], bv[GR];
+    load_n<T, GR>(v, xr + c, dim - c);
+    if (w) load_n<W, GR>(wv, w + c, dim - c);
+    if (b) load_n<W, GR>(bv, b + c, dim - c);
+#pragma unroll
+    for (int i = 0; i < GR; ++i) v[i] = fmaf((v[i] - mu) * rs, w ? wv[i] : 1.0f, b ? bv[i] : 0.0f);
+    store_n<T, GR>(y + r * dim + c, v, dim - c);
   }
   if (threadIdx.x == 0) {
     if (mean) mean[r] = mu;
@@ -48,42 +293,65 @@ __global__ __launch_bounds__(NT) void layer_norm_fwd_kernel(const T* x, int64_t 
 }
 
 template <class T, class W>
-__global__ __launch_bounds__(NT) void layer_norm_dx_kernel(const T* dy, int64_t ldy, const T* x, int64_t ldx,
-                                                           const W* w, const float* mean, const float* rstd, T* dx,
-                                                           int64_t dim) {
-  __shared__ float sh[NT / 64];
+__global__ __launch_bounds__(LONG) void layer_norm_dx_long_kernel(const T* dy, int64_t ldy, const T* x, int64_t ldx,
+                                                                  const W* w, const float* mean, const float* rstd,
+                                                                  T* dx, int64_t dim) {
+  constexpr int GR = GROUP<T>;
+  __shared__ float sh[4 * (LONG / 64)];
   const int64_t r = blockIdx.x;
   const float mu = mean[r], rs = rstd[r];
-  float sg = 0.0f, sx = 0.0f;
-  for (int64_t c = threadIdx.x; c < dim; c += NT) {
-    const float g = (float)dy[r * ldy + c] * (w ? (float)w[c] : 1.0f);
-    sg += g;
-    sx = fmaf(g, ((float)x[r * ldx + c] - mu) * rs, sx);
+  int turn = 0;
+  float s[2] = {0.0f, 0.0f}, v[GR], g[GR], wv[GR];
+  auto load = [&](int64_t c) {
+    load_n<T, GR>(v, x + r * ldx + c, dim - c);
+    load_n<T, GR>(g, dy + r * ldy + c, dim - c);
+    if (w) load_n<W, GR>(wv, w + c, dim - c);
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+      v[i] = (v[i] - mu) * rs;
+      if (w) g[i] *= wv[i];
+    }
+  };
+  for (int64_t c = threadIdx.x * GR; c < dim; c += LONG * GR) {
+    load(c);
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+      s[0] += g[i];
+      s[1] = fmaf(g[i], v[i], s[1]);
+    }
   }
-  sg = block_sum(sg, sh) / (float)dim;
-  sx = block_sum(sx, sh) / (float)dim;
-  for (int64_t c = threadIdx.x; c < dim; c += NT) {
-    const float g = (float)dy[r * ldy + c] * (w ? (float)w[c] : 1.0f);
-    const float xh = ((float)x[r * ldx + c] - mu) * rs;
-    dx[r * dim + c] = (T)(rs * (g - sg - xh * sx));
+  row_sums<LONG>(s, sh, turn);
+  const float sg = s[0] / (float)dim, sx = s[1] / (float)dim;
+  for (int64_t c = threadIdx.x * GR; c < dim; c += LONG * GR) {
+    load(c);
+#pragma unroll
+    for (int i = 0; i < GR; ++i) v[i] = rs * (g[i] - sg - v[i] * sx);
+    store_n<T, GR>(dx + r * dim + c, v, dim - c);
   }
 }
 
-// one thread per column
-template <class T, class W>
-__global__ __launch_bounds__(NT) void layer_norm_dw_kernel(const T* dy, int64_t ldy, const T* x, int64_t ldx,
-                                                           const float* mean, const float* rstd, W* dw, W* db,
-                                                           int64_t rows, int64_t dim) {
-  const int64_t c = (int64_t)blockIdx.x * NT + threadIdx.x;
+// part as in layer_norm_bwd_kernel: workgroup (c, p) sums rows p, p + parts, ... of its 256 groups
+template <class T>
+__global__ __launch_bounds__(256) void layer_norm_dw_long_kernel(const T* dy, int64_t ldy, const T* x, int64_t ldx,
+                                                                 const float* mean, const float* rstd, float* part,
+                                                                 int64_t rows, int64_t dim) {
+  constexpr int GR = GROUP<T>;
+  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * GR;
   if (c >= dim) return;
-  float a = 0.0f, s = 0.0f;
-  for (int64_t r = 0; r < rows; ++r) {
-    const float g = (float)dy[r * ldy + c];
-    a = fmaf(g, ((float)x[r * ldx + c] - mean[r]) * rstd[r], a);
-    s += g;
+  float aw[GR] = {}, ab[GR] = {}, v[GR], d[GR];
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    load_n<T, GR>(v, x + r * ldx + c, dim - c);
+    load_n<T, GR>(d, dy + r * ldy + c, dim - c);
+    const float mu = mean[r], rs = rstd[r];
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+      aw[i] = fmaf(d[i], (v[i] - mu) * rs, aw[i]);
+      ab[i] += d[i];
+    }
   }
-  if (dw) dw[c] = (W)a;
-  if (db) db[c] = (W)s;
+  float* p = part + (int64_t)blockIdx.y * 2 * dim + c;
+  store_n<float, GR>(p, aw, dim - c);
+  store_n<float, GR>(p + dim, ab, dim - c);
 }
 
 template <class F>
@@ -95,11 +363,41 @@ int with_types(int dtype, int wdtype, F&& f) {
   });
 }
 
+// The shape for rows of `dim`: the fewest lanes with at most 2 groups each up to a wave, then
+// workgroups of 256 (up to 4) and of 1024.  False: too long.
+template <class T, class F>
+bool with_shape(int64_t dim, F&& f) {
+  const int64_t g = cdiv(dim, GROUP<T>);
+  if (g <= 16) f(Shape<16, 1>{});
+  else if (g <= 64) f(Shape<64, 1>{});
+  else if (g <= 128) f(Shape<64, 2>{});
+  else if (g <= 256) f(Shape<256, 1>{});
+  else if (g <= 512) f(Shape<256, 2>{});
+  else if (g <= 1024) f(Shape<256, 4>{});
+  else if (g <= 2048) f(Shape<1024, 2>{});
+  else if (g <= 4096) f(Shape<1024, 4>{});
+  else return false;
+  return true;
+}
+
+constexpr int MAX_PARTS = 512;  // partial rows of dw and db: two workgroups of 256 a CU
+
+// workgroups of a launch over all rows
+template <class S>
+unsigned row_blocks(int64_t rows, int64_t most) {
+  const int64_t n = cdiv(rows, S::ROWS);
+  return (unsigned)(n < most ? n : most);
+}
+
 int check(int64_t rows, int64_t dim, int64_t ld) {
   QNN_REQUIRE(rows >= 0 && rows < (1LL << 31), "rows: 0 to 2^31 - 1");
   QNN_REQUIRE(dim >= 1 && dim < (1LL << 31), "dim: 1 to 2^31 - 1");
   QNN_REQUIRE(ld >= dim, "a row stride is shorter than the row");
   return QNN_OK;
+}
+
+int64_t work_bytes_of(int64_t rows, int64_t dim) {
+  return (rows < MAX_PARTS ? rows : MAX_PARTS) * 2 * dim * (int64_t)sizeof(float);
 }
 
 }  // namespace
@@ -119,8 +417,15 @@ int qnn_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b,
   return with_types(dtype, wdtype, [&](auto t, auto tw) {
     using T = decltype(t);
     using W = decltype(tw);
-    hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W>), dim3((unsigned)rows), dim3(NT), 0, (hipStream_t)stream,
-                       (const T*)x, ldx, (const W*)w, (const W*)b, (T*)y, mean, rstd, dim, eps);
+    hipStream_t s = (hipStream_t)stream;
+    const bool held = with_shape<T>(dim, [&](auto shape) {
+      using S = decltype(shape);
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, S>), dim3(row_blocks<S>(rows, 2048)), dim3(S::NT), 0, s,
+                         (const T*)x, ldx, (const W*)w, (const W*)b, (T*)y, mean, rstd, rows, (int)dim, eps);
+    });
+    if (!held)
+      hipLaunchKernelGGL((layer_norm_fwd_long_kernel<T, W>), dim3((unsigned)rows), dim3(LONG), 0, s, (const T*)x, ldx,
+                         (const W*)w, (const W*)b, (T*)y, mean, rstd, dim, eps);
     QNN_LAUNCH_CHECK("qnn_layer_norm_fwd");
     return (int)QNN_OK;
   });
@@ -129,7 +434,7 @@ int qnn_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b,
 int qnn_layer_norm_bwd_work(int64_t rows, int64_t dim, int dtype, int64_t* bytes) {
   if (int rc = check(rows, dim, dim)) return rc;
   QNN_REQUIRE(bytes, "null pointer");
-  *bytes = 0;
+  *bytes = work_bytes_of(rows, dim);
   return QNN_OK;
 }
 
@@ -139,18 +444,37 @@ int qnn_layer_norm_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, 
   if (int rc = check(rows, dim, ldx)) return rc;
   if (int rc = check(rows, dim, ldy)) return rc;
   QNN_REQUIRE(rows == 0 || (dy && x && mean && rstd), "null pointer");
+  const bool sums = dw || db;
+  QNN_REQUIRE(!sums || rows == 0 || (work && work_bytes >= work_bytes_of(rows, dim)),
+              "work: at least what qnn_layer_norm_bwd_work says");
   return with_types(dtype, wdtype, [&](auto t, auto tw) {
     using T = decltype(t);
     using W = decltype(tw);
     hipStream_t s = (hipStream_t)stream;
-    if (dx && rows > 0)
-      hipLaunchKernelGGL((layer_norm_dx_kernel<T, W>), dim3((unsigned)rows), dim3(NT), 0, s, (const T*)dy, ldy,
-                         (const T*)x, ldx, (const W*)w, mean, rstd, (T*)dx, dim);
-    QNN_LAUNCH_CHECK("qnn_layer_norm_bwd");
-    if (dw || db)
-      hipLaunchKernelGGL((layer_norm_dw_kernel<T, W>), dim3((unsigned)cdiv(dim, NT)), dim3(NT), 0, s, (const T*)dy,
-                         ldy, (const T*)x, ldx, mean, rstd, (W*)dw, (W*)db, rows, dim);
-    QNN_LAUNCH_CHECK("qnn_layer_norm_bwd");
+    float* part = sums ? (float*)work : nullptr;
+    unsigned parts = 0;
+    if (rows > 0 && (dx || sums)) {
+      const bool held = with_shape<T>(dim, [&](auto shape) {
+        using S = decltype(shape);
+        parts = row_blocks<S>(rows, MAX_PARTS);
+        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, S>), dim3(parts), dim3(S::NT), 0, s, (const T*)dy, ldy,
+                           (const T*)x, ldx, (const W*)w, mean, rstd, (T*)dx, part, rows, (int)dim);
+      });
+      if (!held && dx)
+        hipLaunchKernelGGL((layer_norm_dx_long_kernel<T, W>), dim3((unsigned)rows), dim3(LONG), 0, s, (const T*)dy,
+                           ldy, (const T*)x, ldx, (const W*)w, mean, rstd, (T*)dx, dim);
+      if (!held && sums) {
+        parts = (unsigned)(rows < 64 ? rows : 64);
+        hipLaunchKernelGGL((layer_norm_dw_long_kernel<T>), dim3((unsigned)cdiv(dim, 256 * GROUP<T>), parts), dim3(256),
+                           0, s, (const T*)dy, ldy, (const T*)x, ldx, mean, rstd, part, rows, dim);
+      }
+      QNN_LAUNCH_CHECK("qnn_layer_norm_bwd");
+    }
+    if (sums) {
+      hipLaunchKernelGGL((layer_norm_join_kernel<W>), dim3((unsigned)cdiv(2 * dim, 64)), dim3(1024), 0, s, part,
+                         (int)parts, (int)dim, (W*)dw, (W*)db);
+      QNN_LAUNCH_CHECK("qnn_layer_norm_bwd");
+    }
     return (int)QNN_OK;
   });
 }

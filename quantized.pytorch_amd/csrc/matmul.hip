@@ -15,7 +15,6 @@ struct Epilogue {
   void* y;
   void* slope;
   int act;
-  bool whole;  // every row of y, res and slope begins on a 16-byte boundary, bias too, n % 8 == 0
 };
 
 template <class T>
@@ -23,13 +22,13 @@ __device__ __forceinline__ void finish8(float (&z)[8], const Epilogue& e, int64_
   const int64_t left = n - col;
   if (e.bias) {
     float b[8];
-    load_n<T, 8>(b, (const T*)e.bias + col, left, e.whole);
+    load_n<T, 8>(b, (const T*)e.bias + col, left);
 #pragma unroll
     for (int i = 0; i < 8; ++i) z[i] += b[i];
   }
   if (e.res) {
     float b[8];
-    load_n<T, 8>(b, (const T*)e.res + row * e.ldr + col, left, e.whole);
+    load_n<T, 8>(b, (const T*)e.res + row * e.ldr + col, left);
 #pragma unroll
     for (int i = 0; i < 8; ++i) z[i] += b[i];
   }
@@ -48,23 +47,16 @@ __device__ __forceinline__ void finish8(float (&z)[8], const Epilogue& e, int64_
     for (int i = 0; i < 8; ++i) gelu_f(z[i], z[i], d[i]);
     if (e.slope) {
       if constexpr (sizeof(T) == 4) {
-        store_n<float, 8>((float*)e.slope + row * n + col, d, left, e.whole);
+        store_n<float, 8>((float*)e.slope + row * n + col, d, left);
       } else {
-        int16_t* p = (int16_t*)e.slope + row * n + col;
         Vec<int16_t, 8> q;
 #pragma unroll
         for (int i = 0; i < 8; ++i) q.v[i] = slope_pack(d[i]);
-        if (e.whole) {
-          *reinterpret_cast<Vec<int16_t, 8>*>(p) = q;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < left) p[i] = q.v[i];
-        }
+        store_group((int16_t*)e.slope + row * n + col, q, left);
       }
     }
   }
-  store_n<T, 8>((T*)e.y + row * n + col, z, left, e.whole);
+  store_n<T, 8>((T*)e.y + row * n + col, z, left);
 }
 
 // c[i][j] = sum over k of a(i, k) b(j, k), a and b by element strides
@@ -164,7 +156,7 @@ int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
   QNN_REQUIRE(x && w && y, "null pointer");
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const Epilogue e = {bias, res, ldr, y, slope, act, false};
+    const Epilogue e = {bias, res, ldr, y, slope, act};
     return matmul<T>(x, ldx, 1, w, ldw, 1, m, n, k, e, (hipStream_t)stream);
   });
 }
@@ -196,7 +188,7 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
       g = (const T*)dz;
       ldg = n;
     }
-    const Epilogue none = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE, false};
+    const Epilogue none = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE};
     if (dx && m > 0)
       if (int rc = matmul<T>(g, ldg, 1, w, 1, ldw, m, k, n, none, s)) return rc;
     Epilogue to_dw = none;
