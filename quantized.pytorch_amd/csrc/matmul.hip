@@ -59,75 +59,556 @@ __device__ __forceinline__ void finish8(float (&z)[8], const Epilogue& e, int64_
   store_n<T, 8>((T*)e.y + row * n + col, z, left);
 }
 
-// c[i][j] = sum over k of a(i, k) b(j, k), a and b by element strides
-template <class T>
-__global__ __launch_bounds__(256) void matmul_kernel(const T* a, int64_t ai, int64_t ak, const T* b, int64_t bj,
-                                                     int64_t bk, int64_t m, int64_t n, int64_t k, Epilogue e) {
-  constexpr int BM = 32, BN = 64, BK = 32;
-  __shared__ float sa[BM][BK + 1], sb[BN][BK + 1];
-  const int64_t tn = (n + BN - 1) / BN, i0 = blockIdx.x / tn * BM, j0 = blockIdx.x % tn * BN;
-  const int t = threadIdx.x, ti = t / 8, tj = t % 8 * 8;
-  float acc[8] = {};
-  for (int64_t k0 = 0; k0 < k; k0 += BK) {
-    __syncthreads();
-    for (int u = t; u < BM * BK; u += 256) {
-      const int i = ak == 1 ? u / BK : u % BM, kk = ak == 1 ? u % BK : u / BM;
-      sa[i][kk] = i0 + i < m && k0 + kk < k ? (float)a[(i0 + i) * ai + (k0 + kk) * ak] : 0.0f;
+// ---------------------------------------------------------------------------- the tiled product
+// c[i][j] = sum over k of a(i, k) b(j, k).  An operand is DENSE in k ([rows][k], as x and w in the
+// forward pass) or not ([k][rows], as both of dz^T x): then its rows are what is contiguous in memory.
+//
+// A workgroup of WM x WN waves computes a (16 TM WM) x (16 TN WN) tile, a wave (16 TM) x (16 TN) of it
+// in 16x16 MFMAs.  k advances in stages of 64 bytes (32 elements of 16 bits, 16 of 32) through a ring
+// of 4 LDS slots that direct loads fill (buffer_load ... lds, 16 bytes a lane), three stages ahead; a
+// wave reads the fragments of the next stage from LDS while the MFMAs work on the present one's, so
+// there is one barrier a stage and no wait for LDS in it.  A fragment is 16 bytes a lane: row lane % 16,
+// the (lane / 16)-th quarter of the stage -- one 16x16x32 MFMA of 16-bit types, four 16x16x4 of fp32,
+// each k in the same place on both sides.
+//   DENSE tile in LDS: [rows][64 bytes], 16-byte chunks XORed by row bits 2-3, read by ds_read_b128.
+//   Else: [k of the stage][rows], granules of 16 rows XORed by the bits of k in which the lanes of a
+//   read differ; 16-bit types are turned around by ds_read_b64_tr_b16, fp32 read by ds_read_b32.
+// The XOR is made on the side of the load's source, since a direct load fills LDS in lane order.
+// Rows past the matrix and k past its end are loaded from an offset past the buffer's size, which
+// fills LDS with zeros; stages past the last are such loads too, so the counts of loads in flight hold.
+constexpr uint32_t PAST = 0x80000000u;  // a buffer offset that is past every size below
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // at most N of this wave's loads in flight, no LDS read
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+typedef __attribute__((address_space(3))) void* lds_t;
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4* lds_s4_t;
+
+struct Operand {
+  const void* p;
+  int64_t ld;    // elements between rows of the matrix in memory
+  int64_t rows;  // of the product's operand: m or n
+};
+
+// R rows of an operand in a workgroup of W waves: its loads into LDS and its fragments from there.
+template <class T, bool DENSE, int R, int W>
+struct Side {
+  static constexpr int ES = (int)sizeof(T), KE = 64 / ES, BYTES = R * 64, LOADS = R / 16 / W;
+  static_assert(R % (16 * W) == 0, "a wave loads whole KiB");
+  static constexpr int GRAN = 16 * ES, GMASK = R / 16 < 8 ? R / 16 - 1 : 7;  // bytes, and the XOR's bits
+
+  static __device__ __forceinline__ int spread(int k) {  // what a granule's index is XORed with, not DENSE
+    if constexpr (ES == 2) return ((k & 3) | (k >> 3 & 1) << 2) & GMASK;
+    else return k >> 2 & 3;
+  }
+
+  uint32_t off[LOADS];  // this lane's byte offsets from the tile's corner, PAST outside the rows
+  int kat[LOADS];       // its k in the stage (elements)
+  const char* base;
+  int64_t step;
+
+  // from row i0 and element k0 on
+  __device__ __forceinline__ void begin(const Operand& o, int64_t i0, int64_t k0, int wave, int lane) {
+    if constexpr (DENSE) {
+      base = (const char*)o.p + (i0 * o.ld + k0) * ES;
+      step = 64;
+    } else {
+      base = (const char*)o.p + (k0 * o.ld + i0) * ES;
+      step = KE * o.ld * ES;
     }
-    for (int u = t; u < BN * BK; u += 256) {
-      const int j = bk == 1 ? u / BK : u % BN, kk = bk == 1 ? u % BK : u / BN;
-      sb[j][kk] = j0 + j < n && k0 + kk < k ? (float)b[(j0 + j) * bj + (k0 + kk) * bk] : 0.0f;
-    }
-    __syncthreads();
-    for (int kk = 0; kk < BK; ++kk) {
-      const float v = sa[ti][kk];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = fmaf(v, sb[tj + j][kk], acc[j]);
+    for (int j = 0; j < LOADS; ++j) {
+      const int at = (wave * LOADS + j) * 1024 + lane * 16;
+      if constexpr (DENSE) {
+        const int row = at / 64, chunk = at / 16 % 4 ^ (row >> 2 & 3);
+        kat[j] = chunk * 16 / ES;
+        off[j] = i0 + row < o.rows ? (uint32_t)(row * (int)o.ld * ES + chunk * 16) : PAST;
+      } else {
+        const int k = at / (R * ES), in = at % (R * ES);
+        const int col = ((in / GRAN ^ spread(k)) * GRAN + in % GRAN) / ES;
+        kat[j] = k;
+        off[j] = i0 + col < o.rows ? (uint32_t)((k * (int)o.ld + col) * ES) : PAST;
+      }
     }
   }
-  if (i0 + ti < m && j0 + tj < n) finish8<T>(acc, e, i0 + ti, j0 + tj, n);
+  // the next stage, of which `left` elements of k are there, into the slot at lds
+  __device__ __forceinline__ void load(char* lds, int left, int wave) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass drops a kernel that names the resource type, without a word
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)(lds + (wave * LOADS + j) * 1024), 16,
+                                               kat[j] < left ? off[j] : PAST, 0, 0, 0);
+#endif
+    base += step;
+  }
+  // fragment f (rows 16 f ... of the wave's, which begin at row r0)
+  static __device__ __forceinline__ int place(int r0, int lane) {
+    if constexpr (DENSE) {
+      const int row = lane & 15;
+      return (r0 + row) * 64 + ((lane >> 4) ^ (row >> 2 & 3)) * 16;
+    } else if constexpr (ES == 2) {
+      return ((lane >> 4) * 8 + (lane >> 2 & 3)) * R * ES + (lane & 3) * 8;
+    } else {
+      return (lane >> 4) * 4 * R * ES + (lane & 15) * 4;
+    }
+  }
+  static __device__ __forceinline__ f4 fragment(char* lds, int at, int r0, int f, int lane) {
+    if constexpr (DENSE) {
+      return *reinterpret_cast<const f4*>(lds + at + f * 1024);
+    } else if constexpr (ES == 2) {
+      const int h = spread((lane >> 4) * 8 + (lane >> 2 & 3));
+      char* p = lds + at + ((r0 / 16 + f) ^ h) * GRAN;
+      union {
+        s4 s[2];
+        f4 v;
+      } u;
+      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)p);
+      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)(p + 4 * R * ES));
+      return u.v;
+    } else {
+      const int h = spread((lane >> 4) * 4);
+      const char* p = lds + at + ((r0 / 16 + f) ^ h) * GRAN;
+      f4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float*>(p + j * R * ES);
+      return v;
+    }
+  }
+};
+
+// acc += the 16x16 product of two fragments; the first's rows become the lane's four neighbours
+template <class T>
+__device__ __forceinline__ f4 mma(f4 a, f4 b, f4 acc) {
+  if constexpr (std::is_same_v<T, bf16>) {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), acc, 0, 0, 0);
+  } else if constexpr (std::is_same_v<T, f16>) {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), acc, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
+    return acc;
+  }
+}
+
+// Where a tile's sums go: through the epilogue, or (splits > 1) as they are into part[split][m][ldp].
+struct Tiles {
+  int64_t m, n, k;
+  int tm, tn;        // tiles
+  int splits;
+  int64_t span;      // elements of k in a split, a whole number of stages
+  float* part;
+  int64_t ldp;
+};
+
+// Workgroup -> (split, tile row, tile column).  The card deals workgroups out to its 8 XCDs in turn; each
+// XCD gets a run of neighbouring tiles, 8 tile rows at a time, so that the panels they share meet in
+// its L2.
+__device__ __forceinline__ void tile_of(const Tiles& t, int& split, int& ti, int& tj) {
+  const int all = t.tm * t.tn * t.splits, id = blockIdx.x, x = id & 7, q = all >> 3, r = all & 7;
+  const int lin = x * q + (x < r ? x : r) + (id >> 3);
+  const int tiles = t.tm * t.tn;
+  split = lin / tiles;
+  const int u = lin - split * tiles, band = u / (8 * t.tn), in = u - band * 8 * t.tn;
+  const int rows = t.tm - band * 8 < 8 ? t.tm - band * 8 : 8;
+  tj = in / rows;
+  ti = band * 8 + in - tj * rows;
+}
+
+template <int WM_, int WN_, int TM_, int TN_, int EU_>
+struct Cfg {
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, W = WM * WN, NT = 64 * W, EU = EU_;
+  static constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN, SLOT = (BM + BN) * 64, LDS = 4 * SLOT;
+};
+
+template <class T, bool AD, bool BD, class C>
+__global__ __launch_bounds__(C::NT, C::EU) void matmul_kernel(Operand a, Operand b, Tiles t, Epilogue e) {
+  using A = Side<T, AD, C::BM, C::W>;
+  using B = Side<T, BD, C::BN, C::W>;
+  constexpr int TM = C::TM, TN = C::TN, KE = A::KE, P = A::LOADS + B::LOADS;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int split, ti, tj;
+  tile_of(t, split, ti, tj);
+  const int64_t i0 = (int64_t)ti * C::BM, j0 = (int64_t)tj * C::BN, k0 = split * t.span;
+  int left = (int)(t.k - k0 < t.span ? t.k - k0 : t.span);
+  const int stages = (left + KE - 1) / KE;
+  const int ri = wave / C::WN * 16 * TM, rj = wave % C::WN * 16 * TN;  // this wave's corner in the tile
+
+  A sa;
+  B sb;
+  sa.begin(a, i0, k0, wave, lane);
+  sb.begin(b, j0, k0, wave, lane);
+  auto load = [&](int slot) {
+    sa.load(lds + slot * C::SLOT, left, wave);
+    sb.load(lds + slot * C::SLOT + A::BYTES, left, wave);
+    left -= KE;
+  };
+  const int pa = A::place(ri, lane), pb = B::place(rj, lane);
+  f4 fa[2][TM], fb[2][TN], acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+  auto fetch = [&](int slot, int to) {
+    char* s = lds + slot * C::SLOT;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fa[to][i] = A::fragment(s, pa, ri, i, lane);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[to][j] = B::fragment(s + A::BYTES, pb, rj, j, lane);
+  };
+#pragma unroll
+  for (int s = 0; s < 4; ++s) load(s);
+  wait_loads<3 * P>();
+  __builtin_amdgcn_s_barrier();
+  fetch(0, 0);
+  // step s: stage s is in registers, s + 1 to s + 3 in LDS or on their way
+  auto step = [&](int s, auto cur) {
+    constexpr int C0 = decltype(cur)::value;
+    wait_loads<2 * P>();  // stage s + 1 has landed, and stage s has left its slot
+    __builtin_amdgcn_s_barrier();
+    load(s & 3);  // stage s + 4
+    fetch((s + 1) & 3, C0 ^ 1);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = mma<T>(fb[C0][j], fa[C0][i], acc[i][j]);
+  };
+  int s = 0;
+  for (; s + 1 < stages; s += 2) {
+    step(s, std::integral_constant<int, 0>{});
+    step(s + 1, std::integral_constant<int, 1>{});
+  }
+  if (s < stages) step(s, std::integral_constant<int, 0>{});
+  wait_loads<0>();
+  __syncthreads();
+
+  // acc[i][j]: row 16 i + lane % 16, columns 16 j + lane / 16 * 4 ... + 3.  A wave turns 16 rows at a
+  // time around in LDS of its own, so that a lane has 8 neighbouring columns and a row's are together.
+  constexpr int COLS = 16 * TN, STRIDE = COLS + 4, PER = COLS / 8;
+  float* mine = reinterpret_cast<float*>(lds) + wave * 16 * STRIDE;
+  static_assert(C::W * 16 * STRIDE * 4 <= C::LDS, "the ring holds the turned rows");
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      *reinterpret_cast<f4*>(mine + (lane & 15) * STRIDE + 16 * j + (lane >> 4) * 4) = acc[i][j];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int u = 0; u < 16 * PER / 64; ++u) {
+      const int row = (u * 64 + lane) / PER, col = (u * 64 + lane) % PER * 8;
+      float z[8];
+      *reinterpret_cast<f4*>(z) = *reinterpret_cast<const f4*>(mine + row * STRIDE + col);
+      *reinterpret_cast<f4*>(z + 4) = *reinterpret_cast<const f4*>(mine + row * STRIDE + col + 4);
+      const int64_t gi = i0 + ri + 16 * i + row, gj = j0 + rj + col;
+      if (gi < t.m && gj < t.n) {
+        if (t.splits > 1)
+          store_n<float, 8>(t.part + (split * t.m + gi) * t.ldp + gj, z, t.ldp - gj);
+        else
+          finish8<T>(z, e, gi, gj, t.n);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The splits' sums, in their order, through the epilogue: 8 columns a thread.
+template <class T>
+__global__ __launch_bounds__(256) void matmul_join_kernel(const float* part, int splits, int64_t m, int64_t n,
+                                                          int64_t ldp, Epilogue e) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, per = ldp / 8, row = at / per, col = at % per * 8;
+  if (row >= m) return;
+  float z[8], v[8];
+  load_n<float, 8>(z, part + row * ldp + col, 8);
+  for (int s = 1; s < splits; ++s) {
+    load_n<float, 8>(v, part + (s * m + row) * ldp + col, 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] += v[i];
+  }
+  finish8<T>(z, e, row, col, n);
+}
+
+// ------------------------------------------------------------------------- few rows: the weight is all
+// y for up to 16 rows of x, both operands dense in k.  A workgroup has 16 outputs; its waves share
+// k between them in turns of 128 bytes a row, loads going straight into the fragments, and join
+// their sums in LDS in a fixed order.  Bound by the weight's way from HBM: the launch's waves have
+// most of it in flight at once.
+template <class T, int W>
+__global__ __launch_bounds__(64 * W) void few_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int m,
+                                                          int64_t n, int64_t k, Epilogue e) {
+  constexpr int GR = GROUP<T>, TURN = 8 * GR, U = 4;  // elements of a row a turn; turns in flight
+  __shared__ f4 sums[W][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15;
+  const int64_t j0 = (int64_t)blockIdx.x * 16;
+  const bool wi = j0 + row < n, xi = row < m;
+  const T* wp = w + (wi ? j0 + row : 0) * ldw;
+  const T* xp = x + (xi ? row : 0) * ldx;
+  f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto frag = [&](const T* p, bool there, int64_t c) {
+    const Vec<T, GR> v = load_group(p + c, there ? k - c : 0);
+    f4 f;
+    __builtin_memcpy(&f, &v, 16);
+    return f;
+  };
+  for (int64_t c0 = (int64_t)wave * TURN; c0 < k; c0 += (int64_t)W * TURN * U) {
+    f4 fw[U][2], fx[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t c = c0 + (int64_t)u * W * TURN + (lane >> 4) * 2 * GR;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        fw[u][h] = frag(wp, wi, c + h * GR);
+        fx[u][h] = frag(xp, xi, c + h * GR);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) acc = mma<T>(fw[u][h], fx[u][h], acc);
+  }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  // thread: row t / 2, 8 columns from 8 (t % 2); lane (c / 4) 16 + row of a wave has columns c ... c + 3
+  const int t = threadIdx.x;
+  if (t >= 2 * m) return;
+  const int r = t >> 1, c = (t & 1) * 8;
+  if (j0 + c >= n) return;
+  float z[8] = {};
+  for (int v = 0; v < W; ++v) {
+    const f4 lo = sums[v][(c / 4) * 16 + r], hi = sums[v][(c / 4 + 1) * 16 + r];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] += lo[i], z[4 + i] += hi[i];
+  }
+  finish8<T>(z, e, r, j0 + c, n);
+}
+
+// ------------------------------------------------------------------------------ rows on boundaries
+// A matrix whose rows are no whole number of 16-byte groups, with rows of ldo that are, zeros behind
+// them: what the tiled product's loads take.
+template <class T>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const T* x, int64_t ld, int64_t rows, int64_t cols, T* out,
+                                                       int64_t ldo) {
+  constexpr int GR = GROUP<T>;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, per = ldo / GR, row = at / per, c = at % per * GR;
+  if (row >= rows) return;
+  store_group(out + row * ldo + c, load_group(x + row * ld + c, cols - c), GR);
 }
 
 template <class T>
-int matmul(const void* a, int64_t ai, int64_t ak, const void* b, int64_t bj, int64_t bk, int64_t m, int64_t n,
-           int64_t k, const Epilogue& e, hipStream_t s) {
-  hipLaunchKernelGGL((matmul_kernel<T>), dim3((unsigned)(cdiv(m, 32) * cdiv(n, 64))), dim3(256), 0, s, (const T*)a, ai,
-                     ak, (const T*)b, bj, bk, m, n, k, e);
+__global__ __launch_bounds__(256) void zero_kernel(T* p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = (T)0.0f;
+}
+
+// -------------------------------------------------------------------------- dz, and the bias's gradient
+// dz = dy act'(z), and this strip of rows' sums of it: 64 lanes with 8 columns each, 4 rows at a time.
+// part: [strips][n] (null: not wanted); dz null: none is to be written (dz is dy).
+template <class T>
+__global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, int64_t ldy, const void* slope, T* dz,
+                                                        float* part, int64_t m, int64_t n, int act, int chunks,
+                                                        int64_t strip) {
+  __shared__ float sh[4][64][9];
+  const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
+  const int64_t c = ((int64_t)(blockIdx.x % chunks) * 64 + lane) * 8, left = n - c;
+  const int64_t s = blockIdx.x / chunks, r1 = (s + 1) * strip < m ? (s + 1) * strip : m;
+  float sum[8] = {};
+  if (left > 0) {
+#pragma unroll 4
+    for (int64_t r = s * strip + sub; r < r1; r += 4) {
+      float g[8];
+      load_n<T, 8>(g, dy + r * ldy + c, left);
+      if (act == QNN_ACT_RELU) {
+        const unsigned on = ((const uint8_t*)slope)[r * ((n + 7) / 8) + c / 8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = on >> i & 1 ? g[i] : 0.0f;
+      } else if (act == QNN_ACT_GELU) {
+        if constexpr (sizeof(T) == 4) {
+          float d[8];
+          load_n<float, 8>(d, (const float*)slope + r * n + c, left);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] *= d[i];
+        } else {
+          const Vec<int16_t, 8> q = load_group((const int16_t*)slope + r * n + c, left);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] *= slope_unpack(q.v[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        g[i] = (float)(T)g[i];  // db is the sum of dz as it is written
+        sum[i] += g[i];
+      }
+      if (dz) store_n<T, 8>(dz + r * n + c, g, left);
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sh[sub][lane][i] = sum[i];
+  __syncthreads();
+  if (sub == 0 && left > 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = sh[0][lane][i] + sh[1][lane][i] + sh[2][lane][i] + sh[3][lane][i];
+    store_n<float, 8>(part + s * n + c, sum, left);
+  }
+}
+
+// db from the strips' sums: 64 columns a workgroup, 4 threads a column
+template <class T>
+__global__ __launch_bounds__(256) void linear_db_kernel(const float* part, int strips, T* db, int64_t n) {
+  __shared__ float sh[4][64];
+  const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.0f;
+  if (c < n)
+#pragma unroll 8
+    for (int p = sub; p < strips; p += 4) s += part[p * n + c];
+  sh[sub][lane] = s;
+  __syncthreads();
+  if (sub == 0 && c < n) db[c] = (T)(sh[0][lane] + sh[1][lane] + sh[2][lane] + sh[3][lane]);
+}
+
+// ---------------------------------------------------------------------------------------- host side
+using Big = Cfg<2, 4, 8, 4, 2>;     // 256 x 256, one workgroup a CU
+using Middle = Cfg<2, 2, 4, 4, 2>;  // 128 x 128
+using Small = Cfg<2, 2, 2, 2, 4>;   // 64 x 64
+
+struct Plan {
+  int cfg;      // 0 Big, 1 Middle, 2 Small
+  int splits;
+  int64_t span;  // elements of k in a split
+  int64_t ldp;
+  int64_t part_bytes;
+};
+
+int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
+
+// The tile and the splits of k of one product.
+Plan plan_of(int64_t m, int64_t n, int64_t k, int dtype) {
+  const int64_t ke = 64 / type_bytes(dtype), stages = cdiv(k, ke);
+  auto tiles = [&](int64_t b) { return cdiv(m, b) * cdiv(n, b); };
+  Plan p = {};
+  if (dtype != QNN_F32 && tiles(256) >= 192) p.cfg = 0;
+  else if (tiles(128) >= 192) p.cfg = 1;
+  else p.cfg = 2;
+  const int64_t have = tiles(p.cfg == 0 ? 256 : p.cfg == 1 ? 128 : 64);
+  int64_t s = 1;
+  if (have < 256) s = cdiv(512, have);
+  if (s > stages / 8) s = stages / 8;
+  if (s > 32) s = 32;
+  if (s < 1) s = 1;
+  const int64_t each = cdiv(stages, s);
+  p.splits = (int)cdiv(stages, each);
+  p.span = each * ke;
+  p.ldp = up(n, 8);
+  p.part_bytes = p.splits > 1 ? p.splits * m * p.ldp * 4 : 0;
+  return p;
+}
+
+constexpr int FEW = 16;  // rows of x that few_rows_kernel takes
+
+template <class T, bool AD, bool BD, class C>
+int launch(const Operand& a, const Operand& b, const Plan& p, int64_t m, int64_t n, int64_t k, float* part,
+           const Epilogue& e, hipStream_t s) {
+  const int64_t tm = cdiv(m, C::BM), tn = cdiv(n, C::BN);
+  QNN_REQUIRE(tm * tn * p.splits < (1LL << 31) && tn < (1LL << 27), "too many tiles for one call");
+  const Tiles t = {m, n, k, (int)tm, (int)tn, p.splits, p.span, part, p.ldp};
+  if constexpr (C::LDS > 65536) {
+    static std::atomic<uint64_t> told{0};  // devices whose runtime knows that this kernel takes more than 64 KiB
+    int dev = 0;
+    if (hipError_t er = hipGetDevice(&dev); er != hipSuccess) return hip_check(er, "hipGetDevice");
+    if (dev >= 64 || !(told.load(std::memory_order_relaxed) >> dev & 1)) {
+      if (hipError_t er = hipFuncSetAttribute((const void*)&matmul_kernel<T, AD, BD, C>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+          er != hipSuccess)
+        return hip_check(er, "hipFuncSetAttribute");
+      if (dev < 64) told.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+  }
+  hipLaunchKernelGGL((matmul_kernel<T, AD, BD, C>), dim3((unsigned)(tm * tn * p.splits)), dim3(C::NT), C::LDS, s, a, b, t, e);
   QNN_LAUNCH_CHECK("matmul_kernel");
+  if (p.splits > 1) {
+    hipLaunchKernelGGL((matmul_join_kernel<T>), dim3((unsigned)cdiv(m * (p.ldp / 8), 256)), dim3(256), 0, s, part,
+                       p.splits, m, n, p.ldp, e);
+    QNN_LAUNCH_CHECK("matmul_join_kernel");
+  }
   return QNN_OK;
 }
 
-// dz = dy act'(z)
-template <class T>
-__global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, int64_t ldy, const void* slope, T* dz, int64_t m,
-                                                        int64_t n, int act) {
-  const int64_t chunks = (n + 255) / 256, row = blockIdx.x / chunks;
-  const int64_t c = blockIdx.x % chunks * 256 + threadIdx.x;
-  if (c >= n) return;
-  const float g = (float)dy[row * ldy + c];
-  float v;
-  if (act == QNN_ACT_RELU)
-    v = ((const uint8_t*)slope)[row * ((n + 7) / 8) + c / 8] >> (c & 7) & 1 ? g : 0.0f;
-  else if constexpr (sizeof(T) == 4)
-    v = g * ((const float*)slope)[row * n + c];
-  else
-    v = g * slope_unpack(((const int16_t*)slope)[row * n + c]);
-  dz[row * n + c] = (T)v;
+// c = a b^T; part: scratch of plan_of(m, n, k).part_bytes
+template <class T, bool AD, bool BD>
+int matmul(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m, int64_t n, int64_t k, void* part,
+           const Epilogue& e, int dtype, hipStream_t s) {
+  const Plan p = plan_of(m, n, k, dtype);
+  const Operand oa = {a, lda, m}, ob = {b, ldb, n};
+  if constexpr (sizeof(T) == 2)
+    if (p.cfg == 0) return launch<T, AD, BD, Big>(oa, ob, p, m, n, k, (float*)part, e, s);
+  if (p.cfg == 1) return launch<T, AD, BD, Middle>(oa, ob, p, m, n, k, (float*)part, e, s);
+  return launch<T, AD, BD, Small>(oa, ob, p, m, n, k, (float*)part, e, s);
 }
 
+// A matrix as the tiled product takes it: itself, or padded into `room`, of which it takes what it needs.
 template <class T>
-__global__ __launch_bounds__(256) void linear_db_kernel(const T* dz, int64_t ld, T* db, int64_t m, int64_t n) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
-  float a = 0.0f;
-  for (int64_t r = 0; r < m; ++r) a += (float)dz[r * ld + c];
-  db[c] = (T)a;
+int on_boundaries(const void*& p, int64_t& ld, int64_t rows, int64_t cols, char*& room, hipStream_t s) {
+  if (cols % GROUP<T> == 0) return QNN_OK;
+  const int64_t ldo = up(cols, GROUP<T>), blocks = cdiv(rows * (ldo / GROUP<T>), 256);
+  QNN_REQUIRE(blocks < (1LL << 31), "a matrix too large for one call");
+  hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, (const T*)p, ld, rows, cols,
+                     (T*)room, ldo);
+  QNN_LAUNCH_CHECK("pad_rows_kernel");
+  p = room;
+  ld = ldo;
+  room += up(rows * ldo * (int64_t)sizeof(T), 256);
+  return QNN_OK;
 }
 
-int check(int64_t m, int64_t n, int64_t k) {
+int64_t padded_bytes(int64_t rows, int64_t cols, int dtype) {
+  const int64_t size = type_bytes(dtype), g = 16 / size;
+  return cols % g == 0 ? 0 : up(rows * up(cols, g) * size, 256);
+}
+
+int64_t fwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
+  if (m <= FEW) return 0;
+  return padded_bytes(m, k, dtype) + padded_bytes(n, k, dtype) + plan_of(m, n, k, dtype).part_bytes;
+}
+
+struct Strips {
+  int chunks;
+  int64_t n, rows;  // strips, and rows in each
+};
+Strips strips_of(int64_t m, int64_t n) {
+  const int64_t chunks = cdiv(n, 512), want = cdiv(1024, chunks), most = cdiv(m, 16);
+  const int64_t s = want < most ? want : most, rows = cdiv(m, s > 0 ? s : 1);
+  return {(int)chunks, m > 0 ? cdiv(m, rows) : 0, rows};
+}
+
+int64_t bwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
+  if (m == 0) return 0;
+  const int64_t dx = plan_of(m, k, n, dtype).part_bytes, dw = plan_of(n, k, m, dtype).part_bytes;
+  return padded_bytes(m, n, dtype) + padded_bytes(n, k, dtype) + padded_bytes(m, k, dtype) +
+         up(strips_of(m, n).n * n * 4, 256) + (dx > dw ? dx : dw);
+}
+
+constexpr int64_t LONGEST = 1LL << 21;  // of a row stride: offsets inside a tile's rows are 32 bits
+
+int check(int64_t m, int64_t n, int64_t k, int dtype) {
   QNN_REQUIRE(m >= 0 && m < (1LL << 31), "m: 0 to 2^31 - 1");
-  QNN_REQUIRE(n >= 1 && n < (1LL << 31), "n: 1 to 2^31 - 1");
-  QNN_REQUIRE(k >= 1 && k < (1LL << 31), "k: 1 to 2^31 - 1");
+  QNN_REQUIRE(n >= 1 && n <= LONGEST, "n: 1 to 2^21");
+  QNN_REQUIRE(k >= 1 && k <= LONGEST, "k: 1 to 2^21");
+  QNN_REQUIRE(dtype == QNN_F32 || dtype == QNN_BF16 || dtype == QNN_F16, "dtype: QNN_F32, QNN_BF16 or QNN_F16");
+  return QNN_OK;
+}
+
+// A matrix that is read: rows of whole 16-byte groups begin on 16-byte boundaries.
+int check_matrix(const void* p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
+  QNN_REQUIRE(p, "null pointer");
+  QNN_REQUIRE(ld >= cols && ld <= LONGEST, "a row stride is shorter than the row, or over 2^21");
+  const int64_t size = type_bytes(dtype);
+  QNN_REQUIRE(cols * size % 16 != 0 || (aligned16(p) && (rows <= 1 || ld * size % 16 == 0)),
+              "rows of whole 16-byte groups have to begin on 16-byte boundaries");
   return QNN_OK;
 }
 
@@ -140,65 +621,113 @@ using namespace qnn::fl;
 extern "C" {
 
 int qnn_linear_act_fwd_work(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes) {
-  if (int rc = check(m, n, k)) return rc;
+  if (int rc = check(m, n, k, dtype)) return rc;
   QNN_REQUIRE(bytes, "null pointer");
-  *bytes = 0;
+  *bytes = fwd_bytes(m, n, k, dtype);
   return QNN_OK;
 }
 
 int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res,
                        int64_t ldr, void* y, void* slope, int64_t m, int64_t n, int64_t k, int dtype, int act,
                        void* work, int64_t work_bytes, qnn_stream_t stream) {
-  if (int rc = check(m, n, k)) return rc;
+  if (int rc = check(m, n, k, dtype)) return rc;
   QNN_REQUIRE(act >= QNN_ACT_NONE && act <= QNN_ACT_GELU, "act: QNN_ACT_NONE, QNN_ACT_RELU or QNN_ACT_GELU");
-  QNN_REQUIRE(ldx >= k && ldw >= k && (!res || ldr >= n), "a row stride is shorter than the row");
   if (m == 0) return QNN_OK;
-  QNN_REQUIRE(x && w && y, "null pointer");
+  if (int rc = check_matrix(x, ldx, m, k, dtype)) return rc;
+  if (int rc = check_matrix(w, ldw, n, k, dtype)) return rc;
+  QNN_REQUIRE(y, "null pointer");
+  QNN_REQUIRE(!res || ldr >= n, "a row stride is shorter than the row");
+  const int64_t need = fwd_bytes(m, n, k, dtype);
+  QNN_REQUIRE(need == 0 || (work && work_bytes >= need && aligned16(work)),
+              "work: at least what qnn_linear_act_fwd_work says, on a 16-byte boundary");
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
+    hipStream_t s = (hipStream_t)stream;
     const Epilogue e = {bias, res, ldr, y, slope, act};
-    return matmul<T>(x, ldx, 1, w, ldw, 1, m, n, k, e, (hipStream_t)stream);
+    if (m <= FEW) {
+      hipLaunchKernelGGL((few_rows_kernel<T, 16>), dim3((unsigned)cdiv(n, 16)), dim3(1024), 0, s, (const T*)x, ldx,
+                         (const T*)w, ldw, (int)m, n, k, e);
+      QNN_LAUNCH_CHECK("few_rows_kernel");
+      return (int)QNN_OK;
+    }
+    char* room = (char*)work;
+    const void *px = x, *pw = w;
+    int64_t lx = ldx, lw = ldw;
+    if (int rc = on_boundaries<T>(px, lx, m, k, room, s)) return rc;
+    if (int rc = on_boundaries<T>(pw, lw, n, k, room, s)) return rc;
+    return matmul<T, true, true>(px, lx, pw, lw, m, n, k, room, e, dtype, s);
   });
 }
 
 int qnn_linear_act_bwd_work(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes) {
-  if (int rc = check(m, n, k)) return rc;
+  if (int rc = check(m, n, k, dtype)) return rc;
   QNN_REQUIRE(bytes, "null pointer");
-  *bytes = 0;
+  *bytes = bwd_bytes(m, n, k, dtype);
   return QNN_OK;
 }
 
 int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const void* x, int64_t ldx, const void* w,
                        int64_t ldw, void* dz, void* dx, void* dw, void* db, int64_t m, int64_t n, int64_t k,
                        int dtype, int act, void* work, int64_t work_bytes, qnn_stream_t stream) {
-  if (int rc = check(m, n, k)) return rc;
+  if (int rc = check(m, n, k, dtype)) return rc;
   QNN_REQUIRE(act >= QNN_ACT_NONE && act <= QNN_ACT_GELU, "act: QNN_ACT_NONE, QNN_ACT_RELU or QNN_ACT_GELU");
-  QNN_REQUIRE(ldy >= n && (!dw || ldx >= k) && (!dx || ldw >= k), "a row stride is shorter than the row");
-  QNN_REQUIRE(m == 0 || (dy && (!dx || w) && (!dw || x)), "null pointer");
-  QNN_REQUIRE(m == 0 || act == QNN_ACT_NONE || (slope && dz), "an activation's gradient needs slope and dz");
+  if (m > 0) {
+    if (int rc = check_matrix(dy, ldy, m, n, dtype)) return rc;
+    if (dx)
+      if (int rc = check_matrix(w, ldw, n, k, dtype)) return rc;
+    if (dw)
+      if (int rc = check_matrix(x, ldx, m, k, dtype)) return rc;
+    QNN_REQUIRE(act == QNN_ACT_NONE || (slope && dz && aligned16(dz)),
+                "an activation's gradient needs slope and dz, on a 16-byte boundary");
+  }
+  const int64_t need = bwd_bytes(m, n, k, dtype);
+  QNN_REQUIRE(need == 0 || (work && work_bytes >= need && aligned16(work)),
+              "work: at least what qnn_linear_act_bwd_work says, on a 16-byte boundary");
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     hipStream_t s = (hipStream_t)stream;
-    const T* g = (const T*)dy;
+    char* room = (char*)work;
+    const void* g = dy;
     int64_t ldg = ldy;
-    if (act != QNN_ACT_NONE && m > 0) {
-      hipLaunchKernelGGL((linear_dz_kernel<T>), dim3((unsigned)(cdiv(n, 256) * m)), dim3(256), 0, s, g, ldy,
-                         slope, (T*)dz, m, n, act);
+    const Strips st = strips_of(m, n);
+    if (m > 0 && (act != QNN_ACT_NONE || db)) {
+      float* part = db ? (float*)room : nullptr;
+      room += up(st.n * n * 4, 256);
+      QNN_REQUIRE(st.n * st.chunks < (1LL << 31), "too many rows for one call");
+      hipLaunchKernelGGL((linear_dz_kernel<T>), dim3((unsigned)(st.n * st.chunks)), dim3(256), 0, s, (const T*)dy, ldy,
+                         slope, act != QNN_ACT_NONE ? (T*)dz : nullptr, part, m, n, act, st.chunks, st.rows);
       QNN_LAUNCH_CHECK("linear_dz_kernel");
-      g = (const T*)dz;
-      ldg = n;
+      if (act != QNN_ACT_NONE) {
+        g = dz;
+        ldg = n;
+      }
     }
-    const Epilogue none = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE};
-    if (dx && m > 0)
-      if (int rc = matmul<T>(g, ldg, 1, w, 1, ldw, m, k, n, none, s)) return rc;
-    Epilogue to_dw = none;
-    to_dw.y = dw;
-    if (dw)
-      if (int rc = matmul<T>(g, 1, ldg, x, 1, ldx, n, k, m, to_dw, s)) return rc;
     if (db) {
-      hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)cdiv(n, 256)), dim3(256), 0, s, g, ldg, (T*)db, m, n);
+      hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)cdiv(n, 64)), dim3(256), 0, s, (const float*)work,
+                         (int)st.n, (T*)db, n);
       QNN_LAUNCH_CHECK("linear_db_kernel");
     }
+    if (!dx && !dw) return (int)QNN_OK;
+    if (m == 0) {  // an empty sum
+      if (dw) {
+        hipLaunchKernelGGL((zero_kernel<T>), dim3((unsigned)cdiv(n * k, 256)), dim3(256), 0, s, (T*)dw, n * k);
+        QNN_LAUNCH_CHECK("zero_kernel");
+      }
+      return (int)QNN_OK;
+    }
+    if (int rc = on_boundaries<T>(g, ldg, m, n, room, s)) return rc;
+    Epilogue e = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE};
+    const void *px = x, *pw = w;
+    int64_t lx = ldx, lw = ldw;
+    if (dx)
+      if (int rc = on_boundaries<T>(pw, lw, n, k, room, s)) return rc;
+    if (dw)
+      if (int rc = on_boundaries<T>(px, lx, m, k, room, s)) return rc;
+    if (dx)
+      if (int rc = matmul<T, true, false>(g, ldg, pw, lw, m, k, n, room, e, dtype, s)) return rc;
+    e.y = dw;
+    if (dw)
+      if (int rc = matmul<T, false, false>(g, ldg, px, lx, n, k, m, room, e, dtype, s)) return rc;
     return (int)QNN_OK;
   });
 }
