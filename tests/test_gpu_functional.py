@@ -1,5 +1,6 @@
 """qnn.functional on the device against its definitions in float64 (oracle/float_oracle.py), at the
 sizes, strides and values where such kernels go wrong.  Every tolerance is the oracle's bound."""
+import ctypes
 import math
 
 import pytest
@@ -177,7 +178,8 @@ def test_linear_act_refusals(F):
             bad()
     for bad, word in ((lambda: F.linear_act(x, w[:, :3]), "in"), (lambda: F.linear_act(x, w, torch.zeros(4, device="cuda")), "bias"),
                       (lambda: F.linear_act(x, w, None, torch.zeros(1, 3, device="cuda")), "residual"),
-                      (lambda: F.linear_act(x, w, activation="tanh"), "activation"), (lambda: F.linear_act(x[:, :0], w[:, :0]), "feature"),
+                      (lambda: F.linear_act(x, w, activation="tanh"), "activation"), (lambda: F.linear_act(x[:, :0], w[:, :0]), "features"),
+                      (lambda: F.linear_act(x[:, :1].expand(2, (1 << 21) + 1), w[:, :1].expand(3, (1 << 21) + 1)), "2\\^21"),
                       (lambda: F.linear_act(x, w[0]), "weight")):
         with pytest.raises(ValueError, match=word):
             bad()
@@ -469,6 +471,42 @@ def test_gradients_against_differences(F):
         assert abs(slope - gr.norm().item()) <= 2e-2 * gr.norm().item() + 2.0 ** -20 * loss.item() / h
 
 
+def test_gradients_of_gradients_are_refused(F):
+    mods, x, t, i = mlp(F, torch.float32)
+    mods, x = mods.cuda(), x.cuda().requires_grad_(True)
+    dy = torch.randn(2, 25, 96, device="cuda", requires_grad=True)
+    y = F.layer_norm(x, mods[0].weight)
+    gx, = torch.autograd.grad(y, x, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="layer_norm's gradients"):
+        gx.sum().backward()
+    up = torch.randn(2, 25, 200, device="cuda", requires_grad=True)
+    gx, = torch.autograd.grad(F.linear_act(x, mods[1].weight, activation="gelu"), x, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="linear_act's gradients"):
+        gx.sum().backward()
+    # a gradient made under create_graph is a plain one where nothing asks further
+    gx, = torch.autograd.grad(F.layer_norm(x), x, dy.detach(), create_graph=True)
+    assert not gx.requires_grad
+
+
+def test_training_with_backward_and_accumulation(F):
+    """loss.backward() into .grad, twice: the sum of two equal gradients."""
+    mods, x, t, i = mlp(F, torch.bfloat16, seed=8)
+    mods, x, t, i = mods.cuda(), x.cuda(), t.cuda(), i.cuda()
+    mlp_step(F, mods, x, t, i).backward()
+    once = [p.grad.clone() for p in mods.parameters()]
+    mlp_step(F, mods, x, t, i).backward()
+    assert all(torch.equal(p.grad, 2 * g) for p, g in zip(mods.parameters(), once))
+
+
+def test_a_saved_input_that_was_changed_is_refused(F):
+    x = torch.randn(4, 8, device="cuda")
+    w = torch.randn(8, 8, device="cuda", requires_grad=True)
+    y = F.linear_act(x, w)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_same_bits_every_time(F):
     for dt in TYPES:
         mods, x, t, i = mlp(F, dt, seed=2, width=264, hidden=520, rows=300)
@@ -535,7 +573,7 @@ def test_two_captured_training_steps(F):
 def test_nothing_is_written_past_the_outputs(F, dt, m, n, k):
     """The C entries on buffers with a guard behind each output and behind the workspace."""
     from qnn import _lib
-    code = F._DTYPES[dt]
+    code = TYPES.index(dt) + 1 if dt != torch.float32 else 0  # QNN_BF16, QNN_F16, QNN_F32
 
     def guarded(count, dtype):
         size = count * torch.empty((), dtype=dtype).element_size()
@@ -543,11 +581,15 @@ def test_nothing_is_written_past_the_outputs(F, dt, m, n, k):
         return b, size
 
     def work(name, *args):
-        return guarded(F._work_bytes(name, *args), torch.uint8)
+        n = ctypes.c_int64(0)
+        _lib.call(name, *args, ctypes.byref(n))
+        return guarded(n.value, torch.uint8)
+
+    def p(t):
+        return None if t is None else t.data_ptr()
 
     x, w, b, r, dy = dev(*linear_case(m, n, k, dt, True, True))
     st = torch.cuda.current_stream().cuda_stream
-    p = F._ptr
     for act in (0, 1, 2):
         slope_n, slope_t = ((m * ((n + 7) // 8), torch.uint8), (m * n, torch.float32 if code == 0 else torch.int16))[act == 2]
         outs = {"y": guarded(m * n, dt), "slope": guarded(slope_n, slope_t), "dz": guarded(m * n, dt), "dx": guarded(m * k, dt),
