@@ -470,7 +470,7 @@ enum { QNN_ACT_NONE = 0, QNN_ACT_RELU = 1, QNN_ACT_GELU = 2 };
  * the int8 epilogue: the residual first, then the activation.  GELU is z Phi(z).  All of one type.
  * slope (nullable): act'(z) for qnn_linear_act_bwd --
  *   ReLU  [m][ceil(n / 8)] bytes, bit c & 7 of byte c / 8: z is not <= 0;
- *   GELU  [m][n], fp32 for QNN_F32, else int16 fixed point of 1 / 28672 (-32768: NaN).
+ *   GELU  [m][n], fp32 for QNN_F32, else uint16 fixed point, 8192 + 28672 act'(z) (0: NaN).
  * 1 <= n, k < 2^31 and m < 2^31; m == 0 is a no-op.  Replaces nothing of the reference (its layers are
  * F.linear on fake-quantized operands, quantize.py:423-430); stands beside qnn_qconv2d_fwd. */
 int qnn_linear_act_fwd_work(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes);

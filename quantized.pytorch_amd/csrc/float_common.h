@@ -100,43 +100,57 @@ __device__ __forceinline__ float wave_sum_f(float v) {
 // e^x by the hardware's 2^x; the product's rounding costs |x| 2^-24 of relative error.
 __device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 
-// GELU z Phi(z) and its derivative Phi(z) + z phi(z) together, from one exponential:
-// Phi(-a) = erfc(a / sqrt 2) / 2 and erfc(u) = e^(-u^2) t P(t), t = 1 / (1 + 0.36 u), with P fitted
-// here to the scaled complement e^(u^2) erfc(u) (relative error 3.6e-8 for all u), so that the
-// far negative side keeps its relative precision too.  z^2 is carried with its rounding error.
-// The limits at the infinities are 0 and 0 below, z and 1 above; a NaN stays one.
+// GELU z Phi(z) and its derivative Phi(z) + z phi(z) together, from one exponential.  With a = |z|, the
+// tail Phi(-a) = erfc(a / sqrt 2) / 2 = e^(-a^2 / 2) t P(t), t = 1 / (1 + c a), P fitted here to the
+// scaled complement e^(u^2) erfc(u), so that the far negative side keeps its relative precision too:
+//   y = max(z, 0) - a tail,  slope = d below 0 and 1 - d above, d = tail - a phi(a).
+// For results of 16 bits P has degree 5 (relative error 1.1e-6 to |z| = 6.5, past which y is under 1e-9;
+// fp16's half step is 2.4e-4); for fp32 degree 9 (3.6e-8 everywhere) and a^2 with its rounding error.
+// The two products with a take it clamped, which gives the limits at the infinities; a NaN stays one.
+template <bool FP32>
 __device__ __forceinline__ void gelu_f(float z, float& y, float& slope) {
-  const float a = fminf(fabsf(z), 20.0f);  // phi and erfc are 0 in 32 bits long before
-  const float s = a * a, sl = fmaf(a, a, -s);
-  const float e = exp_f(-0.5f * s) * fmaf(-0.5f, sl, 1.0f);
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.36f * 0.70710678118654752f, a, 1.0f));
-  float p = 0.03754199f;
-  p = fmaf(p, t, -0.14138553f);
-  p = fmaf(p, t, 0.14222577f);
-  p = fmaf(p, t, -0.02727648f);
-  p = fmaf(p, t, 0.10558839f);
-  p = fmaf(p, t, 0.12331503f);
-  p = fmaf(p, t, 0.16381756f);
-  p = fmaf(p, t, 0.18995832f);
-  p = fmaf(p, t, 0.20310671f);
-  p = fmaf(p, t, 0.20310828f);
-  const float tail = 0.5f * e * p * t;
-  const float cdf = z < 0.0f ? tail : 1.0f - tail;
-  const float zc = z < 0.0f ? -a : a;
-  y = z <= -20.0f ? -0.0f : z * cdf;
-  const float d = fmaf(zc * 0.39894228040143268f, e, cdf);
-  slope = z != z ? z : d;
+  const float s = z * z, a = __builtin_amdgcn_fmed3f(fabsf(z), 0.0f, 20.0f);
+  float e, p, t;
+  if constexpr (FP32) {
+    const float low = fabsf(z) < 20.0f ? fmaf(z, z, -s) : 0.0f;  // (inf - inf; e is 0 in 32 bits long before)
+    e = __builtin_amdgcn_exp2f(-0.72134752044448170f * s) * fmaf(-0.5f, low, 1.0f);
+    t = __builtin_amdgcn_rcpf(fmaf(0.36f * 0.70710678118654752f, fabsf(z), 1.0f));
+    p = 0.5f * 0.03754199f;
+    p = fmaf(p, t, 0.5f * -0.14138553f);
+    p = fmaf(p, t, 0.5f * 0.14222577f);
+    p = fmaf(p, t, 0.5f * -0.02727648f);
+    p = fmaf(p, t, 0.5f * 0.10558839f);
+    p = fmaf(p, t, 0.5f * 0.12331503f);
+    p = fmaf(p, t, 0.5f * 0.16381756f);
+    p = fmaf(p, t, 0.5f * 0.18995832f);
+    p = fmaf(p, t, 0.5f * 0.20310671f);
+    p = fmaf(p, t, 0.5f * 0.20310828f);
+  } else {
+    e = __builtin_amdgcn_exp2f(-0.72134752044448170f * s);
+    t = __builtin_amdgcn_rcpf(fmaf(0.42f * 0.70710678118654752f, fabsf(z), 1.0f));
+    p = 0.5f * -0.171326101f;
+    p = fmaf(p, t, 0.5f * 0.503957272f);
+    p = fmaf(p, t, 0.5f * -0.116222054f);
+    p = fmaf(p, t, 0.5f * 0.331291884f);
+    p = fmaf(p, t, 0.5f * 0.213374555f);
+    p = fmaf(p, t, 0.5f * 0.23892343f);
+  }
+  const float tail = p * (t * e);
+  y = fmaf(-a, tail, z < 0.0f ? 0.0f : z);
+  const float d = fmaf(a * -0.39894228040143268f, e, tail);
+  slope = z < 0.0f ? d : 1.0f - d;
 }
 
-// The derivative of GELU between the passes, for 16-bit types: fixed point of 2^-15 1.75 (it lies in
-// [-0.13, 1.13]), off by at most 1.8e-5 -- a fourteenth of fp16's half step at 1, where z itself
-// rounded to the type would add an error as large as that of the gradient's own rounding.
+// The derivative of GELU between the passes, for 16-bit types: fixed point of 1 / 28672 from 8192 (it lies
+// in [-0.13, 1.13]; 0 is a NaN), off by at most 1.8e-5 -- a fourteenth of fp16's half step at 1, where z
+// itself rounded to the type would add an error as large as that of the gradient's own rounding.
 constexpr float SLOPE_STEPS = 28672.0f;
 __device__ __forceinline__ int16_t slope_pack(float d) {
-  return d != d ? (int16_t)-32768 : (int16_t)(int)rintf(d * SLOPE_STEPS);
+  return (int16_t)(uint16_t)(uint32_t)fmaf(d, SLOPE_STEPS, 8192.5f);  // (of a NaN: 0)
 }
 __device__ __forceinline__ float slope_unpack(int16_t q) {
-  return q == -32768 ? __builtin_nanf("") : (float)q * (1.0f / SLOPE_STEPS);
+  const int v = (uint16_t)q;
+  return v == 0 ? __builtin_nanf("") : (float)(v - 8192) * (1.0f / SLOPE_STEPS);
 }
 
 template <class F>

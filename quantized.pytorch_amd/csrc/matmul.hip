@@ -44,7 +44,7 @@ __device__ __forceinline__ void finish8(float (&z)[8], const Epilogue& e, int64_
   } else if (e.act == QNN_ACT_GELU) {
     float d[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) gelu_f(z[i], z[i], d[i]);
+    for (int i = 0; i < 8; ++i) gelu_f<sizeof(T) == 4>(z[i], z[i], d[i]);
     if (e.slope) {
       if constexpr (sizeof(T) == 4) {
         store_n<float, 8>((float*)e.slope + row * n + col, d, left);
@@ -78,14 +78,28 @@ __device__ __forceinline__ void finish8(float (&z)[8], const Epilogue& e, int64_
 // fills LDS with zeros; stages past the last are such loads too, so the counts of loads in flight hold.
 constexpr uint32_t PAST = 0x80000000u;  // a buffer offset that is past every size below
 
+// Waits until at most N of this wave's loads and none of its LDS reads are under way, then for the other
+// waves.  By the builtin, which the compiler counts with: after an asm wait it would add its own before
+// each use of a fragment, too long a one where more reads are under way than its 4-bit counter holds.
 template <int N>
-__device__ __forceinline__ void wait_loads() {  // at most N of this wave's loads in flight, no LDS read
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 typedef __attribute__((address_space(3))) void* lds_t;
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4* lds_s4_t;
+
+// Four 16-bit elements of one k from each of the lane's neighbours in k (its 16 lanes name 4 k of 16 rows;
+// it gets row lane % 16).  `restrict`, because the compiler gives this read no alias information of its
+// own, and waits for every direct load under way before it if nothing says that they are apart.
+__device__ __forceinline__ s4 turned(const __attribute__((address_space(3))) s4* __restrict p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)p);
+}
 
 struct Operand {
   const void* p;
@@ -100,6 +114,7 @@ struct Side {
   static_assert(R % (16 * W) == 0, "a wave loads whole KiB");
   static constexpr int GRAN = 16 * ES, GMASK = R / 16 < 8 ? R / 16 - 1 : 7;  // bytes, and the XOR's bits
 
+  static __device__ __forceinline__ int turn(int row) { return -(row >> 2) & 3; }  // of a chunk's index, DENSE
   static __device__ __forceinline__ int spread(int k) {  // what a granule's index is XORed with, not DENSE
     if constexpr (ES == 2) return ((k & 3) | (k >> 3 & 1) << 2) & GMASK;
     else return k >> 2 & 3;
@@ -123,7 +138,7 @@ struct Side {
     for (int j = 0; j < LOADS; ++j) {
       const int at = (wave * LOADS + j) * 1024 + lane * 16;
       if constexpr (DENSE) {
-        const int row = at / 64, chunk = at / 16 % 4 ^ (row >> 2 & 3);
+        const int row = at / 64, chunk = at / 16 % 4 ^ turn(row);
         kat[j] = chunk * 16 / ES;
         off[j] = i0 + row < o.rows ? (uint32_t)(row * (int)o.ld * ES + chunk * 16) : PAST;
       } else {
@@ -134,22 +149,19 @@ struct Side {
       }
     }
   }
-  // the next stage, of which `left` elements of k are there, into the slot at lds
-  __device__ __forceinline__ void load(char* lds, int left, int wave) {
+  // load j of the next stage, of which `left` elements of k are there, into the slot at lds
+  __device__ __forceinline__ void load(char* lds, int j, int left, int wave) const {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass drops a kernel that names the resource type, without a word
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)(lds + (wave * LOADS + j) * 1024), 16,
-                                               kat[j] < left ? off[j] : PAST, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)(lds + (wave * LOADS + j) * 1024), 16,
+                                             kat[j] < left ? off[j] : PAST, 0, 0, 0);
 #endif
-    base += step;
   }
   // fragment f (rows 16 f ... of the wave's, which begin at row r0)
   static __device__ __forceinline__ int place(int r0, int lane) {
     if constexpr (DENSE) {
       const int row = lane & 15;
-      return (r0 + row) * 64 + ((lane >> 4) ^ (row >> 2 & 3)) * 16;
+      return (r0 + row) * 64 + ((lane >> 4) ^ turn(row)) * 16;
     } else if constexpr (ES == 2) {
       return ((lane >> 4) * 8 + (lane >> 2 & 3)) * R * ES + (lane & 3) * 8;
     } else {
@@ -166,8 +178,8 @@ struct Side {
         s4 s[2];
         f4 v;
       } u;
-      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)p);
-      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t)(p + 4 * R * ES));
+      u.s[0] = turned((lds_s4_t)p);
+      u.s[1] = turned((lds_s4_t)(p + 4 * R * ES));
       return u.v;
     } else {
       const int h = spread((lane >> 4) * 4);
@@ -244,10 +256,14 @@ __global__ __launch_bounds__(C::NT, C::EU) void matmul_kernel(Operand a, Operand
   B sb;
   sa.begin(a, i0, k0, wave, lane);
   sb.begin(b, j0, k0, wave, lane);
-  auto load = [&](int slot) {
-    sa.load(lds + slot * C::SLOT, left, wave);
-    sb.load(lds + slot * C::SLOT + A::BYTES, left, wave);
-    left -= KE;
+  auto load = [&](int slot, int j) {  // load j of P of the next stage
+    if (j < A::LOADS) sa.load(lds + slot * C::SLOT, j, left, wave);
+    else sb.load(lds + slot * C::SLOT + A::BYTES, j - A::LOADS, left, wave);
+    if (j == P - 1) {
+      sa.base += sa.step;
+      sb.base += sb.step;
+      left -= KE;
+    }
   };
   const int pa = A::place(ri, lane), pb = B::place(rj, lane);
   f4 fa[2][TM], fb[2][TN], acc[TM][TN];
@@ -255,29 +271,36 @@ __global__ __launch_bounds__(C::NT, C::EU) void matmul_kernel(Operand a, Operand
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-  auto fetch = [&](int slot, int to) {
+  auto fetch = [&](int slot, int to, int f) {  // fragment f of TN + TM
     char* s = lds + slot * C::SLOT;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) fa[to][i] = A::fragment(s, pa, ri, i, lane);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) fb[to][j] = B::fragment(s + A::BYTES, pb, rj, j, lane);
+    if (f < TN) fb[to][f] = B::fragment(s + A::BYTES, pb, rj, f, lane);
+    else fa[to][f - TN] = A::fragment(s, pa, ri, f - TN, lane);
   };
 #pragma unroll
-  for (int s = 0; s < 4; ++s) load(s);
-  wait_loads<3 * P>();
-  __builtin_amdgcn_s_barrier();
-  fetch(0, 0);
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int j = 0; j < P; ++j) load(s, j);
+  meet<3 * P>();
+#pragma unroll
+  for (int f = 0; f < TM + TN; ++f) fetch(0, 0, f);
   // step s: stage s is in registers, s + 1 to s + 3 in LDS or on their way
   auto step = [&](int s, auto cur) {
     constexpr int C0 = decltype(cur)::value;
-    wait_loads<2 * P>();  // stage s + 1 has landed, and stage s has left its slot
-    __builtin_amdgcn_s_barrier();
-    load(s & 3);  // stage s + 4
-    fetch((s + 1) & 3, C0 ^ 1);
+    meet<2 * P>();  // stage s + 1 has landed, and stage s has left its slot
+    // rows of MFMAs with the loads of stage s + 4 and the reads of stage s + 1 between them, in this
+    // order: left to itself the compiler puts the reads last, where the next step waits for them
+    constexpr int BUSY = TM > 2 ? TM - 2 : 1, READS = (TM + TN + BUSY - 1) / BUSY, LOADS = (P + BUSY - 1) / BUSY;
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int j = i * LOADS; j < (i + 1) * LOADS && j < P; ++j) load(s & 3, j);
+#pragma unroll
+      for (int f = i * READS; f < (i + 1) * READS && f < TM + TN; ++f) fetch((s + 1) & 3, C0 ^ 1, f);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = mma<T>(fb[C0][j], fa[C0][i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   int s = 0;
   for (; s + 1 < stages; s += 2) {
@@ -285,8 +308,7 @@ __global__ __launch_bounds__(C::NT, C::EU) void matmul_kernel(Operand a, Operand
     step(s + 1, std::integral_constant<int, 1>{});
   }
   if (s < stages) step(s, std::integral_constant<int, 0>{});
-  wait_loads<0>();
-  __syncthreads();
+  meet<0>();
 
   // acc[i][j]: row 16 i + lane % 16, columns 16 j + lane / 16 * 4 ... + 3.  A wave turns 16 rows at a
   // time around in LDS of its own, so that a lane has 8 neighbouring columns and a row's are together.
@@ -473,7 +495,10 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* part, int s
 }
 
 // ---------------------------------------------------------------------------------------- host side
-using Big = Cfg<2, 4, 8, 4, 2>;     // 256 x 256, one workgroup a CU
+#ifndef BIGC
+#define BIGC 2, 4, 8, 4, 2
+#endif
+using Big = Cfg<BIGC>;     // 256 x 256, one workgroup a CU
 using Middle = Cfg<2, 2, 4, 4, 2>;  // 128 x 128
 using Small = Cfg<2, 2, 2, 2, 4>;   // 64 x 64
 
