@@ -42,10 +42,29 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* sh, int& turn) {
   }
 }
 
-// L lanes a row, G groups of 16 bytes a lane: lane l has columns (j L + l) GROUP + i, j < G, i < GROUP.
+// L lanes a row, G groups of 16 bytes a lane, D rows ahead of the present one on their way.
 template <int L_, int G_>
 struct Shape {
-  static constexpr int L = L_, G = G_, NT = L > 256 ? L : 256, ROWS = NT / L;
+  static constexpr int L = L_, G = G_, NT = L > 256 ? L : 256, ROWS = NT / L, D = 2;
+};
+
+// A lane's columns: group j is columns at[j] ... at[j] + GROUP - 1, of which the first skip[j] belong to
+// another lane too.  The groups lie (j L + lane) GROUP from the row's start, but no further than the last
+// whole one that the row holds: every load is a whole group inside the row, without a branch, and what a
+// lane has twice is left out of sums and written twice with the same value.
+template <class T, class S>
+struct Columns {
+  int at[S::G], skip[S::G];
+  __device__ __forceinline__ Columns(int lane, int dim) {
+#pragma unroll
+    for (int j = 0; j < S::G; ++j) {
+      const int c = (j * S::L + lane) * GROUP<T>;
+      at[j] = c < dim - GROUP<T> ? c : dim - GROUP<T>;
+      skip[j] = c - at[j];
+    }
+  }
+  __device__ __forceinline__ bool owns(int j, int i) const { return i >= skip[j]; }
+  __device__ __forceinline__ bool any(int j) const { return skip[j] < GROUP<T>; }
 };
 
 template <class T, class W, class S>
@@ -54,46 +73,43 @@ __global__ __launch_bounds__(S::NT) void layer_norm_fwd_kernel(const T* __restri
                                                                T* __restrict__ y, float* __restrict__ mean,
                                                                float* __restrict__ rstd, int64_t rows, int dim,
                                                                float eps) {
-  constexpr int L = S::L, G = S::G, GR = GROUP<T>;
+  constexpr int L = S::L, G = S::G, GR = GROUP<T>, D = S::D;
   __shared__ float sh[4 * (L > 64 ? L / 64 : 1)];
   const int lane = threadIdx.x % L, sub = threadIdx.x / L;
+  const Columns<T, S> col(lane, dim);
   int turn = 0;
   const float inv = 1.0f / (float)dim;
   float wv[G][GR], bv[G][GR];
+  Vec<T, GR> ahead[D][G];
+  const int64_t first = (int64_t)blockIdx.x * S::ROWS + sub, step = (int64_t)gridDim.x * S::ROWS;
+  auto fetch = [&](int64_t row, int d) {  // (past the last row: that one again, which is not used)
+    const T* p = x + (row < rows ? row : rows - 1) * ldx;
+#pragma unroll
+    for (int j = 0; j < G; ++j) ahead[d][j] = load_group(p + col.at[j], GR);
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) fetch(first + d * step, d);
 #pragma unroll
   for (int j = 0; j < G; ++j) {
-    const int c = (j * L + lane) * GR;
 #pragma unroll
     for (int i = 0; i < GR; ++i) {
       wv[j][i] = 1.0f;
       bv[j][i] = 0.0f;
     }
-    if (w) load_n<W, GR>(wv[j], w + c, dim - c);
-    if (b) load_n<W, GR>(bv[j], b + c, dim - c);
+    if (w) load_n<W, GR>(wv[j], w + col.at[j], GR);
+    if (b) load_n<W, GR>(bv[j], b + col.at[j], GR);
   }
-  Vec<T, GR> next[G];
-  int64_t r = (int64_t)blockIdx.x * S::ROWS + sub;
-  const int64_t step = (int64_t)gridDim.x * S::ROWS;
-  auto fetch = [&](int64_t row) {
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-      const int c = (j * L + lane) * GR;
-      next[j] = load_group(x + row * ldx + c, row < rows ? dim - c : 0);
-    }
-  };
-  fetch(r);
-  // every lane of a workgroup takes part in every round, for the barriers in its sums
-  for (int64_t r0 = (int64_t)blockIdx.x * S::ROWS; r0 < rows; r0 += step, r += step) {
+  auto one = [&](int64_t r, int d) {
     float v[G][GR];
     float s[1] = {0.0f};
 #pragma unroll
     for (int j = 0; j < G; ++j)
 #pragma unroll
       for (int i = 0; i < GR; ++i) {
-        v[j][i] = (float)next[j].v[i];
-        s[0] += v[j][i];
+        v[j][i] = (float)ahead[d][j].v[i];
+        s[0] += col.owns(j, i) ? v[j][i] : 0.0f;
       }
-    fetch(r + step);
+    fetch(r + D * step, d);
     row_sums<L>(s, sh, turn);
     const float mu = s[0] * inv;
     float q[1] = {0.0f};
@@ -101,24 +117,29 @@ __global__ __launch_bounds__(S::NT) void layer_norm_fwd_kernel(const T* __restri
     for (int j = 0; j < G; ++j)
 #pragma unroll
       for (int i = 0; i < GR; ++i) {
-        v[j][i] = (j * L + lane) * GR + i < dim ? v[j][i] - mu : 0.0f;
-        q[0] = fmaf(v[j][i], v[j][i], q[0]);
+        v[j][i] -= mu;
+        q[0] = fmaf(v[j][i], col.owns(j, i) ? v[j][i] : 0.0f, q[0]);
       }
     row_sums<L>(q, sh, turn);
     const float rs = 1.0f / sqrtf(fmaf(q[0], inv, eps));
     if (r < rows) {
 #pragma unroll
       for (int j = 0; j < G; ++j) {
-        const int c = (j * L + lane) * GR;
         Vec<T, GR> o;
 #pragma unroll
         for (int i = 0; i < GR; ++i) o.v[i] = (T)fmaf(v[j][i] * rs, wv[j][i], bv[j][i]);
-        store_group(y + r * dim + c, o, dim - c);
+        if (col.any(j)) store_group(y + r * dim + col.at[j], o, GR);
       }
       if (lane == 0 && mean) mean[r] = mu;
       if (lane == 0 && rstd) rstd[r] = rs;
     }
-  }
+  };
+  // every lane of a workgroup takes part in every round, for the barriers in its sums
+  int64_t r = first;
+  for (int64_t r0 = (int64_t)blockIdx.x * S::ROWS; r0 < rows; r0 += D * step, r += D * step)
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (d == 0 || r0 + d * step < rows) one(r + d * step, d);
 }
 
 // part: [gridDim.x][2][dim], this workgroup's sums of dw and db (null: not wanted)
@@ -129,70 +150,72 @@ __global__ __launch_bounds__(S::NT) void layer_norm_bwd_kernel(const T* __restri
                                                                const float* __restrict__ mean,
                                                                const float* __restrict__ rstd, T* __restrict__ dx,
                                                                float* __restrict__ part, int64_t rows, int dim) {
-  constexpr int L = S::L, G = S::G, GR = GROUP<T>;
+  constexpr int L = S::L, G = S::G, GR = GROUP<T>, D = S::D;
   __shared__ float sh[4 * (L > 64 ? L / 64 : 1)];
   const int lane = threadIdx.x % L, sub = threadIdx.x / L;
+  const Columns<T, S> col(lane, dim);
   int turn = 0;
   const float inv = 1.0f / (float)dim;
   float wv[G][GR], aw[G][GR] = {}, ab[G][GR] = {};
-#pragma unroll
-  for (int j = 0; j < G; ++j) {
-    const int c = (j * L + lane) * GR;
-#pragma unroll
-    for (int i = 0; i < GR; ++i) wv[j][i] = 1.0f;
-    if (w) load_n<W, GR>(wv[j], w + c, dim - c);
-  }
-  Vec<T, GR> nx[G], ny[G];
-  float nmu, nrs;
-  int64_t r = (int64_t)blockIdx.x * S::ROWS + sub;
-  const int64_t step = (int64_t)gridDim.x * S::ROWS;
-  auto fetch = [&](int64_t row) {
-    const bool there = row < rows;
+  Vec<T, GR> nx[D][G], ny[D][G];
+  float nmu[D], nrs[D];
+  const int64_t first = (int64_t)blockIdx.x * S::ROWS + sub, step = (int64_t)gridDim.x * S::ROWS;
+  auto fetch = [&](int64_t row, int d) {
+    const int64_t k = row < rows ? row : rows - 1;
 #pragma unroll
     for (int j = 0; j < G; ++j) {
-      const int c = (j * L + lane) * GR;
-      nx[j] = load_group(x + row * ldx + c, there ? dim - c : 0);
-      ny[j] = load_group(dy + row * ldy + c, there ? dim - c : 0);
+      nx[d][j] = load_group(x + k * ldx + col.at[j], GR);
+      ny[d][j] = load_group(dy + k * ldy + col.at[j], GR);
     }
-    nmu = there ? mean[row] : 0.0f;
-    nrs = there ? rstd[row] : 0.0f;
+    nmu[d] = mean[k];
+    nrs[d] = rstd[k];
   };
-  fetch(r);
-  for (int64_t r0 = (int64_t)blockIdx.x * S::ROWS; r0 < rows; r0 += step, r += step) {
+#pragma unroll
+  for (int d = 0; d < D; ++d) fetch(first + d * step, d);
+#pragma unroll
+  for (int j = 0; j < G; ++j) {
+#pragma unroll
+    for (int i = 0; i < GR; ++i) wv[j][i] = 1.0f;
+    if (w) load_n<W, GR>(wv[j], w + col.at[j], GR);
+  }
+  auto one = [&](int64_t r, int d) {
     float h[G][GR], g[G][GR];
     float s[2] = {0.0f, 0.0f};
-    const float mu = nmu, rs = nrs;
+    const float mu = nmu[d], rs = nrs[d];
+    const bool there = r < rows;
 #pragma unroll
     for (int j = 0; j < G; ++j)
 #pragma unroll
       for (int i = 0; i < GR; ++i) {
-        // past the row's end x and dy are 0 here: xh is off, but dy xh and g xh are 0 and so no sum is
-        // (a mean that is no number makes them NaN; they are not written)
-        h[j][i] = ((float)nx[j].v[i] - mu) * rs;
-        const float d = (float)ny[j].v[i];
-        const float dh = d * h[j][i];
-        g[j][i] = d * wv[j][i];
-        aw[j][i] += dh;
-        ab[j][i] += d;
-        s[0] += g[j][i];
-        s[1] = fmaf(g[j][i], h[j][i], s[1]);
+        h[j][i] = ((float)nx[d][j].v[i] - mu) * rs;
+        const float v = there ? (float)ny[d][j].v[i] : 0.0f;
+        g[j][i] = v * wv[j][i];
+        aw[j][i] = fmaf(v, there ? h[j][i] : 0.0f, aw[j][i]);
+        ab[j][i] += v;
+        const float mine = col.owns(j, i) ? g[j][i] : 0.0f;
+        s[0] += mine;
+        s[1] = fmaf(mine, h[j][i], s[1]);
       }
-    fetch(r + step);
+    fetch(r + D * step, d);
     if (dx) {
       row_sums<L>(s, sh, turn);
       const float sg = s[0] * inv, sx = s[1] * inv;
-      if (r < rows) {
+      if (there) {
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-          const int c = (j * L + lane) * GR;
           Vec<T, GR> o;
 #pragma unroll
           for (int i = 0; i < GR; ++i) o.v[i] = (T)(rs * (g[j][i] - sg - h[j][i] * sx));
-          store_group(dx + r * dim + c, o, dim - c);
+          if (col.any(j)) store_group(dx + r * dim + col.at[j], o, GR);
         }
       }
     }
-  }
+  };
+  int64_t r = first;
+  for (int64_t r0 = (int64_t)blockIdx.x * S::ROWS; r0 < rows; r0 += D * step, r += D * step)
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (d == 0 || r0 + d * step < rows) one(r + d * step, d);
   if (!part) return;
   if constexpr (S::ROWS > 1) {  // the workgroup's rows, in their order
     __shared__ float all[S::ROWS][L * G * GR];
@@ -202,7 +225,8 @@ __global__ __launch_bounds__(S::NT) void layer_norm_bwd_kernel(const T* __restri
 #pragma unroll
       for (int j = 0; j < G; ++j)
 #pragma unroll
-        for (int i = 0; i < GR; ++i) all[sub][(j * L + lane) * GR + i] = which ? ab[j][i] : aw[j][i];
+        for (int i = 0; i < GR; ++i)
+          if (col.owns(j, i)) all[sub][col.at[j] + i] = which ? ab[j][i] : aw[j][i];
       __syncthreads();
       for (int c = threadIdx.x; c < dim; c += S::NT) {
         float s = all[0][c];
@@ -213,12 +237,12 @@ __global__ __launch_bounds__(S::NT) void layer_norm_bwd_kernel(const T* __restri
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < G; ++j) {
-      const int c = (j * L + lane) * GR;
-      float* p = part + (int64_t)blockIdx.x * 2 * dim + c;
-      store_n<float, GR>(p, aw[j], dim - c);
-      store_n<float, GR>(p + dim, ab[j], dim - c);
-    }
+    for (int j = 0; j < G; ++j)
+      if (col.any(j)) {
+        float* p = part + (int64_t)blockIdx.x * 2 * dim + col.at[j];
+        store_n<float, GR>(p, aw[j], GR);
+        store_n<float, GR>(p + dim, ab[j], GR);
+      }
   }
 }
 
@@ -247,7 +271,7 @@ __global__ __launch_bounds__(1024) void layer_norm_join_kernel(const float* __re
   }
 }
 
-// ---- rows too long for registers: a workgroup a row, read again (from L2) for each step
+// ---- rows too long for registers (or shorter than a group): a workgroup a row, read again (from L2) for each step
 constexpr int LONG = 1024;
 
 template <class T, class W>
@@ -364,10 +388,11 @@ int with_types(int dtype, int wdtype, F&& f) {
 }
 
 // The shape for rows of `dim`: the fewest lanes with at most 2 groups each up to a wave, then
-// workgroups of 256 (up to 4) and of 1024.  False: too long.
+// workgroups of 256 (up to 4) and of 1024.  False: too long, or shorter than a group.
 template <class T, class F>
 bool with_shape(int64_t dim, F&& f) {
   const int64_t g = cdiv(dim, GROUP<T>);
+  if (dim < GROUP<T>) return false;  // no whole group
   if (g <= 16) f(Shape<16, 1>{});
   else if (g <= 64) f(Shape<64, 1>{});
   else if (g <= 128) f(Shape<64, 2>{});
@@ -420,7 +445,7 @@ int qnn_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b,
     hipStream_t s = (hipStream_t)stream;
     const bool held = with_shape<T>(dim, [&](auto shape) {
       using S = decltype(shape);
-      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, S>), dim3(row_blocks<S>(rows, 2048)), dim3(S::NT), 0, s,
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, S>), dim3(row_blocks<S>(rows, S::NT > 256 ? 512 : 1024)), dim3(S::NT), 0, s,
                          (const T*)x, ldx, (const W*)w, (const W*)b, (T*)y, mean, rstd, rows, (int)dim, eps);
     });
     if (!held)
