@@ -297,8 +297,16 @@ __global__ __launch_bounds__(C::NT, C::EU) void matmul_kernel(Operand a, Operand
 #pragma unroll
       for (int f = i * READS; f < (i + 1) * READS && f < TM + TN; ++f) fetch((s + 1) & 3, C0 ^ 1, f);
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mma<T>(fb[C0][j], fa[C0][i], acc[i][j]);
+        for (int j = 0; j < TN; ++j) acc[i][j] = mma<T>(fb[C0][j], fa[C0][i], acc[i][j]);
+      } else {  // one after another on different sums
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < TN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[C0][j][q], fa[C0][i][q], acc[i][j], 0, 0, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -495,15 +503,28 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* part, int s
 }
 
 // ---------------------------------------------------------------------------------------- host side
-#ifndef BIGC
-#define BIGC 2, 4, 8, 4, 2
-#endif
-using Big = Cfg<BIGC>;     // 256 x 256, one workgroup a CU
-using Middle = Cfg<2, 2, 4, 4, 2>;  // 128 x 128
-using Small = Cfg<2, 2, 2, 2, 4>;   // 64 x 64
+// The tiles.  Measured time of one stage of k for a workgroup that has its CU's turn, and of a workgroup's
+// start and end, in us (stage: 16-bit types, fp32):
+//   Big    256 x 256  0.72   -    10   (8 waves, one workgroup a CU)
+//   Middle 128 x 128  0.26  0.97   5   (8 waves)
+//   Half   128 x 64   0.19  0.50   4
+//   Small  64 x 64    0.10  0.25   4   (0.13 alone on its CU: latency)
+// A larger tile does more MFMAs for each byte it loads; a smaller one fills the chip with fewer rows.
+using Big = Cfg<2, 4, 8, 4, 2>;
+using Middle = Cfg<2, 4, 4, 2, 2>;
+using Half = Cfg<2, 2, 4, 2, 2>;
+using Small = Cfg<2, 2, 2, 2, 4>;
+struct Shape {
+  int bm, bn;
+  float stage16, stage32, ends, alone;  // alone: what one by itself on a CU takes of its stage's time (16 bits)
+};
+constexpr Shape SHAPES[] = {{Big::BM, Big::BN, 0.72f, 0.0f, 10.0f, 1.0f},
+                            {Middle::BM, Middle::BN, 0.26f, 0.97f, 5.0f, 1.0f},
+                            {Half::BM, Half::BN, 0.19f, 0.50f, 4.0f, 1.0f},
+                            {Small::BM, Small::BN, 0.105f, 0.25f, 4.0f, 1.2f}};
 
 struct Plan {
-  int cfg;      // 0 Big, 1 Middle, 2 Small
+  int cfg;      // of SHAPES
   int splits;
   int64_t span;  // elements of k in a split
   int64_t ldp;
@@ -512,23 +533,36 @@ struct Plan {
 
 int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
-// The tile and the splits of k of one product.
+// The tile and the splits of k of one product: the least of the times above, for as many turns as the
+// busiest of 256 CUs takes; splits cost a second launch (5.5 us with its host time) and their sums' way
+// through memory (at 4 TB/s).  Over the sizes that were swept (m, n 64 to 8192, k 64 to 8192) what it
+// picks is within 10 % of the best pair, 20 % where the whole takes under 20 us.
 Plan plan_of(int64_t m, int64_t n, int64_t k, int dtype) {
   const int64_t ke = 64 / type_bytes(dtype), stages = cdiv(k, ke);
-  auto tiles = [&](int64_t b) { return cdiv(m, b) * cdiv(n, b); };
   Plan p = {};
-  if (dtype != QNN_F32 && tiles(256) >= 192) p.cfg = 0;
-  else if (tiles(128) >= 192) p.cfg = 1;
-  else p.cfg = 2;
-  const int64_t have = tiles(p.cfg == 0 ? 256 : p.cfg == 1 ? 128 : 64);
-  int64_t s = 1;
-  if (have < 256) s = cdiv(512, have);
-  if (s > stages / 8) s = stages / 8;
-  if (s > 32) s = 32;
-  if (s < 1) s = 1;
-  const int64_t each = cdiv(stages, s);
-  p.splits = (int)cdiv(stages, each);
-  p.span = each * ke;
+  float best = INFINITY;
+  for (int c = dtype == QNN_F32 ? 1 : 0; c < 4; ++c) {
+    const Shape& h = SHAPES[c];
+    const int64_t tiles = cdiv(m, h.bm) * cdiv(n, h.bn);
+    const float stage = dtype == QNN_F32 ? h.stage32 : h.stage16;
+    for (int turns = 0; turns <= 3; ++turns) {  // 0: no split; else as many as fill the CUs so many times
+      int64_t s = turns == 0 ? 1 : 256 * turns / tiles;
+      if (turns > 0 && s < 2) continue;
+      if (s > stages / 4) s = stages / 4;
+      if (s > 32) s = 32;
+      if (s < 1) s = 1;
+      const int64_t each = cdiv(stages, s), splits = cdiv(stages, each);
+      const float busiest = (float)cdiv(tiles * splits, 256);
+      float us = fmaxf(busiest, dtype == QNN_F32 ? 1.0f : h.alone) * (float)each * stage + busiest * 0.6f * h.ends + 0.4f * h.ends;
+      if (splits > 1) us += 5.5f + (float)(splits * m * n) * 2e-6f;
+      if (us < best) {
+        best = us;
+        p.cfg = c;
+        p.splits = (int)splits;
+        p.span = each * ke;
+      }
+    }
+  }
   p.ldp = up(n, 8);
   p.part_bytes = p.splits > 1 ? p.splits * m * p.ldp * 4 : 0;
   return p;
@@ -572,6 +606,7 @@ int matmul(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m, in
   if constexpr (sizeof(T) == 2)
     if (p.cfg == 0) return launch<T, AD, BD, Big>(oa, ob, p, m, n, k, (float*)part, e, s);
   if (p.cfg == 1) return launch<T, AD, BD, Middle>(oa, ob, p, m, n, k, (float*)part, e, s);
+  if (p.cfg == 2) return launch<T, AD, BD, Half>(oa, ob, p, m, n, k, (float*)part, e, s);
   return launch<T, AD, BD, Small>(oa, ob, p, m, n, k, (float*)part, e, s);
 }
 
