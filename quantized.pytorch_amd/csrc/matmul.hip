@@ -17,21 +17,27 @@ struct Epilogue {
   int act;
 };
 
+// The bias of 8 columns.
 template <class T>
-__device__ __forceinline__ void finish8(float (&z)[8], const Epilogue& e, int64_t row, int64_t col, int64_t n) {
-  const int64_t left = n - col;
-  if (e.bias) {
-    float b[8];
-    load_n<T, 8>(b, (const T*)e.bias + col, left);
+__device__ __forceinline__ void bias8(float (&b)[8], const Epilogue& e, int64_t col, int64_t n) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] += b[i];
-  }
+  for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+  if (e.bias) load_n<T, 8>(b, (const T*)e.bias + col, n - col);
+}
+
+// WHOLE: all 8 are inside the matrix, which the compiler then need not ask in front of each access.
+template <class T, bool WHOLE>
+__device__ __forceinline__ void finish8(float (&z)[8], const float (&bias)[8], const Epilogue& e, int64_t row,
+                                        int64_t col, int64_t n) {
+  const int64_t left = WHOLE ? 8 : n - col;
   if (e.res) {
-    float b[8];
-    load_n<T, 8>(b, (const T*)e.res + row * e.ldr + col, left);
+    float r[8];
+    load_n<T, 8>(r, (const T*)e.res + row * e.ldr + col, left);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] += b[i];
+    for (int i = 0; i < 8; ++i) z[i] += r[i];
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] += bias[i];
   if (e.act == QNN_ACT_RELU) {
     unsigned mask = 0;
 #pragma unroll
@@ -318,31 +324,48 @@ __global__ __launch_bounds__(C::NT, C::EU) void matmul_kernel(Operand a, Operand
   if (s < stages) step(s, std::integral_constant<int, 0>{});
   meet<0>();
 
-  // acc[i][j]: row 16 i + lane % 16, columns 16 j + lane / 16 * 4 ... + 3.  A wave turns 16 rows at a
-  // time around in LDS of its own, so that a lane has 8 neighbouring columns and a row's are together.
-  constexpr int COLS = 16 * TN, STRIDE = COLS + 4, PER = COLS / 8;
-  float* mine = reinterpret_cast<float*>(lds) + wave * 16 * STRIDE;
-  static_assert(C::W * 16 * STRIDE * 4 <= C::LDS, "the ring holds the turned rows");
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-      *reinterpret_cast<f4*>(mine + (lane & 15) * STRIDE + 16 * j + (lane >> 4) * 4) = acc[i][j];
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int u = 0; u < 16 * PER / 64; ++u) {
-      const int row = (u * 64 + lane) / PER, col = (u * 64 + lane) % PER * 8;
+  // acc[i][j]: row 16 i + lane % 16, columns 16 j + lane / 16 * 4 ... + 3.  A wave turns as many rows at a
+  // time around in its share of LDS as fit, so that a lane has 8 neighbouring columns, the same ones in
+  // every row, and a row's are together.  Chunks of 16 bytes are XORed by the row.
+  constexpr int COLS = 16 * TN, PER = COLS / 8, FIT = C::LDS / C::W / (COLS * 4) / 16;
+  constexpr int TURN = FIT < TM ? FIT : TM;  // 16-row tiles at a time
+  static_assert(TURN > 0 && TM % TURN == 0, "whole turns");
+  char* mine = lds + wave * (C::LDS / C::W);
+  const int col = lane % PER * 8;
+  const int64_t gj = j0 + rj + col;
+  float bias[8];
+  bias8<T>(bias, e, gj, t.n);
+  auto rows_out = [&](int64_t gi0, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+#pragma unroll 2
+    for (int u = 0; u < TURN * 16 * PER / 64; ++u) {
+      const int row = u * (64 / PER) + lane / PER;
       float z[8];
-      *reinterpret_cast<f4*>(z) = *reinterpret_cast<const f4*>(mine + row * STRIDE + col);
-      *reinterpret_cast<f4*>(z + 4) = *reinterpret_cast<const f4*>(mine + row * STRIDE + col + 4);
-      const int64_t gi = i0 + ri + 16 * i + row, gj = j0 + rj + col;
-      if (gi < t.m && gj < t.n) {
-        if (t.splits > 1)
-          store_n<float, 8>(t.part + (split * t.m + gi) * t.ldp + gj, z, t.ldp - gj);
-        else
-          finish8<T>(z, e, gi, gj, t.n);
-      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<f4*>(z + 4 * h) =
+            *reinterpret_cast<const f4*>(mine + row * COLS * 4 + ((col / 4 + h) ^ (row & (COLS / 4 - 1))) * 16);
+      const int64_t gi = gi0 + row;
+      if (!WHOLE && (gi >= t.m || gj >= t.n)) continue;
+      if (t.splits > 1)
+        store_n<float, 8>(t.part + (split * t.m + gi) * t.ldp + gj, z, 8);  // (ldp: whole groups of 8)
+      else
+        finish8<T, WHOLE>(z, bias, e, gi, gj, t.n);
     }
+  };
+  const bool inside = i0 + C::BM <= t.m && j0 + C::BN <= t.n;
+#pragma unroll
+  for (int i = 0; i < TM; i += TURN) {
+#pragma unroll
+    for (int k = 0; k < TURN; ++k)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int row = 16 * k + (lane & 15);
+        *reinterpret_cast<f4*>(mine + row * COLS * 4 + ((4 * j + (lane >> 4)) ^ (row & (COLS / 4 - 1))) * 16) = acc[i + k][j];
+      }
+    __builtin_amdgcn_wave_barrier();
+    if (inside) rows_out(i0 + ri + 16 * i, std::true_type{});
+    else rows_out(i0 + ri + 16 * i, std::false_type{});
     __builtin_amdgcn_wave_barrier();
   }
 }
@@ -360,7 +383,9 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(const float* part, int
 #pragma unroll
     for (int i = 0; i < 8; ++i) z[i] += v[i];
   }
-  finish8<T>(z, e, row, col, n);
+  float bias[8];
+  bias8<T>(bias, e, col, n);
+  finish8<T, false>(z, bias, e, row, col, n);
 }
 
 // ------------------------------------------------------------------------- few rows: the weight is all
@@ -408,13 +433,15 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(const T* x, int64_t ld
   if (t >= 2 * m) return;
   const int r = t >> 1, c = (t & 1) * 8;
   if (j0 + c >= n) return;
+  float bias[8];
+  bias8<T>(bias, e, j0 + c, n);
   float z[8] = {};
   for (int v = 0; v < W; ++v) {
     const f4 lo = sums[v][(c / 4) * 16 + r], hi = sums[v][(c / 4 + 1) * 16 + r];
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] += lo[i], z[4 + i] += hi[i];
   }
-  finish8<T>(z, e, r, j0 + c, n);
+  finish8<T, false>(z, bias, e, r, j0 + c, n);
 }
 
 // ------------------------------------------------------------------------------ rows on boundaries
@@ -447,11 +474,12 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, int64_t ldy
   const int64_t c = ((int64_t)(blockIdx.x % chunks) * 64 + lane) * 8, left = n - c;
   const int64_t s = blockIdx.x / chunks, r1 = (s + 1) * strip < m ? (s + 1) * strip : m;
   float sum[8] = {};
-  if (left > 0) {
+  auto rows = [&](auto whole) {
+    const int64_t there = decltype(whole)::value ? 8 : left;
 #pragma unroll 4
     for (int64_t r = s * strip + sub; r < r1; r += 4) {
       float g[8];
-      load_n<T, 8>(g, dy + r * ldy + c, left);
+      load_n<T, 8>(g, dy + r * ldy + c, there);
       if (act == QNN_ACT_RELU) {
         const unsigned on = ((const uint8_t*)slope)[r * ((n + 7) / 8) + c / 8];
 #pragma unroll
@@ -459,11 +487,11 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, int64_t ldy
       } else if (act == QNN_ACT_GELU) {
         if constexpr (sizeof(T) == 4) {
           float d[8];
-          load_n<float, 8>(d, (const float*)slope + r * n + c, left);
+          load_n<float, 8>(d, (const float*)slope + r * n + c, there);
 #pragma unroll
           for (int i = 0; i < 8; ++i) g[i] *= d[i];
         } else {
-          const Vec<int16_t, 8> q = load_group((const int16_t*)slope + r * n + c, left);
+          const Vec<int16_t, 8> q = load_group((const int16_t*)slope + r * n + c, there);
 #pragma unroll
           for (int i = 0; i < 8; ++i) g[i] *= slope_unpack(q.v[i]);
         }
@@ -473,9 +501,11 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, int64_t ldy
         g[i] = (float)(T)g[i];  // db is the sum of dz as it is written
         sum[i] += g[i];
       }
-      if (dz) store_n<T, 8>(dz + r * n + c, g, left);
+      if (dz) store_n<T, 8>(dz + r * n + c, g, there);
     }
-  }
+  };
+  if ((blockIdx.x % chunks + 1) * 512 <= n) rows(std::true_type{});  // all of the workgroup's columns are there
+  else if (left > 0) rows(std::false_type{});
   if (!part) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sh[sub][lane][i] = sum[i];
