@@ -180,15 +180,31 @@ __global__ __launch_bounds__(WIDE) void distill_part_kernel(const T* s, int64_t 
   if (threadIdx.x == 0) part[(int64_t)blockIdx.x] = a;
 }
 
-template <class T>
-__global__ __launch_bounds__(NT) void distill_split_rows_kernel(const T* s, int64_t lds, Entries en, int64_t rows,
-                                                                int64_t vocab, float temp, int splits,
-                                                                const Run* part, float* row_loss, float* stats) {
+// The rows' statistics from their pieces' runs, a wave a row.  ALL: the launch is one workgroup that has
+// every row, and gives the loss too.
+constexpr int ALL_ROWS = 16;
+template <class T, bool ALL>
+__global__ __launch_bounds__(ALL ? 64 * ALL_ROWS : NT) void distill_split_rows_kernel(
+    const T* s, int64_t lds, Entries en, int64_t rows, int64_t vocab, float temp, int splits, const Run* part,
+    float* row_loss, float* stats, float* loss, int mean) {
   const int64_t r = (int64_t)blockIdx.x * (NT / 64) + threadIdx.x / 64;
-  if (r >= rows) return;
-  const int lane = threadIdx.x % 64;
-  const Run a = lane < splits ? part[r * splits + lane] : Run{-INFINITY, 0.0f};
-  finish_row<T, 64>(s + r * lds, a, en, r, vocab, temp, lane, row_loss, stats);
+  if (r < rows) {
+    const int lane = threadIdx.x % 64;
+    const Run a = lane < splits ? part[r * splits + lane] : Run{-INFINITY, 0.0f};
+    finish_row<T, 64>(s + r * lds, a, en, r, vocab, temp, lane, row_loss, stats);
+  }
+  if constexpr (ALL) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double a = 0.0, n = 0.0;
+      for (int k = 0; k < (int)rows; ++k) {
+        a += (double)row_loss[k];
+        n += stats[4 * k + 3] != 0.0f ? 1.0 : 0.0;
+      }
+      stats[4 * rows] = (float)n;
+      if (loss) loss[0] = (float)(mean ? a / (n > 0.0 ? n : 1.0) : a);
+    }
+  }
 }
 
 __global__ __launch_bounds__(NT) void distill_join_kernel(const float* row_loss, float* stats, float* loss,
@@ -341,9 +357,10 @@ int qnn_topk_distill_fwd(const void* s, int64_t lds, const void* t, int64_t ldt,
   QNN_REQUIRE(rows == 0 || row_loss, "null pointer");
   const Entries en = {t, ldt, index, ldi, (int)top, tdtype, index_bytes};
   hipStream_t st = (hipStream_t)stream;
+  const int splits = splits_of(rows, vocab, dtype);
+  const bool all = splits > 1 && rows <= ALL_ROWS;
   const int rc = with_type(dtype, [&](auto z) {
     using T = decltype(z);
-    const int splits = splits_of(rows, vocab, dtype);
     if (rows == 0) return (int)QNN_OK;
     if (splits > 1) {
       QNN_REQUIRE(work && work_bytes >= rows * splits * (int64_t)sizeof(Run),
@@ -353,8 +370,13 @@ int qnn_topk_distill_fwd(const void* s, int64_t lds, const void* t, int64_t ldt,
       hipLaunchKernelGGL((distill_part_kernel<T>), dim3((unsigned)(rows * splits)), dim3(WIDE), 0, st, (const T*)s, lds,
                          vocab, temp, splits, piece, (Run*)work);
       QNN_LAUNCH_CHECK("qnn_topk_distill_fwd");
-      hipLaunchKernelGGL((distill_split_rows_kernel<T>), dim3((unsigned)cdiv(rows, NT / 64)), dim3(NT), 0, st,
-                         (const T*)s, lds, en, rows, vocab, temp, splits, (const Run*)work, row_loss, stats);
+      if (all)
+        hipLaunchKernelGGL((distill_split_rows_kernel<T, true>), dim3(1), dim3(64 * ALL_ROWS), 0, st, (const T*)s, lds, en,
+                           rows, vocab, temp, splits, (const Run*)work, row_loss, stats, loss, mean);
+      else
+        hipLaunchKernelGGL((distill_split_rows_kernel<T, false>), dim3((unsigned)cdiv(rows, NT / 64)), dim3(NT), 0, st,
+                           (const T*)s, lds, en, rows, vocab, temp, splits, (const Run*)work, row_loss, stats, loss,
+                           mean);
     } else if (vocab * (int64_t)sizeof(T) <= WAVE_BYTES) {
       hipLaunchKernelGGL((distill_rows_kernel<T, 64>), dim3((unsigned)cdiv(rows, NT / 64)), dim3(NT), 0, st,
                          (const T*)s, lds, en, rows, vocab, temp, row_loss, stats);
@@ -365,7 +387,7 @@ int qnn_topk_distill_fwd(const void* s, int64_t lds, const void* t, int64_t ldt,
     QNN_LAUNCH_CHECK("qnn_topk_distill_fwd");
     return (int)QNN_OK;
   });
-  if (rc) return rc;
+  if (rc || all) return rc;
   hipLaunchKernelGGL(distill_join_kernel, dim3(1), dim3(NT), 0, st, row_loss, stats, loss, rows, mean);
   QNN_LAUNCH_CHECK("qnn_topk_distill_fwd");
   return QNN_OK;

@@ -445,15 +445,26 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(const T* x, int64_t ld
 }
 
 // ------------------------------------------------------------------------------ rows on boundaries
-// A matrix whose rows are no whole number of 16-byte groups, with rows of ldo that are, zeros behind
-// them: what the tiled product's loads take.
+// Matrices whose rows are no whole number of 16-byte groups, with rows that are, zeros behind them: what
+// the tiled product's loads take.  Up to three in one launch.  Bound by memory (15 MB of fp16 in 7 us).
+struct Padding {
+  int count;
+  struct One {
+    const void* from;
+    void* to;
+    int64_t ld, rows, cols, per, blocks;  // per: groups of an output row
+  } one[3];
+};
 template <class T>
-__global__ __launch_bounds__(256) void pad_rows_kernel(const T* x, int64_t ld, int64_t rows, int64_t cols, T* out,
-                                                       int64_t ldo) {
+__global__ __launch_bounds__(256) void pad_rows_kernel(Padding p) {
   constexpr int GR = GROUP<T>;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, per = ldo / GR, row = at / per, c = at % per * GR;
-  if (row >= rows) return;
-  store_group(out + row * ldo + c, load_group(x + row * ld + c, cols - c), GR);
+  int64_t block = blockIdx.x;
+  int which = 0;
+  while (which + 1 < p.count && block >= p.one[which].blocks) block -= p.one[which++].blocks;
+  const Padding::One& o = p.one[which];
+  const int64_t at = block * 256 + threadIdx.x, row = at / o.per, c = at % o.per * GR;
+  if (row >= o.rows) return;
+  store_group((T*)o.to + at * GR, load_group((const T*)o.from + row * o.ld + c, o.cols - c), GR);
 }
 
 template <class T>
@@ -463,13 +474,14 @@ __global__ __launch_bounds__(256) void zero_kernel(T* p, int64_t n) {
 }
 
 // -------------------------------------------------------------------------- dz, and the bias's gradient
-// dz = dy act'(z), and this strip of rows' sums of it: 64 lanes with 8 columns each, 4 rows at a time.
-// part: [strips][n] (null: not wanted); dz null: none is to be written (dz is dy).
-template <class T>
-__global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, int64_t ldy, const void* slope, T* dz,
-                                                        float* part, int64_t m, int64_t n, int act, int chunks,
-                                                        int64_t strip) {
-  __shared__ float sh[4][64][9];
+// dz = dy act'(z), and this strip of rows' sums of it: 64 lanes with 8 columns each, SUBS rows at a time.
+// part: [strips][n], or where one strip is all of it db itself (both null: not wanted); dz null: none is
+// to be written (dz is dy).
+template <class T, int SUBS>
+__global__ __launch_bounds__(64 * SUBS) void linear_dz_kernel(const T* dy, int64_t ldy, const void* slope, T* dz,
+                                                              float* part, T* db, int64_t m, int64_t n, int act,
+                                                              int chunks, int64_t strip) {
+  __shared__ float sh[SUBS][64][9];
   const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
   const int64_t c = ((int64_t)(blockIdx.x % chunks) * 64 + lane) * 8, left = n - c;
   const int64_t s = blockIdx.x / chunks, r1 = (s + 1) * strip < m ? (s + 1) * strip : m;
@@ -477,7 +489,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, int64_t ldy
   auto rows = [&](auto whole) {
     const int64_t there = decltype(whole)::value ? 8 : left;
 #pragma unroll 4
-    for (int64_t r = s * strip + sub; r < r1; r += 4) {
+    for (int64_t r = s * strip + sub; r < r1; r += SUBS) {
       float g[8];
       load_n<T, 8>(g, dy + r * ldy + c, there);
       if (act == QNN_ACT_RELU) {
@@ -506,14 +518,17 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, int64_t ldy
   };
   if ((blockIdx.x % chunks + 1) * 512 <= n) rows(std::true_type{});  // all of the workgroup's columns are there
   else if (left > 0) rows(std::false_type{});
-  if (!part) return;
+  if (!part && !db) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sh[sub][lane][i] = sum[i];
   __syncthreads();
   if (sub == 0 && left > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] = sh[0][lane][i] + sh[1][lane][i] + sh[2][lane][i] + sh[3][lane][i];
-    store_n<float, 8>(part + s * n + c, sum, left);
+    for (int k = 1; k < SUBS; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += sh[k][lane][i];
+    if (db) store_n<T, 8>(db + c, sum, left);
+    else store_n<float, 8>(part + s * n + c, sum, left);
   }
 }
 
@@ -640,18 +655,25 @@ int matmul(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m, in
   return launch<T, AD, BD, Small>(oa, ob, p, m, n, k, (float*)part, e, s);
 }
 
-// A matrix as the tiled product takes it: itself, or padded into `room`, of which it takes what it needs.
+// A matrix as the tiled product takes it: itself, or (noted in `pads`) padded into `room`, of which it
+// takes what it needs.
 template <class T>
-int on_boundaries(const void*& p, int64_t& ld, int64_t rows, int64_t cols, char*& room, hipStream_t s) {
-  if (cols % GROUP<T> == 0) return QNN_OK;
-  const int64_t ldo = up(cols, GROUP<T>), blocks = cdiv(rows * (ldo / GROUP<T>), 256);
-  QNN_REQUIRE(blocks < (1LL << 31), "a matrix too large for one call");
-  hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, (const T*)p, ld, rows, cols,
-                     (T*)room, ldo);
-  QNN_LAUNCH_CHECK("pad_rows_kernel");
+void on_boundaries(const void*& p, int64_t& ld, int64_t rows, int64_t cols, char*& room, Padding& pads) {
+  if (cols % GROUP<T> == 0) return;
+  const int64_t per = cdiv(cols, GROUP<T>);
+  pads.one[pads.count++] = {p, room, ld, rows, cols, per, cdiv(rows * per, 256)};
   p = room;
-  ld = ldo;
-  room += up(rows * ldo * (int64_t)sizeof(T), 256);
+  ld = per * GROUP<T>;
+  room += up(rows * ld * (int64_t)sizeof(T), 256);
+}
+template <class T>
+int pad(const Padding& pads, hipStream_t s) {
+  int64_t blocks = 0;
+  for (int i = 0; i < pads.count; ++i) blocks += pads.one[i].blocks;
+  if (blocks == 0) return QNN_OK;
+  QNN_REQUIRE(blocks < (1LL << 31), "a matrix too large for one call");
+  hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, pads);
+  QNN_LAUNCH_CHECK("pad_rows_kernel");
   return QNN_OK;
 }
 
@@ -665,14 +687,17 @@ int64_t fwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
   return padded_bytes(m, k, dtype) + padded_bytes(n, k, dtype) + plan_of(m, n, k, dtype).part_bytes;
 }
 
+// Strips of rows for dz's sums: one of 16 rows at a time for a few rows, which saves the launch that adds
+// the strips up; else enough workgroups of 4 to fill the chip.
 struct Strips {
   int chunks;
   int64_t n, rows;  // strips, and rows in each
 };
 Strips strips_of(int64_t m, int64_t n) {
-  const int64_t chunks = cdiv(n, 512), want = cdiv(1024, chunks), most = cdiv(m, 16);
-  const int64_t s = want < most ? want : most, rows = cdiv(m, s > 0 ? s : 1);
-  return {(int)chunks, m > 0 ? cdiv(m, rows) : 0, rows};
+  const int64_t chunks = cdiv(n, 512);
+  if (m <= 256) return {(int)chunks, m > 0, m};
+  const int64_t want = cdiv(1024, chunks), most = cdiv(m, 16), s = want < most ? want : most, rows = cdiv(m, s);
+  return {(int)chunks, cdiv(m, rows), rows};
 }
 
 int64_t bwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
@@ -743,8 +768,10 @@ int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     char* room = (char*)work;
     const void *px = x, *pw = w;
     int64_t lx = ldx, lw = ldw;
-    if (int rc = on_boundaries<T>(px, lx, m, k, room, s)) return rc;
-    if (int rc = on_boundaries<T>(pw, lw, n, k, room, s)) return rc;
+    Padding pads = {};
+    on_boundaries<T>(px, lx, m, k, room, pads);
+    on_boundaries<T>(pw, lw, n, k, room, pads);
+    if (int rc = pad<T>(pads, s)) return rc;
     return matmul<T, true, true>(px, lx, pw, lw, m, n, k, room, e, dtype, s);
   });
 }
@@ -780,21 +807,27 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
     const void* g = dy;
     int64_t ldg = ldy;
     const Strips st = strips_of(m, n);
+    float* part = db && st.n > 1 ? (float*)room : nullptr;
+    room += up(st.n * n * 4, 256);
     if (m > 0 && (act != QNN_ACT_NONE || db)) {
-      float* part = db ? (float*)room : nullptr;
-      room += up(st.n * n * 4, 256);
       QNN_REQUIRE(st.n * st.chunks < (1LL << 31), "too many rows for one call");
-      hipLaunchKernelGGL((linear_dz_kernel<T>), dim3((unsigned)(st.n * st.chunks)), dim3(256), 0, s, (const T*)dy, ldy,
-                         slope, act != QNN_ACT_NONE ? (T*)dz : nullptr, part, m, n, act, st.chunks, st.rows);
+      auto launch_dz = [&](auto subs) {
+        constexpr int SUBS = decltype(subs)::value;
+        hipLaunchKernelGGL((linear_dz_kernel<T, SUBS>), dim3((unsigned)(st.n * st.chunks)), dim3(64 * SUBS), 0, s,
+                           (const T*)dy, ldy, slope, act != QNN_ACT_NONE ? (T*)dz : nullptr, part,
+                           st.n == 1 ? (T*)db : nullptr, m, n, act, st.chunks, st.rows);
+      };
+      if (st.n == 1) launch_dz(std::integral_constant<int, 16>{});
+      else launch_dz(std::integral_constant<int, 4>{});
       QNN_LAUNCH_CHECK("linear_dz_kernel");
       if (act != QNN_ACT_NONE) {
         g = dz;
         ldg = n;
       }
     }
-    if (db) {
-      hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)cdiv(n, 64)), dim3(256), 0, s, (const float*)work,
-                         (int)st.n, (T*)db, n);
+    if (db && st.n != 1) {  // (no strip: zeros)
+      hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)cdiv(n, 64)), dim3(256), 0, s, part, (int)st.n, (T*)db,
+                         n);
       QNN_LAUNCH_CHECK("linear_db_kernel");
     }
     if (!dx && !dw) return (int)QNN_OK;
@@ -805,14 +838,14 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
       }
       return (int)QNN_OK;
     }
-    if (int rc = on_boundaries<T>(g, ldg, m, n, room, s)) return rc;
+    Padding pads = {};
+    on_boundaries<T>(g, ldg, m, n, room, pads);
     Epilogue e = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE};
     const void *px = x, *pw = w;
     int64_t lx = ldx, lw = ldw;
-    if (dx)
-      if (int rc = on_boundaries<T>(pw, lw, n, k, room, s)) return rc;
-    if (dw)
-      if (int rc = on_boundaries<T>(px, lx, m, k, room, s)) return rc;
+    if (dx) on_boundaries<T>(pw, lw, n, k, room, pads);
+    if (dw) on_boundaries<T>(px, lx, m, k, room, pads);
+    if (int rc = pad<T>(pads, s)) return rc;
     if (dx)
       if (int rc = matmul<T, true, false>(g, ldg, pw, lw, m, k, n, room, e, dtype, s)) return rc;
     e.y = dw;
