@@ -43,6 +43,19 @@ __device__ __forceinline__ Vec<T, GROUP<T>> load_group(const T* p, int64_t left)
   return o;
 }
 
+// The same of 8 elements: one group of a 16-bit type, two of fp32.
+template <class T>
+__device__ __forceinline__ Vec<T, 8> load_eight(const T* p, int64_t left) {
+  Vec<T, 8> o;
+#pragma unroll
+  for (int g = 0; g < 8 / GROUP<T>; ++g) {
+    const Vec<T, GROUP<T>> t = load_group(p + g * GROUP<T>, left - g * GROUP<T>);
+#pragma unroll
+    for (int i = 0; i < GROUP<T>; ++i) o.v[g * GROUP<T> + i] = t.v[i];
+  }
+  return o;
+}
+
 template <class T>
 __device__ __forceinline__ void store_group(T* p, const Vec<T, GROUP<T>>& o, int64_t left) {
   if (left >= GROUP<T>) {

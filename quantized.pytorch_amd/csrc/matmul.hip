@@ -69,6 +69,7 @@ __device__ __forceinline__ void finish8(float (&z)[8], const float (&bias)[8], c
 // c[i][j] = sum over k of a(i, k) b(j, k).  An operand is DENSE in k ([rows][k], as x and w in the
 // forward pass) or not ([k][rows], as both of dz^T x): then its rows are what is contiguous in memory.
 //
+// (linear_y_kernel: the forward pass; linear_grads_kernel: both products of the backward pass.)
 // A workgroup of WM x WN waves computes a (16 TM WM) x (16 TN WN) tile, a wave (16 TM) x (16 TN) of it
 // in 16x16 MFMAs.  k advances in stages of 64 bytes (32 elements of 16 bits, 16 of 32) through a ring
 // of 4 LDS slots that direct loads fill (buffer_load ... lds, 16 bytes a lane), three stages ahead; a
@@ -214,21 +215,25 @@ __device__ __forceinline__ f4 mma(f4 a, f4 b, f4 acc) {
   }
 }
 
-// Where a tile's sums go: through the epilogue, or (splits > 1) as they are into part[split][m][ldp].
-struct Tiles {
+// One product, as a launch's workgroups take it.  Its tiles' sums go through the epilogue, or (splits > 1)
+// as they are into part[split][m][ldp].
+struct Product {
+  Operand a, b;
   int64_t m, n, k;
   int tm, tn;        // tiles
   int splits;
+  int blocks;        // tm tn splits
   int64_t span;      // elements of k in a split, a whole number of stages
   float* part;
   int64_t ldp;
+  Epilogue e;
 };
 
 // Workgroup -> (split, tile row, tile column).  The card deals workgroups out to its 8 XCDs in turn; each
 // XCD gets a run of neighbouring tiles, 8 tile rows at a time, so that the panels they share meet in
 // its L2.
-__device__ __forceinline__ void tile_of(const Tiles& t, int& split, int& ti, int& tj) {
-  const int all = t.tm * t.tn * t.splits, id = blockIdx.x, x = id & 7, q = all >> 3, r = all & 7;
+__device__ __forceinline__ void tile_of(const Product& t, int id, int& split, int& ti, int& tj) {
+  const int x = id & 7, q = t.blocks >> 3, r = t.blocks & 7;
   const int lin = x * q + (x < r ? x : r) + (id >> 3);
   const int tiles = t.tm * t.tn;
   split = lin / tiles;
@@ -244,15 +249,17 @@ struct Cfg {
   static constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN, SLOT = (BM + BN) * 64, LDS = 4 * SLOT;
 };
 
+// Workgroup `id` of the product's.
 template <class T, bool AD, bool BD, class C>
-__global__ __launch_bounds__(C::NT, C::EU) void matmul_kernel(Operand a, Operand b, Tiles t, Epilogue e) {
+__device__ __forceinline__ void tile(const Product& t, int id) {
   using A = Side<T, AD, C::BM, C::W>;
   using B = Side<T, BD, C::BN, C::W>;
   constexpr int TM = C::TM, TN = C::TN, KE = A::KE, P = A::LOADS + B::LOADS;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const Epilogue& e = t.e;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int split, ti, tj;
-  tile_of(t, split, ti, tj);
+  tile_of(t, id, split, ti, tj);
   const int64_t i0 = (int64_t)ti * C::BM, j0 = (int64_t)tj * C::BN, k0 = split * t.span;
   int left = (int)(t.k - k0 < t.span ? t.k - k0 : t.span);
   const int stages = (left + KE - 1) / KE;
@@ -260,8 +267,8 @@ __global__ __launch_bounds__(C::NT, C::EU) void matmul_kernel(Operand a, Operand
 
   A sa;
   B sb;
-  sa.begin(a, i0, k0, wave, lane);
-  sb.begin(b, j0, k0, wave, lane);
+  sa.begin(t.a, i0, k0, wave, lane);
+  sb.begin(t.b, j0, k0, wave, lane);
   auto load = [&](int slot, int j) {  // load j of P of the next stage
     if (j < A::LOADS) sa.load(lds + slot * C::SLOT, j, left, wave);
     else sb.load(lds + slot * C::SLOT + A::BYTES, j - A::LOADS, left, wave);
@@ -370,22 +377,45 @@ __global__ __launch_bounds__(C::NT, C::EU) void matmul_kernel(Operand a, Operand
   }
 }
 
-// The splits' sums, in their order, through the epilogue: 8 columns a thread.
+template <class T, class C>
+__global__ __launch_bounds__(C::NT, C::EU) void linear_y_kernel(Product y) {
+  tile<T, true, true, C>(y, blockIdx.x);
+}
+
+// dx = dz w and dw = dz^T x in one launch, so that the one's last tiles and the other's first share the
+// chip.  The first's workgroups are counted up to a multiple of 8, which keeps the second's on the XCDs
+// that tile_of takes them to be on; a product with no workgroups is not wanted.
+template <class T, class C>
+__global__ __launch_bounds__(C::NT, C::EU) void linear_grads_kernel(Product dx, Product dw, int dw_first) {
+  const int lead = ((dw_first ? dw.blocks : dx.blocks) + 7) & ~7, id = blockIdx.x;
+  const bool is_dw = (id < lead) == (dw_first != 0);
+  const int at = id < lead ? id : id - lead;
+  if (at >= (is_dw ? dw.blocks : dx.blocks)) return;
+  if (is_dw) tile<T, false, false, C>(dw, at);
+  else tile<T, true, false, C>(dx, at);
+}
+
+// The splits' sums of up to two products, in their order, through the epilogue: 8 columns a thread.
+struct Joins {
+  Product p[2];
+  int64_t blocks[2];  // 0: not split
+};
 template <class T>
-__global__ __launch_bounds__(256) void matmul_join_kernel(const float* part, int splits, int64_t m, int64_t n,
-                                                          int64_t ldp, Epilogue e) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, per = ldp / 8, row = at / per, col = at % per * 8;
-  if (row >= m) return;
-  float z[8], v[8];
-  load_n<float, 8>(z, part + row * ldp + col, 8);
-  for (int s = 1; s < splits; ++s) {
-    load_n<float, 8>(v, part + (s * m + row) * ldp + col, 8);
+__global__ __launch_bounds__(256) void matmul_join_kernel(Joins j) {
+  const bool second = blockIdx.x >= j.blocks[0];
+  const Product& t = second ? j.p[1] : j.p[0];
+  const int64_t at = (blockIdx.x - (second ? j.blocks[0] : 0)) * 256 + threadIdx.x, per = t.ldp / 8;
+  const int64_t row = at / per, col = at % per * 8;
+  if (row >= t.m) return;
+  float z[8], v[8], bias[8];
+  load_n<float, 8>(z, t.part + row * t.ldp + col, 8);
+  for (int s = 1; s < t.splits; ++s) {
+    load_n<float, 8>(v, t.part + (s * t.m + row) * t.ldp + col, 8);
 #pragma unroll
     for (int i = 0; i < 8; ++i) z[i] += v[i];
   }
-  float bias[8];
-  bias8<T>(bias, e, col, n);
-  finish8<T, false>(z, bias, e, row, col, n);
+  bias8<T>(bias, t.e, col, t.n);
+  finish8<T, false>(z, bias, t.e, row, col, t.n);
 }
 
 // ------------------------------------------------------------------------- few rows: the weight is all
@@ -474,13 +504,17 @@ __global__ __launch_bounds__(256) void zero_kernel(T* p, int64_t n) {
 }
 
 // -------------------------------------------------------------------------- dz, and the bias's gradient
-// dz = dy act'(z), and this strip of rows' sums of it: 64 lanes with 8 columns each, SUBS rows at a time.
-// part: [strips][n], or where one strip is all of it db itself (both null: not wanted); dz null: none is
-// to be written (dz is dy).
-template <class T, int SUBS>
-__global__ __launch_bounds__(64 * SUBS) void linear_dz_kernel(const T* dy, int64_t ldy, const void* slope, T* dz,
-                                                              float* part, T* db, int64_t m, int64_t n, int act,
-                                                              int chunks, int64_t strip) {
+// dz = dy act'(z), and this strip of rows' sums of it: 64 lanes with 8 columns each, SUBS rows at a time,
+// 4 of a lane's rows on their way together.  part: [strips][n], or where one strip is all of it db itself
+// (both null: not wanted).  Without an activation dz is dy and is not written.  Bound by memory: 8192 x 8192 bf16
+// of GELU in 81 us (dy, slopes and dz: 5.0 TB/s).
+template <class T, int SUBS, int ACT>
+__global__ __launch_bounds__(64 * SUBS) void linear_dz_kernel(const T* __restrict__ dy, int64_t ldy,
+                                                              const void* __restrict__ slope, T* __restrict__ dz,
+                                                              float* __restrict__ part, T* __restrict__ db, int64_t m,
+                                                              int64_t n, int chunks, int64_t strip) {
+  constexpr int U = 4;
+  using Slope = std::conditional_t<ACT == QNN_ACT_RELU, uint8_t, std::conditional_t<sizeof(T) == 4, float, int16_t>>;
   __shared__ float sh[SUBS][64][9];
   const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
   const int64_t c = ((int64_t)(blockIdx.x % chunks) * 64 + lane) * 8, left = n - c;
@@ -488,32 +522,32 @@ __global__ __launch_bounds__(64 * SUBS) void linear_dz_kernel(const T* dy, int64
   float sum[8] = {};
   auto rows = [&](auto whole) {
     const int64_t there = decltype(whole)::value ? 8 : left;
-#pragma unroll 4
-    for (int64_t r = s * strip + sub; r < r1; r += SUBS) {
-      float g[8];
-      load_n<T, 8>(g, dy + r * ldy + c, there);
-      if (act == QNN_ACT_RELU) {
-        const unsigned on = ((const uint8_t*)slope)[r * ((n + 7) / 8) + c / 8];
+    for (int64_t r = s * strip + sub; r < r1; r += U * SUBS) {
+      Vec<T, 8> g[U];
+      Vec<Slope, 8> d[U];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = on >> i & 1 ? g[i] : 0.0f;
-      } else if (act == QNN_ACT_GELU) {
-        if constexpr (sizeof(T) == 4) {
-          float d[8];
-          load_n<float, 8>(d, (const float*)slope + r * n + c, there);
+      for (int u = 0; u < U; ++u) {  // (past the last row: that one again, which is not used)
+        const int64_t k = r + u * SUBS < r1 ? r + u * SUBS : r1 - 1;
+        g[u] = load_eight(dy + k * ldy + c, there);
+        if constexpr (ACT == QNN_ACT_RELU) d[u].v[0] = ((const uint8_t*)slope)[k * ((n + 7) / 8) + c / 8];
+        else if constexpr (ACT == QNN_ACT_GELU) d[u] = load_eight((const Slope*)slope + k * n + c, there);
+      }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] *= d[i];
-        } else {
-          const Vec<int16_t, 8> q = load_group((const int16_t*)slope + r * n + c, there);
+      for (int u = 0; u < U; ++u) {
+        const int64_t k = r + u * SUBS;
+        if (k >= r1) break;
+        float v[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] *= slope_unpack(q.v[i]);
+        for (int i = 0; i < 8; ++i) {
+          v[i] = (float)g[u].v[i];
+          if constexpr (ACT == QNN_ACT_RELU) v[i] = d[u].v[0] >> i & 1 ? v[i] : 0.0f;
+          else if constexpr (ACT == QNN_ACT_GELU && sizeof(T) == 4) v[i] *= d[u].v[i];
+          else if constexpr (ACT == QNN_ACT_GELU) v[i] *= slope_unpack(d[u].v[i]);
+          v[i] = (float)(T)v[i];  // db is the sum of dz as it is written
+          sum[i] += v[i];
         }
+        if (ACT != QNN_ACT_NONE) store_n<T, 8>(dz + k * n + c, v, there);
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        g[i] = (float)(T)g[i];  // db is the sum of dz as it is written
-        sum[i] += g[i];
-      }
-      if (dz) store_n<T, 8>(dz + r * n + c, g, there);
     }
   };
   if ((blockIdx.x % chunks + 1) * 512 <= n) rows(std::true_type{});  // all of the workgroup's columns are there
@@ -568,91 +602,155 @@ constexpr Shape SHAPES[] = {{Big::BM, Big::BN, 0.72f, 0.0f, 10.0f, 1.0f},
                             {Half::BM, Half::BN, 0.19f, 0.50f, 4.0f, 1.0f},
                             {Small::BM, Small::BN, 0.105f, 0.25f, 4.0f, 1.2f}};
 
-struct Plan {
-  int cfg;      // of SHAPES
-  int splits;
-  int64_t span;  // elements of k in a split
-  int64_t ldp;
-  int64_t part_bytes;
-};
-
 int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
-// The tile and the splits of k of one product: the least of the times above, for as many turns as the
-// busiest of 256 CUs takes; splits cost a second launch (5.5 us with its host time) and their sums' way
+struct Split {
+  int n;         // splits of k
+  int64_t span;  // elements of k in each
+  int64_t ldp, bytes;
+};
+struct Size {
+  int64_t m, n, k;
+};
+struct Plan {
+  int shape;  // of SHAPES, for all products of the launch
+  Split split[2];
+};
+
+// The tile and the splits of k of the one or two products of a launch: the least of the times above for
+// the busiest of 256 CUs; splits cost a second launch (5.5 us with its host time) and their sums' way
 // through memory (at 4 TB/s).  Over the sizes that were swept (m, n 64 to 8192, k 64 to 8192) what it
-// picks is within 10 % of the best pair, 20 % where the whole takes under 20 us.
-Plan plan_of(int64_t m, int64_t n, int64_t k, int dtype) {
-  const int64_t ke = 64 / type_bytes(dtype), stages = cdiv(k, ke);
-  Plan p = {};
-  float best = INFINITY;
+// picks for one product is within 10 % of the best pair, 20 % where the whole takes under 20 us.
+Plan plan_of(const Size* size, int count, int dtype) {
+  const int64_t ke = 64 / type_bytes(dtype);
+  Plan best = {};
+  float least = INFINITY;
   for (int c = dtype == QNN_F32 ? 1 : 0; c < 4; ++c) {
     const Shape& h = SHAPES[c];
-    const int64_t tiles = cdiv(m, h.bm) * cdiv(n, h.bn);
-    const float stage = dtype == QNN_F32 ? h.stage32 : h.stage16;
-    for (int turns = 0; turns <= 3; ++turns) {  // 0: no split; else as many as fill the CUs so many times
-      int64_t s = turns == 0 ? 1 : 256 * turns / tiles;
-      if (turns > 0 && s < 2) continue;
-      if (s > stages / 4) s = stages / 4;
-      if (s > 32) s = 32;
-      if (s < 1) s = 1;
-      const int64_t each = cdiv(stages, s), splits = cdiv(stages, each);
-      const float busiest = (float)cdiv(tiles * splits, 256);
-      float us = fmaxf(busiest, dtype == QNN_F32 ? 1.0f : h.alone) * (float)each * stage + busiest * 0.6f * h.ends + 0.4f * h.ends;
-      if (splits > 1) us += 5.5f + (float)(splits * m * n) * 2e-6f;
-      if (us < best) {
-        best = us;
-        p.cfg = c;
-        p.splits = (int)splits;
-        p.span = each * ke;
+    const float stage = dtype == QNN_F32 ? h.stage32 : h.stage16, alone = dtype == QNN_F32 ? 1.0f : h.alone;
+    int64_t tiles[2], stages[2];
+    for (int i = 0; i < count; ++i) {
+      tiles[i] = cdiv(size[i].m, h.bm) * cdiv(size[i].n, h.bn);
+      stages[i] = cdiv(size[i].k, ke);
+    }
+    // a split for each product: none, or as many as give it so many workgroups
+    constexpr int WANT[] = {0, 128, 256, 512};
+    for (int x = 0; x < (count > 1 ? 16 : 4); ++x) {
+      int64_t each[2], n[2];
+      float work = 0.0f, longest = 0.0f, shortest = INFINITY, us = 0.0f;
+      int64_t blocks = 0;
+      bool skip = false, split = false;
+      for (int i = 0; i < count; ++i) {
+        const int want = WANT[i ? x / 4 : x % 4];
+        int64_t s = want / tiles[i];
+        if (s > stages[i] / 4) s = stages[i] / 4;
+        if (s > 32) s = 32;
+        skip = skip || (want > 0 && s < 2);
+        if (s < 1) s = 1;
+        each[i] = cdiv(stages[i], s);
+        n[i] = cdiv(stages[i], each[i]);
+        blocks += tiles[i] * n[i];
+        work += (float)(tiles[i] * n[i]) * (float)each[i];
+        longest = fmaxf(longest, (float)each[i]);
+        shortest = fminf(shortest, (float)each[i]);
+        split = split || n[i] > 1;
+        if (n[i] > 1) us += (float)(n[i] * size[i].m * size[i].n) * 2e-6f;
+      }
+      if (skip) continue;
+      const float turns = (float)cdiv(blocks, 256);
+      // in whole turns of the longest, or evenly but for the end, where the shortest ones are
+      const float most = fmaxf(longest * alone, fminf(turns * longest, work / 256.0f + 0.6f * shortest));
+      us += most * stage + (0.6f * turns + 0.4f) * h.ends + (split ? 5.5f : 0.0f);
+      if (us < least) {
+        least = us;
+        best.shape = c;
+        for (int i = 0; i < count; ++i) {
+          const int64_t ldp = up(size[i].n, 8);
+          best.split[i] = {(int)n[i], each[i] * ke, ldp, n[i] > 1 ? up(n[i] * size[i].m * ldp * 4, 256) : 0};
+        }
       }
     }
   }
-  p.ldp = up(n, 8);
-  p.part_bytes = p.splits > 1 ? p.splits * m * p.ldp * 4 : 0;
-  return p;
+  return best;
 }
 
 constexpr int FEW = 16;  // rows of x that few_rows_kernel takes
 
-template <class T, bool AD, bool BD, class C>
-int launch(const Operand& a, const Operand& b, const Plan& p, int64_t m, int64_t n, int64_t k, float* part,
-           const Epilogue& e, hipStream_t s) {
-  const int64_t tm = cdiv(m, C::BM), tn = cdiv(n, C::BN);
-  QNN_REQUIRE(tm * tn * p.splits < (1LL << 31) && tn < (1LL << 27), "too many tiles for one call");
-  const Tiles t = {m, n, k, (int)tm, (int)tn, p.splits, p.span, part, p.ldp};
-  if constexpr (C::LDS > 65536) {
-    static std::atomic<uint64_t> told{0};  // devices whose runtime knows that this kernel takes more than 64 KiB
-    int dev = 0;
-    if (hipError_t er = hipGetDevice(&dev); er != hipSuccess) return hip_check(er, "hipGetDevice");
-    if (dev >= 64 || !(told.load(std::memory_order_relaxed) >> dev & 1)) {
-      if (hipError_t er = hipFuncSetAttribute((const void*)&matmul_kernel<T, AD, BD, C>, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
-          er != hipSuccess)
-        return hip_check(er, "hipFuncSetAttribute");
-      if (dev < 64) told.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
-  }
-  hipLaunchKernelGGL((matmul_kernel<T, AD, BD, C>), dim3((unsigned)(tm * tn * p.splits)), dim3(C::NT), C::LDS, s, a, b, t, e);
-  QNN_LAUNCH_CHECK("matmul_kernel");
-  if (p.splits > 1) {
-    hipLaunchKernelGGL((matmul_join_kernel<T>), dim3((unsigned)cdiv(m * (p.ldp / 8), 256)), dim3(256), 0, s, part,
-                       p.splits, m, n, p.ldp, e);
-    QNN_LAUNCH_CHECK("matmul_join_kernel");
-  }
+// The plan's product i of c = a b^T; its sums' scratch is taken from room.
+int product_of(Product& p, const Plan& plan, int i, const Size& z, const Operand& a, const Operand& b,
+               const Epilogue& e, char*& room) {
+  const Shape& h = SHAPES[plan.shape];
+  const Split& s = plan.split[i];
+  const int64_t tm = cdiv(z.m, h.bm), tn = cdiv(z.n, h.bn);
+  QNN_REQUIRE(tm * tn * s.n < (1LL << 30) && tn < (1LL << 27), "too many tiles for one call");
+  p = {a, b, z.m, z.n, z.k, (int)tm, (int)tn, s.n, (int)(tm * tn * s.n), s.span, (float*)room, s.ldp, e};
+  room += s.bytes;
   return QNN_OK;
 }
 
-// c = a b^T; part: scratch of plan_of(m, n, k).part_bytes
-template <class T, bool AD, bool BD>
-int matmul(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t m, int64_t n, int64_t k, void* part,
-           const Epilogue& e, int dtype, hipStream_t s) {
-  const Plan p = plan_of(m, n, k, dtype);
-  const Operand oa = {a, lda, m}, ob = {b, ldb, n};
+// More than 64 KiB of LDS: said once for each kernel and device.
+int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& told) {
+  if (bytes <= 65536) return QNN_OK;
+  int dev = 0;
+  if (hipError_t er = hipGetDevice(&dev); er != hipSuccess) return hip_check(er, "hipGetDevice");
+  if (dev < 64 && (told.load(std::memory_order_relaxed) >> dev & 1)) return QNN_OK;
+  if (hipError_t er = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); er != hipSuccess)
+    return hip_check(er, "hipFuncSetAttribute");
+  if (dev < 64) told.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return QNN_OK;
+}
+
+template <class T, class F>
+int with_cfg(int shape, F&& f) {
   if constexpr (sizeof(T) == 2)
-    if (p.cfg == 0) return launch<T, AD, BD, Big>(oa, ob, p, m, n, k, (float*)part, e, s);
-  if (p.cfg == 1) return launch<T, AD, BD, Middle>(oa, ob, p, m, n, k, (float*)part, e, s);
-  if (p.cfg == 2) return launch<T, AD, BD, Half>(oa, ob, p, m, n, k, (float*)part, e, s);
-  return launch<T, AD, BD, Small>(oa, ob, p, m, n, k, (float*)part, e, s);
+    if (shape == 0) return f(Big{});
+  if (shape == 1) return f(Middle{});
+  if (shape == 2) return f(Half{});
+  return f(Small{});
+}
+
+template <class T>
+int join(const Product* p, int count, hipStream_t s) {
+  Joins j = {};
+  for (int i = 0; i < count; ++i) {
+    j.p[i] = p[i];
+    if (p[i].blocks > 0 && p[i].splits > 1) j.blocks[i] = cdiv(p[i].m * (p[i].ldp / 8), 256);
+  }
+  const int64_t blocks = j.blocks[0] + j.blocks[1];
+  if (blocks == 0) return QNN_OK;
+  QNN_REQUIRE(blocks < (1LL << 31), "too many rows for one call");
+  hipLaunchKernelGGL((matmul_join_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, j);
+  QNN_LAUNCH_CHECK("matmul_join_kernel");
+  return QNN_OK;
+}
+
+template <class T>
+int launch_y(int shape, const Product& y, hipStream_t s) {
+  const int rc = with_cfg<T>(shape, [&](auto cfg) {
+    using C = decltype(cfg);
+    static std::atomic<uint64_t> told{0};
+    if (int rc = allow_lds((const void*)&linear_y_kernel<T, C>, C::LDS, told)) return rc;
+    hipLaunchKernelGGL((linear_y_kernel<T, C>), dim3((unsigned)y.blocks), dim3(C::NT), C::LDS, s, y);
+    QNN_LAUNCH_CHECK("linear_y_kernel");
+    return (int)QNN_OK;
+  });
+  return rc ? rc : join<T>(&y, 1, s);
+}
+
+// p: dx, dw (no blocks: not wanted); the one whose workgroups take longer goes first
+template <class T>
+int launch_grads(int shape, const Product (&p)[2], hipStream_t s) {
+  const int rc = with_cfg<T>(shape, [&](auto cfg) {
+    using C = decltype(cfg);
+    static std::atomic<uint64_t> told{0};
+    if (int rc = allow_lds((const void*)&linear_grads_kernel<T, C>, C::LDS, told)) return rc;
+    const int first = p[1].blocks > 0 && (p[0].blocks == 0 || p[1].span > p[0].span) ? 1 : 0;
+    const unsigned blocks = (unsigned)up(p[first].blocks, 8) + (unsigned)p[1 - first].blocks;
+    hipLaunchKernelGGL((linear_grads_kernel<T, C>), dim3(blocks), dim3(C::NT), C::LDS, s, p[0], p[1], first);
+    QNN_LAUNCH_CHECK("linear_grads_kernel");
+    return (int)QNN_OK;
+  });
+  return rc ? rc : join<T>(p, 2, s);
 }
 
 // A matrix as the tiled product takes it: itself, or (noted in `pads`) padded into `room`, of which it
@@ -684,7 +782,8 @@ int64_t padded_bytes(int64_t rows, int64_t cols, int dtype) {
 
 int64_t fwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
   if (m <= FEW) return 0;
-  return padded_bytes(m, k, dtype) + padded_bytes(n, k, dtype) + plan_of(m, n, k, dtype).part_bytes;
+  const Size y = {m, n, k};
+  return padded_bytes(m, k, dtype) + padded_bytes(n, k, dtype) + plan_of(&y, 1, dtype).split[0].bytes;
 }
 
 // Strips of rows for dz's sums: one of 16 rows at a time for a few rows, which saves the launch that adds
@@ -702,9 +801,10 @@ Strips strips_of(int64_t m, int64_t n) {
 
 int64_t bwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
   if (m == 0) return 0;
-  const int64_t dx = plan_of(m, k, n, dtype).part_bytes, dw = plan_of(n, k, m, dtype).part_bytes;
+  const Size grads[2] = {{m, k, n}, {n, k, m}};
+  const Plan p = plan_of(grads, 2, dtype);
   return padded_bytes(m, n, dtype) + padded_bytes(n, k, dtype) + padded_bytes(m, k, dtype) +
-         up(strips_of(m, n).n * n * 4, 256) + (dx > dw ? dx : dw);
+         up(strips_of(m, n).n * n * 4, 256) + p.split[0].bytes + p.split[1].bytes;
 }
 
 constexpr int64_t LONGEST = 1LL << 21;  // of a row stride: offsets inside a tile's rows are 32 bits
@@ -772,7 +872,11 @@ int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     on_boundaries<T>(px, lx, m, k, room, pads);
     on_boundaries<T>(pw, lw, n, k, room, pads);
     if (int rc = pad<T>(pads, s)) return rc;
-    return matmul<T, true, true>(px, lx, pw, lw, m, n, k, room, e, dtype, s);
+    const Size z = {m, n, k};
+    const Plan plan = plan_of(&z, 1, dtype);
+    Product p;
+    if (int rc = product_of(p, plan, 0, z, {px, lx, m}, {pw, lw, n}, e, room)) return rc;
+    return launch_y<T>(plan.shape, p, s);
   });
 }
 
@@ -811,14 +915,19 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
     room += up(st.n * n * 4, 256);
     if (m > 0 && (act != QNN_ACT_NONE || db)) {
       QNN_REQUIRE(st.n * st.chunks < (1LL << 31), "too many rows for one call");
-      auto launch_dz = [&](auto subs) {
-        constexpr int SUBS = decltype(subs)::value;
-        hipLaunchKernelGGL((linear_dz_kernel<T, SUBS>), dim3((unsigned)(st.n * st.chunks)), dim3(64 * SUBS), 0, s,
-                           (const T*)dy, ldy, slope, act != QNN_ACT_NONE ? (T*)dz : nullptr, part,
-                           st.n == 1 ? (T*)db : nullptr, m, n, act, st.chunks, st.rows);
+      auto launch_dz = [&](auto subs, auto of) {
+        constexpr int SUBS = decltype(subs)::value, ACT = decltype(of)::value;
+        hipLaunchKernelGGL((linear_dz_kernel<T, SUBS, ACT>), dim3((unsigned)(st.n * st.chunks)), dim3(64 * SUBS), 0, s,
+                           (const T*)dy, ldy, slope, (T*)dz, part, st.n == 1 ? (T*)db : nullptr, m, n, st.chunks,
+                           st.rows);
       };
-      if (st.n == 1) launch_dz(std::integral_constant<int, 16>{});
-      else launch_dz(std::integral_constant<int, 4>{});
+      auto with_subs = [&](auto of) {
+        if (st.n == 1) launch_dz(std::integral_constant<int, 16>{}, of);
+        else launch_dz(std::integral_constant<int, 4>{}, of);
+      };
+      if (act == QNN_ACT_RELU) with_subs(std::integral_constant<int, QNN_ACT_RELU>{});
+      else if (act == QNN_ACT_GELU) with_subs(std::integral_constant<int, QNN_ACT_GELU>{});
+      else with_subs(std::integral_constant<int, QNN_ACT_NONE>{});
       QNN_LAUNCH_CHECK("linear_dz_kernel");
       if (act != QNN_ACT_NONE) {
         g = dz;
@@ -840,17 +949,22 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
     }
     Padding pads = {};
     on_boundaries<T>(g, ldg, m, n, room, pads);
-    Epilogue e = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE};
     const void *px = x, *pw = w;
     int64_t lx = ldx, lw = ldw;
     if (dx) on_boundaries<T>(pw, lw, n, k, room, pads);
     if (dw) on_boundaries<T>(px, lx, m, k, room, pads);
     if (int rc = pad<T>(pads, s)) return rc;
+    // one plan whichever of the two is wanted, as the workspace's size goes by it
+    const Size z[2] = {{m, k, n}, {n, k, m}};
+    const Plan plan = plan_of(z, 2, dtype);
+    Product p[2] = {};
+    const Epilogue to_dx = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE};
+    const Epilogue to_dw = {nullptr, nullptr, 0, dw, nullptr, QNN_ACT_NONE};
     if (dx)
-      if (int rc = matmul<T, true, false>(g, ldg, pw, lw, m, k, n, room, e, dtype, s)) return rc;
-    e.y = dw;
+      if (int rc = product_of(p[0], plan, 0, z[0], {g, ldg, m}, {pw, lw, k}, to_dx, room)) return rc;
     if (dw)
-      if (int rc = matmul<T, false, false>(g, ldg, px, lx, n, k, m, room, e, dtype, s)) return rc;
+      if (int rc = product_of(p[1], plan, 1, z[1], {g, ldg, n}, {px, lx, k}, to_dw, room)) return rc;
+    if (int rc = launch_grads<T>(plan.shape, p, s)) return rc;
     return (int)QNN_OK;
   });
 }
