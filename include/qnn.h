@@ -462,7 +462,7 @@ int qnn_chain_epilogue(const uint8_t* bncode, int n, int ho, int wo, int c, cons
  * dense.  Sums, statistics and states are held in fp32 whatever the type; each output is rounded
  * once.  Nothing is kept between calls: `work` is scratch of at least the size that the matching
  * *_work call gives (16-byte aligned), free for other use once the call's kernels have run.  Every
- * result is the same from run to run (no floating-point atomics). */
+ * result is the same from run to run (no floating-point atomics).  No output overlaps an input. */
 enum { QNN_F32 = 0, QNN_BF16 = 1, QNN_F16 = 2 };
 enum { QNN_ACT_NONE = 0, QNN_ACT_RELU = 1, QNN_ACT_GELU = 2 };
 
@@ -471,12 +471,16 @@ enum { QNN_ACT_NONE = 0, QNN_ACT_RELU = 1, QNN_ACT_GELU = 2 };
  * slope (nullable): act'(z) for qnn_linear_act_bwd --
  *   ReLU  [m][ceil(n / 8)] bytes, bit c & 7 of byte c / 8: z is not <= 0;
  *   GELU  [m][n], fp32 for QNN_F32, else uint16 fixed point, 8192 + 28672 act'(z) (0: NaN).
- * 1 <= n, k < 2^31 and m < 2^31; m == 0 is a no-op.  Replaces nothing of the reference (its layers are
+ * 1 <= n, k and the row strides <= 2^21, m < 2^31; m == 0 is a no-op.  Rows of x, w (and dy, dz) that are
+ * whole 16-byte groups begin on 16-byte boundaries.  Replaces nothing of the reference (its layers are
  * F.linear on fake-quantized operands, quantize.py:423-430); stands beside qnn_qconv2d_fwd. */
 int qnn_linear_act_fwd_work(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes);
 int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res,
                        int64_t ldr, void* y, void* slope, int64_t m, int64_t n, int64_t k, int dtype, int act,
                        void* work, int64_t work_bytes, qnn_stream_t stream);
+/* Introspection: the output tile that the forward product (grads == 0) or the two of the backward pass use,
+ * and the splits of their reductions (splits[0], and for the backward pass dx's and dw's in turn). */
+int qnn_linear_act_plan(int64_t m, int64_t n, int64_t k, int dtype, int grads, int* tile_m, int* tile_n, int* splits);
 /* dz = dy * act'(z); dx[m][k] = dz w; dw[n][k] = dz^T x; db[n] = sum over m of dz; each of dx, dw, db is
  * nullable.  dz [m][n] (it is the residual's gradient too): required unless act is QNN_ACT_NONE, for
  * which dz == dy and it is not written.  slope: what the forward wrote.  dz, rounded to the type, is
@@ -507,7 +511,8 @@ int qnn_layer_norm_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, 
  * A row without entries, or whose teacher logits are all -inf, is not counted: loss 0, gradient 0.
  * row_loss [rows]; stats [4 rows + 4] fp32, what the backward takes; loss (nullable): one fp32,
  * the sum of the counted rows' losses, over their number when mean != 0 (0 rows counted: 0).
- * 1 <= top <= 1024, vocab < 2^31.  Replaces the soft-target loss of the distillation trainer
+ * 1 <= top <= 1024, vocab < 2^31, temp 2^-60 to 2^60; stats on a 16-byte boundary.  A teacher logit that is
+ * NaN makes its row NaN too.  Replaces the soft-target loss of the distillation trainer
  * (qdistiler_main.py) for teachers of whom only the top logits are kept. */
 int qnn_topk_distill_fwd_work(int64_t rows, int64_t vocab, int dtype, int64_t* bytes);
 int qnn_topk_distill_fwd(const void* s, int64_t lds, const void* t, int64_t ldt, const void* index, int64_t ldi,

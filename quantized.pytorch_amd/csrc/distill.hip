@@ -207,21 +207,36 @@ __global__ __launch_bounds__(ALL ? 64 * ALL_ROWS : NT) void distill_split_rows_k
   }
 }
 
-__global__ __launch_bounds__(NT) void distill_join_kernel(const float* row_loss, float* stats, float* loss,
-                                                          int64_t rows, int mean) {
-  __shared__ double sh[NT / 64], shn[NT / 64];
+// The loss from the rows' losses, one workgroup, eight of a thread's rows under way.
+constexpr int JOIN = 1024;
+__global__ __launch_bounds__(JOIN) void distill_join_kernel(const float* __restrict__ row_loss,
+                                                            const float* __restrict__ row_stats,
+                                                            float* __restrict__ count, float* __restrict__ loss,
+                                                            int64_t rows, int mean) {
+  __shared__ double sh[JOIN / 64], shn[JOIN / 64];
   double a = 0.0, n = 0.0;
-  for (int64_t r = threadIdx.x; r < rows; r += NT) {
-    a += (double)row_loss[r];
-    n += stats[4 * r + 3] != 0.0f ? 1.0 : 0.0;
+  for (int64_t r0 = threadIdx.x; r0 < rows; r0 += 8 * JOIN) {
+    float l[8], c[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t r = r0 + u * JOIN < rows ? r0 + u * JOIN : rows - 1;
+      l[u] = row_loss[r];
+      c[u] = row_stats[4 * r + 3];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (r0 + u * JOIN < rows) {
+        a += (double)l[u];
+        n += c[u] != 0.0f ? 1.0 : 0.0;
+      }
   }
   a = wave_sum(a);
   n = wave_sum(n);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a, shn[threadIdx.x >> 6] = n;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < NT / 64; ++w) a += sh[w], n += shn[w];
-    stats[4 * rows] = (float)n;
+    for (int w = 1; w < JOIN / 64; ++w) a += sh[w], n += shn[w];
+    count[0] = (float)n;
     if (loss) loss[0] = (float)(mean ? a / (n > 0.0 ? n : 1.0) : a);
   }
 }
@@ -325,7 +340,7 @@ int check(const void* s, int64_t lds, const void* t, int64_t ldt, const void* in
   QNN_REQUIRE(vocab >= 1 && vocab < (1LL << 31), "vocab: 1 to 2^31 - 1");
   QNN_REQUIRE(top >= 1 && top <= MAX_TOP, "top: 1 to 1024");
   QNN_REQUIRE(lds >= vocab && ldt >= top && ldi >= top, "a row stride is shorter than the row");
-  QNN_REQUIRE(temp > 0.0f && temp < INFINITY, "temp: positive and finite");
+  QNN_REQUIRE(temp >= 0x1p-60f && temp <= 0x1p60f, "temp: 2^-60 to 2^60");
   QNN_REQUIRE(tdtype == QNN_F32 || tdtype == QNN_BF16 || tdtype == QNN_F16, "tdtype: QNN_F32, QNN_BF16 or QNN_F16");
   QNN_REQUIRE(index_bytes == 4 || index_bytes == 8, "index_bytes: 4 or 8");
   QNN_REQUIRE(stats && (rows == 0 || (s && t && index)), "null pointer");
@@ -388,7 +403,8 @@ int qnn_topk_distill_fwd(const void* s, int64_t lds, const void* t, int64_t ldt,
     return (int)QNN_OK;
   });
   if (rc || all) return rc;
-  hipLaunchKernelGGL(distill_join_kernel, dim3(1), dim3(NT), 0, st, row_loss, stats, loss, rows, mean);
+  hipLaunchKernelGGL(distill_join_kernel, dim3(1), dim3(JOIN), 0, st, row_loss, stats, stats + 4 * rows, loss, rows,
+                     mean);
   QNN_LAUNCH_CHECK("qnn_topk_distill_fwd");
   return QNN_OK;
 }

@@ -10,7 +10,6 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
-#include <cmath>
 #include <optional>
 
 #include "../../include/qnn.h"
@@ -384,8 +383,8 @@ Tensor topk_distill_loss(py::handle hs, py::handle ht, py::handle hi, double tem
                    "qnn: topk_distill_loss expects teacher_index of int64 or int32, got ", i.scalar_type());
   same_device(t, s, op, "teacher_logits");
   same_device(i, s, op, "teacher_index");
-  TORCH_CHECK_VALUE((float)temp > 0.0f && std::isfinite((float)temp),
-                    "qnn: topk_distill_loss needs a positive, finite temperature, got ", temp);
+  TORCH_CHECK_VALUE(temp >= 0x1p-60 && temp <= 0x1p60,
+                    "qnn: topk_distill_loss needs a positive, finite temperature (2^-60 to 2^60), got ", temp);
   TORCH_CHECK_VALUE(s.dim() >= 1 && s.size(-1) >= 1, "qnn: topk_distill_loss needs logits [..., vocab], got ", s.sizes());
   TORCH_CHECK_VALUE(t.sizes() == i.sizes() && t.dim() == s.dim() && t.sizes().slice(0, s.dim() - 1) == s.sizes().slice(0, s.dim() - 1),
                     "qnn: topk_distill_loss needs teacher_logits and teacher_index [..., top] beside logits ", s.sizes(),

@@ -409,6 +409,7 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(Joins j) {
   if (row >= t.m) return;
   float z[8], v[8], bias[8];
   load_n<float, 8>(z, t.part + row * t.ldp + col, 8);
+#pragma unroll 8
   for (int s = 1; s < t.splits; ++s) {
     load_n<float, 8>(v, t.part + (s * t.m + row) * t.ldp + col, 8);
 #pragma unroll
@@ -617,6 +618,8 @@ struct Plan {
   Split split[2];
 };
 
+constexpr int MAX_SPLITS = 64;
+
 // The tile and the splits of k of the one or two products of a launch: the least of the times above for
 // the busiest of 256 CUs; splits cost a second launch (5.5 us with its host time) and their sums' way
 // through memory (at 4 TB/s).  Over the sizes that were swept (m, n 64 to 8192, k 64 to 8192) what it
@@ -644,7 +647,7 @@ Plan plan_of(const Size* size, int count, int dtype) {
         const int want = WANT[i ? x / 4 : x % 4];
         int64_t s = want / tiles[i];
         if (s > stages[i] / 4) s = stages[i] / 4;
-        if (s > 32) s = 32;
+        if (s > MAX_SPLITS) s = MAX_SPLITS;
         skip = skip || (want > 0 && s < 2);
         if (s < 1) s = 1;
         each[i] = cdiv(stages[i], s);
@@ -878,6 +881,24 @@ int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     if (int rc = product_of(p, plan, 0, z, {px, lx, m}, {pw, lw, n}, e, room)) return rc;
     return launch_y<T>(plan.shape, p, s);
   });
+}
+
+int qnn_linear_act_plan(int64_t m, int64_t n, int64_t k, int dtype, int grads, int* tile_m, int* tile_n, int* splits) {
+  if (int rc = check(m, n, k, dtype)) return rc;
+  QNN_REQUIRE(m > 0, "m: at least 1");
+  QNN_REQUIRE(tile_m && tile_n && splits, "null pointer");
+  if (!grads && m <= FEW) {
+    *tile_m = *tile_n = FEW;
+    splits[0] = splits[1] = 1;
+    return QNN_OK;
+  }
+  const Size y = {m, n, k}, both[2] = {{m, k, n}, {n, k, m}};
+  const Plan p = plan_of(grads ? both : &y, grads ? 2 : 1, dtype);
+  *tile_m = SHAPES[p.shape].bm;
+  *tile_n = SHAPES[p.shape].bn;
+  splits[0] = p.split[0].n;
+  splits[1] = grads ? p.split[1].n : 1;
+  return QNN_OK;
 }
 
 int qnn_linear_act_bwd_work(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes) {

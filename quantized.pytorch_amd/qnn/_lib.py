@@ -115,6 +115,7 @@ SIGNATURES = {
     "qnn_linear_act_fwd_work": [c_i64, c_i64, c_i64, c_int, c_ptr],
     "qnn_linear_act_fwd": [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_int,
                            c_int, c_ptr, c_i64, c_ptr],
+    "qnn_linear_act_plan": [c_i64, c_i64, c_i64, c_int, c_int, c_ptr, c_ptr, c_ptr],
     "qnn_linear_act_bwd_work": [c_i64, c_i64, c_i64, c_int, c_ptr],
     "qnn_linear_act_bwd": [c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64,
                            c_i64, c_int, c_int, c_ptr, c_i64, c_ptr],

@@ -115,7 +115,8 @@ def topk_distill_loss(logits, teacher_logits, teacher_index, temperature=1.0, re
     teacher_index [..., top] (int64 or int32), top <= 1024.  p is the softmax of teacher_logits /
     temperature over a row's entries, q that of logits / temperature over the vocabulary.  An entry
     with a negative index is absent (padding); a class that is named twice has the sum of its
-    entries; an index past the vocabulary makes its row's loss and gradient NaN.  A row without
+    entries; an index past the vocabulary, or a teacher logit that is NaN, makes its row's loss and
+    gradient NaN.  A row without
     entries (or whose teacher logits are all -inf) is not counted: loss 0, gradient 0.
 
     The loss is float32: the mean over the counted rows (0 if there is none), their sum, or with

@@ -120,6 +120,37 @@ def test_work_entries():
         assert _call(name, -1, *args[1:], ctypes.byref(n))[0] == 1
 
 
+def test_linear_act_plan():
+    from qnn import _lib
+    tm, tn, sp = ctypes.c_int(), ctypes.c_int(), (ctypes.c_int * 2)()
+    out = (ctypes.byref(tm), ctypes.byref(tn), sp)
+    _lib.call("qnn_linear_act_plan", 8192, 8192, 4096, 1, 0, *out)
+    assert (tm.value, tn.value, *sp) == (256, 256, 1, 1)
+    _lib.call("qnn_linear_act_plan", 64, 4096, 4096, 1, 0, *out)
+    assert (tm.value, tn.value) == (64, 64) and sp[0] > 1
+    for grads in (0, 1):  # every size has a plan with scratch to match
+        for m, n, k in ((1, 1, 1), (17, 1, 1 << 21), (1 << 20, 64, 64), (300, 1 << 21, 8), (2 ** 31 - 1, 8, 8)):
+            for code in (0, 1, 2):
+                assert _call("qnn_linear_act_plan", m, n, k, code, grads, *out)[0] == 0 and 1 <= sp[0] <= 64 and 1 <= sp[1] <= 64
+    assert _call("qnn_linear_act_plan", 0, 8, 8, 0, 0, *out)[0] == 1
+    assert _call("qnn_linear_act_plan", 8, 8, (1 << 21) + 1, 0, 0, *out)[0] == 1
+    assert _call("qnn_linear_act_plan", 8, 8, 8, 0, 0, None, None, None)[0] == 1
+
+
+def test_misaligned_rows_and_missing_work_are_refused():
+    a = ctypes.c_void_p(4098)
+    rc, msg = _call("qnn_linear_act_fwd", a, 64, P, 64, None, None, 0, P, None, 20, 8, 64, 1, 0, P, 1 << 20, None)
+    assert rc == 1 and b"boundaries" in msg
+    rc, msg = _call("qnn_linear_act_fwd", P, 65, P, 64, None, None, 0, P, None, 20, 8, 64, 1, 0, P, 1 << 20, None)
+    assert rc == 1 and b"boundaries" in msg
+    rc, msg = _call("qnn_linear_act_fwd", P, 63, P, 63, None, None, 0, P, None, 20, 8, 63, 1, 0, None, 0, None)
+    assert rc == 1 and b"work" in msg
+    rc, msg = _call("qnn_layer_norm_bwd", P, 8, P, 8, P, P, P, P, P, P, 4, 8, 0, 0, None, 0, None)
+    assert rc == 1 and b"work" in msg
+    rc, msg = _call("qnn_topk_distill_fwd", P, 100000, P, 3, P, 3, 2, 100000, 3, 1.0, 1, 0, 0, 8, P, P, P, None, 0, None)
+    assert rc == 1 and b"work" in msg
+
+
 def test_empty_batches_are_no_ops():
     assert _call("qnn_linear_act_fwd", None, 8, None, 8, None, None, 0, None, None, 0, 4, 8, 0, 0, None, 0, None)[0] == 0
     assert _call("qnn_layer_norm_fwd", None, 8, None, None, None, None, None, 0, 8, 1e-5, 0, 0, None)[0] == 0

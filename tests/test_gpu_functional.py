@@ -24,7 +24,7 @@ def gen(seed):
 
 
 def near(got, want, name):
-    v, err = want
+    v, err = want[0].detach().cpu(), want[1].detach().cpu()
     got = got.detach().cpu().double().reshape(v.shape)
     assert torch.equal(torch.isnan(got), torch.isnan(v)), f"{name}: NaN elsewhere"
     inf = torch.isinf(v)
@@ -83,6 +83,56 @@ def test_linear_act(F, dt, m, n, k):
 def test_linear_act_larger(F, dt, m, n, k):
     x, w, b, r, dy = linear_case(m, n, k, dt, True, True)
     linear_check(F, x, w, b, r, dy, "gelu")
+
+
+def plan(m, n, k, dt, grads):
+    from qnn import _lib
+    tm, tn, sp = ctypes.c_int(), ctypes.c_int(), (ctypes.c_int * 2)()
+    _lib.call("qnn_linear_act_plan", m, n, k, code_of(dt), int(grads), ctypes.byref(tm), ctypes.byref(tn), sp)
+    return (tm.value, tn.value), tuple(sp)
+
+
+def code_of(dt):
+    return TYPES.index(dt) + 1 if dt != torch.float32 else 0  # QNN_BF16, QNN_F16, QNN_F32
+
+
+# sizes whose products take every tile, split and whole, with ragged edges on each side
+TILED = [(300, 200, 4000), (700, 5100, 136), (1500, 1900, 1032), (2100, 3900, 360), (4200, 4100, 520), (4090, 4000, 4072), (30000, 72, 40), (50, 40, 20000),
+         (1030, 1020, 999)]
+
+
+@pytest.mark.parametrize("m,n,k", TILED)
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_linear_act_every_tile(F, dt, m, n, k):
+    """Against the definition in float64 on the device."""
+    print(m, n, k, dt, plan(m, n, k, dt, False), plan(m, n, k, dt, True), flush=True)
+    x, w, b, r, dy = dev(*linear_case(m, n, k, dt, True, (m + n) % 200 != 0))
+    act = ("gelu", "relu", "none")[(m + k) // 10 % 3]
+    want = O.linear_act(x, w, b, r, act, dy)
+    leaves = {"dx": x, "dw": w, "db": b, "dr": r}
+    leaves = {q: v.requires_grad_(True) for q, v in leaves.items() if v is not None}
+    y = F.linear_act(x, w, b, r, act)
+    near(y, want["y"], "y")
+    for q, v in zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)):
+        near(v, want[q], q)
+
+
+def test_tiled_sizes_take_every_tile(F):
+    for dt in TYPES:
+        for grads in (False, True):
+            seen = {(plan(*z, dt, grads)[0], max(plan(*z, dt, grads)[1]) > 1) for z in TILED}
+            tiles = {t for t, _ in seen}
+            assert tiles >= ({(64, 64)} if dt == torch.float32 else {(256, 256), (128, 128), (128, 64)}), seen
+            assert dt != torch.float32 or {(128, 128), (128, 64)} & tiles, seen
+            assert {s for _, s in seen} == {False, True}, seen
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_linear_act_around_few_rows(F, dt):
+    for m in (2, 4, 8, 15, 16, 17, 18):
+        for n, k in ((50, 1000), (33, 77), (16, 2050)):
+            x, w, b, r, dy = linear_case(m, n, k, dt, True, m % 2 == 0)
+            linear_check(F, x, w, b, r, dy, "gelu" if m % 3 else "relu", f"{m} {n} {k} ")
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=IDS)
@@ -216,6 +266,22 @@ def test_layer_norm(F, dt, rows, dim):
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_layer_norm_at_every_width(F, dt):
+    """Both sides of each width at which the kernels change, and rows that are no whole number of groups."""
+    g = gen(12)
+    group = 4 if dt == torch.float32 else 8
+    for groups in (1, 16, 64, 128, 256, 512, 1024, 2048, 4096):
+        for dim in (groups * group - 1, groups * group, groups * group + 1):
+            if dim < 1:
+                continue
+            x, dy = torch.randn(3, dim, generator=g).to(dt), torch.randn(3, dim, generator=g).to(dt)
+            norm_check(F, x, torch.randn(dim, generator=g).to(dt), torch.randn(dim, generator=g).to(dt), dy)
+    for rows, dim in ((3000, 40), (2600, 136), (1700, 264), (1300, 2056)):  # more rows than one turn of the launch
+        x, dy = torch.randn(rows, dim, generator=g).to(dt), torch.randn(rows, dim, generator=g).to(dt)
+        norm_check(F, x, torch.randn(dim, generator=g), None, dy)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
 def test_layer_norm_hard_rows(F, dt):
     """Rows of one value (variance 0), far from 0, very small and very large, infinite and NaN."""
     g = gen(9)
@@ -307,6 +373,14 @@ def test_topk_distill(F, dt, rows, vocab, top):
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("rows,vocab,top", [(2, 4095, 3), (2, 4096, 3), (2, 4097, 3), (3, 8191, 3), (3, 8192, 3), (3, 8193, 3), (16, 30000, 9),
+                                            (17, 30000, 9), (1, 200001, 1024), (520, 9000, 4), (20000, 11, 2)])
+def test_topk_distill_where_the_kernels_change(F, dt, rows, vocab, top):
+    s, t, i = distill_case(rows, vocab, top, dt, torch.float32)
+    distill_check(F, s, t, i, 2.0, "mean")
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
 @pytest.mark.parametrize("vocab", [50, 4099, 66000])
 def test_topk_distill_hard_rows(F, dt, vocab):
     g = gen(vocab)
@@ -335,12 +409,13 @@ def test_topk_distill_hard_rows(F, dt, vocab):
     s[2], t[2] = -math.inf, 1.0
     i[3, 0], i[4, 1] = vocab, 1 << 40
     s[5, 2] = math.inf
+    t[8, 1] = math.nan
     sd = s.cuda().requires_grad_(True)
     loss = F.topk_distill_loss(sd, t.cuda(), i.cuda(), 1.0, "none")
     ds, = torch.autograd.grad(loss, sd, torch.ones_like(loss))
-    assert loss.cpu().isnan().tolist() == [True, False, True, True, True, True] + [False] * 6
-    assert ds.cpu().isnan().any(1).tolist() == [True, False, True, True, True, True] + [False] * 6
-    assert ds[[2, 3, 4]].isnan().all() and not ds[1].any()
+    nans = [True, False, True, True, True, True, False, False, True, False, False, False]
+    assert loss.cpu().isnan().tolist() == nans and ds.cpu().isnan().any(1).tolist() == nans
+    assert ds[[2, 3, 4, 8]].isnan().all() and not ds[1].any()
 
 
 def test_topk_distill_nothing_counted(F):
@@ -373,7 +448,7 @@ def test_topk_distill_strides(F, dt):
 def test_topk_distill_refusals(F):
     s, t, i = torch.zeros(2, 9, device="cuda"), torch.zeros(2, 3, device="cuda"), torch.zeros(2, 3, dtype=torch.long, device="cuda")
     for bad in (lambda: F.topk_distill_loss(s, t, i[:, :2]), lambda: F.topk_distill_loss(s, t[:1], i[:1]), lambda: F.topk_distill_loss(s, t, i, 0.0),
-                lambda: F.topk_distill_loss(s, t, i, math.inf), lambda: F.topk_distill_loss(s, t, i, reduction="batchmean"),
+                lambda: F.topk_distill_loss(s, t, i, math.inf), lambda: F.topk_distill_loss(s, t, i, 1e-30), lambda: F.topk_distill_loss(s, t, i, math.nan), lambda: F.topk_distill_loss(s, t, i, reduction="batchmean"),
                 lambda: F.topk_distill_loss(s, t[:, :0], i[:, :0]), lambda: F.topk_distill_loss(s, t.repeat(1, 400), i.repeat(1, 400)),
                 lambda: F.topk_distill_loss(s[:, :0], t, i)):
         with pytest.raises(ValueError):
@@ -573,7 +648,7 @@ def test_two_captured_training_steps(F):
 def test_nothing_is_written_past_the_outputs(F, dt, m, n, k):
     """The C entries on buffers with a guard behind each output and behind the workspace."""
     from qnn import _lib
-    code = TYPES.index(dt) + 1 if dt != torch.float32 else 0  # QNN_BF16, QNN_F16, QNN_F32
+    code = code_of(dt)
 
     def guarded(count, dtype):
         size = count * torch.empty((), dtype=dtype).element_size()
