@@ -6,11 +6,11 @@ on first use by `qnn._lib.load()`.
 """
 from . import synthetic  # noqa: F401
 
-__all__ = ["quantize", "resnet_quantized", "mobilenet_quantized", "synthetic", "engine", "functional"]
+__all__ = ["quantize", "resnet_quantized", "mobilenet_quantized", "synthetic", "engine", "functional", "distill"]
 
 
 def __getattr__(name):
-    if name in ("quantize", "resnet_quantized", "mobilenet_quantized", "engine", "dist", "functional", "_lib"):
+    if name in ("quantize", "resnet_quantized", "mobilenet_quantized", "engine", "dist", "functional", "distill", "_lib"):
         import importlib
         return importlib.import_module(f".{name}", __name__)
     raise AttributeError(name)
