@@ -249,6 +249,58 @@ struct Cfg {
   static constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN, SLOT = (BM + BN) * 64, LDS = 4 * SLOT;
 };
 
+// A wave's sums to where they go.
+template <class T, class C>
+__device__ __forceinline__ void emit(const Product& t, const f4 (&acc)[C::TM][C::TN], char* lds, int split, int64_t i0,
+                                     int64_t j0, int ri, int rj, int wave, int lane) {
+  constexpr int TM = C::TM, TN = C::TN;
+  const Epilogue& e = t.e;
+  // acc[i][j]: row 16 i + lane % 16, columns 16 j + lane / 16 * 4 ... + 3.  A wave turns as many rows at a
+  // time around in its share of LDS as fit, so that a lane has 8 neighbouring columns, the same ones in
+  // every row, and a row's are together.  Chunks of 16 bytes are XORed by the row.
+  constexpr int COLS = 16 * TN, PER = COLS / 8, FIT = C::LDS / C::W / (COLS * 4) / 16;
+  constexpr int TURN = FIT < TM ? FIT : TM;  // 16-row tiles at a time
+  static_assert(TURN > 0 && TM % TURN == 0, "whole turns");
+  char* mine = lds + wave * (C::LDS / C::W);
+  const int col = lane % PER * 8;
+  const int64_t gj = j0 + rj + col;
+  float bias[8];
+  bias8<T>(bias, e, gj, t.n);
+  auto rows_out = [&](int64_t gi0, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+#pragma unroll 2
+    for (int u = 0; u < TURN * 16 * PER / 64; ++u) {
+      const int row = u * (64 / PER) + lane / PER;
+      float z[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<f4*>(z + 4 * h) =
+            *reinterpret_cast<const f4*>(mine + row * COLS * 4 + ((col / 4 + h) ^ (row & (COLS / 4 - 1))) * 16);
+      const int64_t gi = gi0 + row;
+      if (!WHOLE && (gi >= t.m || gj >= t.n)) continue;
+      if (t.splits > 1)
+        store_n<float, 8>(t.part + (split * t.m + gi) * t.ldp + gj, z, 8);  // (ldp: whole groups of 8)
+      else
+        finish8<T, WHOLE>(z, bias, e, gi, gj, t.n);
+    }
+  };
+  const bool inside = i0 + C::BM <= t.m && j0 + C::BN <= t.n;
+#pragma unroll
+  for (int i = 0; i < TM; i += TURN) {
+#pragma unroll
+    for (int k = 0; k < TURN; ++k)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int row = 16 * k + (lane & 15);
+        *reinterpret_cast<f4*>(mine + row * COLS * 4 + ((4 * j + (lane >> 4)) ^ (row & (COLS / 4 - 1))) * 16) = acc[i + k][j];
+      }
+    __builtin_amdgcn_wave_barrier();
+    if (inside) rows_out(i0 + ri + 16 * i, std::true_type{});
+    else rows_out(i0 + ri + 16 * i, std::false_type{});
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 // Workgroup `id` of the product's.
 template <class T, bool AD, bool BD, class C>
 __device__ __forceinline__ void tile(const Product& t, int id) {
@@ -256,7 +308,6 @@ __device__ __forceinline__ void tile(const Product& t, int id) {
   using B = Side<T, BD, C::BN, C::W>;
   constexpr int TM = C::TM, TN = C::TN, KE = A::KE, P = A::LOADS + B::LOADS;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const Epilogue& e = t.e;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int split, ti, tj;
   tile_of(t, id, split, ti, tj);
@@ -331,55 +382,115 @@ __device__ __forceinline__ void tile(const Product& t, int id) {
   if (s < stages) step(s, std::integral_constant<int, 0>{});
   meet<0>();
 
-  // acc[i][j]: row 16 i + lane % 16, columns 16 j + lane / 16 * 4 ... + 3.  A wave turns as many rows at a
-  // time around in its share of LDS as fit, so that a lane has 8 neighbouring columns, the same ones in
-  // every row, and a row's are together.  Chunks of 16 bytes are XORed by the row.
-  constexpr int COLS = 16 * TN, PER = COLS / 8, FIT = C::LDS / C::W / (COLS * 4) / 16;
-  constexpr int TURN = FIT < TM ? FIT : TM;  // 16-row tiles at a time
-  static_assert(TURN > 0 && TM % TURN == 0, "whole turns");
-  char* mine = lds + wave * (C::LDS / C::W);
-  const int col = lane % PER * 8;
-  const int64_t gj = j0 + rj + col;
-  float bias[8];
-  bias8<T>(bias, e, gj, t.n);
-  auto rows_out = [&](int64_t gi0, auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
-#pragma unroll 2
-    for (int u = 0; u < TURN * 16 * PER / 64; ++u) {
-      const int row = u * (64 / PER) + lane / PER;
-      float z[8];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<f4*>(z + 4 * h) =
-            *reinterpret_cast<const f4*>(mine + row * COLS * 4 + ((col / 4 + h) ^ (row & (COLS / 4 - 1))) * 16);
-      const int64_t gi = gi0 + row;
-      if (!WHOLE && (gi >= t.m || gj >= t.n)) continue;
-      if (t.splits > 1)
-        store_n<float, 8>(t.part + (split * t.m + gi) * t.ldp + gj, z, 8);  // (ldp: whole groups of 8)
-      else
-        finish8<T, WHOLE>(z, bias, e, gi, gj, t.n);
-    }
-  };
-  const bool inside = i0 + C::BM <= t.m && j0 + C::BN <= t.n;
-#pragma unroll
-  for (int i = 0; i < TM; i += TURN) {
-#pragma unroll
-    for (int k = 0; k < TURN; ++k)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int row = 16 * k + (lane & 15);
-        *reinterpret_cast<f4*>(mine + row * COLS * 4 + ((4 * j + (lane >> 4)) ^ (row & (COLS / 4 - 1))) * 16) = acc[i + k][j];
-      }
-    __builtin_amdgcn_wave_barrier();
-    if (inside) rows_out(i0 + ri + 16 * i, std::true_type{});
-    else rows_out(i0 + ri + 16 * i, std::false_type{});
-    __builtin_amdgcn_wave_barrier();
+  emit<T, C>(t, acc, lds, split, i0, j0, ri, rj, wave, lane);
+}
+
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for<N, I + 1>(f);
   }
+}
+
+// The same for operands DENSE in k whose rows begin anywhere, which direct loads do not take: 16 bytes a
+// lane into registers, four stages ahead, and from there to LDS.  Rows past the matrix are its last one
+// again (their sums are not written); the stage that is no whole one comes first, so that all others'
+// loads need no guard.  Against padded copies it saves their launch and twice the operands' bytes:
+// 203 x 5003 x 1535 fp16 24.0 -> 22.8 us, 64 x 1000 x 4001 bf16 17.1 -> 12.3, 2000 x 301 x 5003 fp32
+// 80 -> 63 (eight stages ahead are no faster than four).
+template <class T, class C>
+__device__ __forceinline__ void loose_tile(const Product& t, int id) {
+  using A = Side<T, true, C::BM, C::W>;
+  using B = Side<T, true, C::BN, C::W>;
+  constexpr int TM = C::TM, TN = C::TN, KE = A::KE, GR = GROUP<T>, P = A::LOADS + B::LOADS, D = 4;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int split, ti, tj;
+  tile_of(t, id, split, ti, tj);
+  const int64_t i0 = (int64_t)ti * C::BM, j0 = (int64_t)tj * C::BN, k0 = split * t.span;
+  const int all = (int)(t.k - k0 < t.span ? t.k - k0 : t.span), stages = (all + KE - 1) / KE;
+  const int head = all - (stages - 1) * KE;  // elements of stage 0
+  const int ri = wave / C::WN * 16 * TM, rj = wave % C::WN * 16 * TN;
+
+  const T* from[P];  // this lane's group of load j in stage 1; its byte in a slot
+  int to[P], group[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const bool is_a = j < A::LOADS;
+    const int at = (wave * (is_a ? A::LOADS : B::LOADS) + (is_a ? j : j - A::LOADS)) * 1024 + lane * 16;
+    const int row = at / 64, chunk = at / 16 % 4 ^ A::turn(row);
+    const Operand& o = is_a ? t.a : t.b;
+    const int64_t r = (is_a ? i0 : j0) + row;
+    from[j] = (const T*)o.p + (r < o.rows ? r : o.rows - 1) * o.ld + k0 + head + chunk * GR;
+    to[j] = (is_a ? 0 : A::BYTES) + at;
+    group[j] = chunk * GR;
+  }
+  Vec<T, GR> held[D][P];  // stage s in held[s % D]
+  auto load = [&](int s, auto slot) {  // stage s >= 1 (past the last: that one again, which is not used)
+    const int64_t c = (int64_t)((s < stages ? s : stages - 1) - 1) * KE;
+#pragma unroll
+    for (int j = 0; j < P; ++j) held[decltype(slot)::value][j] = load_group(from[j] + c, GR);
+  };
+  auto put = [&](int s, auto slot) {
+#pragma unroll
+    for (int j = 0; j < P; ++j) *reinterpret_cast<Vec<T, GR>*>(lds + (s & 3) * C::SLOT + to[j]) = held[decltype(slot)::value][j];
+  };
+  const int pa = A::place(ri, lane), pb = B::place(rj, lane);
+  f4 fa[2][TM], fb[2][TN], acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+  auto fetch = [&](int slot, int set) {
+    char* s = lds + slot * C::SLOT;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[set][j] = B::fragment(s + A::BYTES, pb, rj, j, lane);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fa[set][i] = A::fragment(s, pa, ri, i, lane);
+  };
+  if (stages > 1) static_for<D - 1>([&](auto j) { load(1 + j, std::integral_constant<int, 1 + j>{}); });
+#pragma unroll
+  for (int j = 0; j < P; ++j) held[0][j] = load_group(from[j] - head, head - group[j]);
+  put(0, std::integral_constant<int, 0>{});
+  if (stages > 1) {
+    load(D, std::integral_constant<int, 0>{});
+    put(1, std::integral_constant<int, 1>{});
+    load(D + 1, std::integral_constant<int, 1>{});
+  }
+  meet<63>();
+  fetch(0, 0);
+  // step s: stage s is in registers for the MFMAs, s + 1 in LDS, s + 2 to s + D + 1 on their way to `held`
+  auto step = [&](int s, auto slot, auto set) {
+    constexpr int S = decltype(set)::value;
+    meet<63>();  // every wave has read stage s from LDS and written stage s + 1
+    if (stages > 1) {
+      put(s + 2, slot);
+      load(s + 2 + D, slot);
+    }
+    fetch((s + 1) & 3, S ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = mma<T>(fb[S][j], fa[S][i], acc[i][j]);
+  };
+  for (int s = 0; s < stages; s += D)
+    static_for<D>([&](auto j) {
+      if (s + j < stages) step(s + j, std::integral_constant<int, (j + 2) % D>{}, std::integral_constant<int, j % 2>{});
+    });
+  meet<0>();
+  emit<T, C>(t, acc, lds, split, i0, j0, ri, rj, wave, lane);
 }
 
 template <class T, class C>
 __global__ __launch_bounds__(C::NT, C::EU) void linear_y_kernel(Product y) {
   tile<T, true, true, C>(y, blockIdx.x);
+}
+
+template <class T, class C>
+__global__ __launch_bounds__(C::NT, C::EU) void linear_y_loose_kernel(Product y) {
+  loose_tile<T, C>(y, blockIdx.x);
 }
 
 // dx = dz w and dw = dz^T x in one launch, so that the one's last tiles and the other's first share the
@@ -616,6 +727,8 @@ struct Size {
 struct Plan {
   int shape;  // of SHAPES, for all products of the launch
   Split split[2];
+  float us;      // what it is taken to cost
+  bool loose;    // forward: rows as they are (Small) and not padded
 };
 
 constexpr int MAX_SPLITS = 64;
@@ -624,11 +737,11 @@ constexpr int MAX_SPLITS = 64;
 // the busiest of 256 CUs; splits cost a second launch (5.5 us with its host time) and their sums' way
 // through memory (at 4 TB/s).  Over the sizes that were swept (m, n 64 to 8192, k 64 to 8192) what it
 // picks for one product is within 10 % of the best pair, 20 % where the whole takes under 20 us.
-Plan plan_of(const Size* size, int count, int dtype) {
+Plan plan_of(const Size* size, int count, int dtype, int from = 0) {
   const int64_t ke = 64 / type_bytes(dtype);
   Plan best = {};
   float least = INFINITY;
-  for (int c = dtype == QNN_F32 ? 1 : 0; c < 4; ++c) {
+  for (int c = dtype == QNN_F32 && from == 0 ? 1 : from; c < 4; ++c) {
     const Shape& h = SHAPES[c];
     const float stage = dtype == QNN_F32 ? h.stage32 : h.stage16, alone = dtype == QNN_F32 ? 1.0f : h.alone;
     int64_t tiles[2], stages[2];
@@ -666,6 +779,7 @@ Plan plan_of(const Size* size, int count, int dtype) {
       us += most * stage + (0.6f * turns + 0.4f) * h.ends + (split ? 5.5f : 0.0f);
       if (us < least) {
         least = us;
+        best.us = us;
         best.shape = c;
         for (int i = 0; i < count; ++i) {
           const int64_t ldp = up(size[i].n, 8);
@@ -678,6 +792,20 @@ Plan plan_of(const Size* size, int count, int dtype) {
 }
 
 constexpr int FEW = 16;  // rows of x that few_rows_kernel takes
+
+// The forward product's plan: rows that are no whole number of groups are padded (a launch and their bytes
+// there and back, 4 us and 4 TB/s) or taken as they are, whichever is the less.  Loads of 16 bytes that
+// begin at any 2 bound loose_tile: 1.3 of the Small tile's time or more (as long in fp32, whose loads begin
+// at a word).
+Plan plan_y(const Size& z, int dtype) {
+  Plan p = plan_of(&z, 1, dtype);
+  if (z.k * type_bytes(dtype) % 16 == 0) return p;
+  const float padded = p.us + 4.0f + (float)((z.m + z.n) * z.k) * (float)type_bytes(dtype) * 0.5e-6f;
+  Plan q = plan_of(&z, 1, dtype, 3);
+  if (q.us * (dtype == QNN_F32 ? 1.0f : 1.3f) > padded) return p;
+  q.loose = true;
+  return q;
+}
 
 // The plan's product i of c = a b^T; its sums' scratch is taken from room.
 int product_of(Product& p, const Plan& plan, int i, const Size& z, const Operand& a, const Operand& b,
@@ -785,8 +913,8 @@ int64_t padded_bytes(int64_t rows, int64_t cols, int dtype) {
 
 int64_t fwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
   if (m <= FEW) return 0;
-  const Size y = {m, n, k};
-  return padded_bytes(m, k, dtype) + padded_bytes(n, k, dtype) + plan_of(&y, 1, dtype).split[0].bytes;
+  const Plan p = plan_y({m, n, k}, dtype);
+  return (p.loose ? 0 : padded_bytes(m, k, dtype) + padded_bytes(n, k, dtype)) + p.split[0].bytes;
 }
 
 // Strips of rows for dz's sums: one of 16 rows at a time for a few rows, which saves the launch that adds
@@ -871,14 +999,21 @@ int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     char* room = (char*)work;
     const void *px = x, *pw = w;
     int64_t lx = ldx, lw = ldw;
-    Padding pads = {};
-    on_boundaries<T>(px, lx, m, k, room, pads);
-    on_boundaries<T>(pw, lw, n, k, room, pads);
-    if (int rc = pad<T>(pads, s)) return rc;
     const Size z = {m, n, k};
-    const Plan plan = plan_of(&z, 1, dtype);
+    const Plan plan = plan_y(z, dtype);
+    if (!plan.loose) {
+      Padding pads = {};
+      on_boundaries<T>(px, lx, m, k, room, pads);
+      on_boundaries<T>(pw, lw, n, k, room, pads);
+      if (int rc = pad<T>(pads, s)) return rc;
+    }
     Product p;
     if (int rc = product_of(p, plan, 0, z, {px, lx, m}, {pw, lw, n}, e, room)) return rc;
+    if (plan.loose) {
+      hipLaunchKernelGGL((linear_y_loose_kernel<T, Small>), dim3((unsigned)p.blocks), dim3(Small::NT), Small::LDS, s, p);
+      QNN_LAUNCH_CHECK("linear_y_loose_kernel");
+      return join<T>(&p, 1, s);
+    }
     return launch_y<T>(plan.shape, p, s);
   });
 }
@@ -893,7 +1028,7 @@ int qnn_linear_act_plan(int64_t m, int64_t n, int64_t k, int dtype, int grads, i
     return QNN_OK;
   }
   const Size y = {m, n, k}, both[2] = {{m, k, n}, {n, k, m}};
-  const Plan p = plan_of(grads ? both : &y, grads ? 2 : 1, dtype);
+  const Plan p = grads ? plan_of(both, 2, dtype) : plan_y(y, dtype);
   *tile_m = SHAPES[p.shape].bm;
   *tile_n = SHAPES[p.shape].bn;
   splits[0] = p.split[0].n;

@@ -98,7 +98,7 @@ def code_of(dt):
 
 # sizes whose products take every tile, split and whole, with ragged edges on each side
 TILED = [(300, 200, 4000), (700, 5100, 136), (1500, 1900, 1032), (2100, 3900, 360), (4200, 4100, 520), (4090, 4000, 4072), (30000, 72, 40), (50, 40, 20000),
-         (1030, 1020, 999)]
+         (1030, 1020, 999), (510, 4080, 1024)]
 
 
 @pytest.mark.parametrize("m,n,k", TILED)
@@ -125,6 +125,15 @@ def test_tiled_sizes_take_every_tile(F):
             assert tiles >= ({(64, 64)} if dt == torch.float32 else {(256, 256), (128, 128), (128, 64)}), seen
             assert dt != torch.float32 or {(128, 128), (128, 64)} & tiles, seen
             assert {s for _, s in seen} == {False, True}, seen
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(20, 70, 1), (20, 70, 5), (33, 65, 31), (64, 64, 33), (65, 130, 47), (100, 1001, 95), (203, 500, 129),
+                                   (64, 100, 4001), (130, 2001, 515), (1000, 1001, 259), (40, 33, 20001)])
+def test_linear_act_rows_that_begin_anywhere(F, dt, m, n, k):
+    """Odd lengths around whole stages, short and split reductions, edges on both sides."""
+    x, w, b, r, dy = linear_case(m, n, k, dt, True, k % 4 == 1)
+    linear_check(F, x, w, b, r, dy, "gelu" if m % 2 else "none")
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=IDS)
