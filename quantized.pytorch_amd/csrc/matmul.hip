@@ -385,6 +385,10 @@ __device__ __forceinline__ void tile(const Product& t, int id) {
   emit<T, C>(t, acc, lds, split, i0, j0, ri, rj, wave, lane);
 }
 
+struct __attribute__((packed, aligned(4))) Words {
+  uint32_t v[4];
+};
+
 template <int N, int I = 0, class F>
 __device__ __forceinline__ void static_for(F&& f) {
   if constexpr (I < N) {
@@ -397,8 +401,8 @@ __device__ __forceinline__ void static_for(F&& f) {
 // lane into registers, four stages ahead, and from there to LDS.  Rows past the matrix are its last one
 // again (their sums are not written); the stage that is no whole one comes first, so that all others'
 // loads need no guard.  Against padded copies it saves their launch and twice the operands' bytes:
-// 203 x 5003 x 1535 fp16 24.0 -> 22.8 us, 64 x 1000 x 4001 bf16 17.1 -> 12.3, 2000 x 301 x 5003 fp32
-// 80 -> 63 (eight stages ahead are no faster than four).
+// 203 x 5003 x 1535 fp16 24.0 -> 18.6 us (with 1536 and direct loads: 11.6), 64 x 1000 x 4001 bf16
+// 17.1 -> 12.2, 2000 x 301 x 5003 fp32 80 -> 63 (six or eight stages ahead are no faster than four).
 template <class T, class C>
 __device__ __forceinline__ void loose_tile(const Product& t, int id) {
   using A = Side<T, true, C::BM, C::W>;
@@ -426,15 +430,45 @@ __device__ __forceinline__ void loose_tile(const Product& t, int id) {
     to[j] = (is_a ? 0 : A::BYTES) + at;
     group[j] = chunk * GR;
   }
-  Vec<T, GR> held[D][P];  // stage s in held[s % D]
+  // Loads of 16 bytes that do not begin at a word take twice as long.  So a group of 16-bit elements that
+  // begins inside a word is loaded from the element before it on (there is one from stage 1 on), and its last
+  // element comes from the lane with the row's next group, which has it first in its own -- for the last
+  // group of a stage that is the first one's lane, with the next stage; after the last stage `tail`.
+  constexpr bool SHIFT = sizeof(T) == 2;
+  const bool shift = SHIFT && (((uintptr_t)t.a.p | (uintptr_t)t.b.p | t.a.ld << 1 | t.b.ld << 1) & 2);  // some row does
+  int odd[P], next[P];  // bytes of a word before the group; the lane with the next one
+  uint32_t tail[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    odd[j] = SHIFT ? (int)((uintptr_t)from[j] & 2) : 0;
+    const int chunk = group[j] / GR, flip = chunk ^ (lane & 3);
+    next[j] = ((lane & ~3) | ((chunk + 1 & 3) ^ flip)) * 4;
+    if constexpr (SHIFT) tail[j] = reinterpret_cast<const uint16_t*>(from[j])[all - 1 - head - group[j]];
+  }
+  Words held[D][P];  // stage s in held[s % D]
   auto load = [&](int s, auto slot) {  // stage s >= 1 (past the last: that one again, which is not used)
     const int64_t c = (int64_t)((s < stages ? s : stages - 1) - 1) * KE;
 #pragma unroll
-    for (int j = 0; j < P; ++j) held[decltype(slot)::value][j] = load_group(from[j] + c, GR);
+    for (int j = 0; j < P; ++j)
+      held[decltype(slot)::value][j] = *reinterpret_cast<const Words*>((const char*)(from[j] + c) - odd[j]);
   };
   auto put = [&](int s, auto slot) {
+    constexpr int S = decltype(slot)::value;
 #pragma unroll
-    for (int j = 0; j < P; ++j) *reinterpret_cast<Vec<T, GR>*>(lds + (s & 3) * C::SLOT + to[j]) = held[decltype(slot)::value][j];
+    for (int j = 0; j < P; ++j) {
+      const uint32_t* v = held[S][j].v;
+      uint4 w = {v[0], v[1], v[2], v[3]};
+      if (shift) {
+        const uint32_t mine = group[j] == 0 ? held[(S + 1) % D][j].v[0] : v[0];
+        uint32_t last = (uint32_t)__builtin_amdgcn_ds_bpermute(next[j], (int)mine);
+        last = s == stages - 1 && group[j] == 3 * GR ? tail[j] : last;
+        w.x = __builtin_amdgcn_alignbyte(v[1], v[0], odd[j]);
+        w.y = __builtin_amdgcn_alignbyte(v[2], v[1], odd[j]);
+        w.z = __builtin_amdgcn_alignbyte(v[3], v[2], odd[j]);
+        w.w = __builtin_amdgcn_alignbyte(last, v[3], odd[j]);
+      }
+      *reinterpret_cast<uint4*>(lds + (s & 3) * C::SLOT + to[j]) = w;
+    }
   };
   const int pa = A::place(ri, lane), pb = B::place(rj, lane);
   f4 fa[2][TM], fb[2][TN], acc[TM][TN];
@@ -451,8 +485,8 @@ __device__ __forceinline__ void loose_tile(const Product& t, int id) {
   };
   if (stages > 1) static_for<D - 1>([&](auto j) { load(1 + j, std::integral_constant<int, 1 + j>{}); });
 #pragma unroll
-  for (int j = 0; j < P; ++j) held[0][j] = load_group(from[j] - head, head - group[j]);
-  put(0, std::integral_constant<int, 0>{});
+  for (int j = 0; j < P; ++j)
+    *reinterpret_cast<Vec<T, GR>*>(lds + to[j]) = load_group(from[j] - head, head - group[j]);
   if (stages > 1) {
     load(D, std::integral_constant<int, 0>{});
     put(1, std::integral_constant<int, 1>{});
@@ -794,9 +828,8 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0) {
 constexpr int FEW = 16;  // rows of x that few_rows_kernel takes
 
 // The forward product's plan: rows that are no whole number of groups are padded (a launch and their bytes
-// there and back, 4 us and 4 TB/s) or taken as they are, whichever is the less.  Loads of 16 bytes that
-// begin at any 2 bound loose_tile: 1.3 of the Small tile's time or more (as long in fp32, whose loads begin
-// at a word).
+// there and back, 4 us and 4 TB/s) or taken as they are, whichever is the less.  What
+// loose_tile does besides takes it to 1.3 of the Small tile's estimate in 16-bit types, none in fp32.
 Plan plan_y(const Size& z, int dtype) {
   Plan p = plan_of(&z, 1, dtype);
   if (z.k * type_bytes(dtype) % 16 == 0) return p;
