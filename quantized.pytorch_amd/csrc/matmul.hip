@@ -435,7 +435,7 @@ __device__ __forceinline__ void loose_tile(const Product& t, int id) {
   // element comes from the lane with the row's next group, which has it first in its own -- for the last
   // group of a stage that is the first one's lane, with the next stage; after the last stage `tail`.
   constexpr bool SHIFT = sizeof(T) == 2;
-  const bool shift = SHIFT && (((uintptr_t)t.a.p | (uintptr_t)t.b.p | t.a.ld << 1 | t.b.ld << 1) & 2);  // some row does
+  const bool shift = SHIFT && (((uintptr_t)t.a.p | (uintptr_t)t.b.p | (t.a.ld | t.b.ld | head) << 1) & 2);  // some do
   int odd[P], next[P];  // bytes of a word before the group; the lane with the next one
   uint32_t tail[P];
 #pragma unroll
