@@ -567,8 +567,9 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(Joins j) {
 // ------------------------------------------------------------------------- few rows: the weight is all
 // y for up to 16 rows of x, both operands dense in k.  A workgroup has 16 outputs; its waves share
 // k between them in turns of 128 bytes a row, loads going straight into the fragments, and join
-// their sums in LDS in a fixed order.  Bound by the weight's way from HBM: the launch's waves have
-// most of it in flight at once.
+// their sums in LDS in a fixed order.  Bound by the weight's way from HBM: one row of 16384 x 16384
+// bf16 in 109 us (4.9 TB/s), of 4096 x 4096 in 7.2; the launch's waves have most of it in flight at once.  Rows past either matrix are its last one again: their sums are not
+// written, and no load needs a guard but those of the last turn, where k ends inside it.
 template <class T, int W>
 __global__ __launch_bounds__(64 * W) void few_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int m,
                                                           int64_t n, int64_t k, Epilogue e) {
@@ -576,32 +577,38 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(const T* x, int64_t ld
   __shared__ f4 sums[W][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15;
   const int64_t j0 = (int64_t)blockIdx.x * 16;
-  const bool wi = j0 + row < n, xi = row < m;
-  const T* wp = w + (wi ? j0 + row : 0) * ldw;
-  const T* xp = x + (xi ? row : 0) * ldx;
+  const T* wp = w + (j0 + row < n ? j0 + row : n - 1) * ldw + (lane >> 4) * GR;
+  const T* xp = x + (row < m ? row : m - 1) * ldx + (lane >> 4) * GR;
   f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  auto frag = [&](const T* p, bool there, int64_t c) {
-    const Vec<T, GR> v = load_group(p + c, there ? k - c : 0);
+  auto frag = [](const Vec<T, GR>& v) {
     f4 f;
     __builtin_memcpy(&f, &v, 16);
     return f;
   };
-  for (int64_t c0 = (int64_t)wave * TURN; c0 < k; c0 += (int64_t)W * TURN * U) {
+  const int64_t whole = k / TURN;
+  for (int64_t t = wave; t < whole; t += W * U) {
     f4 fw[U][2], fx[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t c = c0 + (int64_t)u * W * TURN + (lane >> 4) * 2 * GR;
+      const int64_t c = (t + u * W < whole ? t + u * W : t) * TURN;  // (past the last: the first again, not used)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        fw[u][h] = frag(wp, wi, c + h * GR);
-        fx[u][h] = frag(xp, xi, c + h * GR);
+        fw[u][h] = frag(load_group(wp + c + h * 4 * GR, GR));
+        fx[u][h] = frag(load_group(xp + c + h * 4 * GR, GR));
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
+      if (t + u * W < whole)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) acc = mma<T>(fw[u][h], fx[u][h], acc);
+        for (int h = 0; h < 2; ++h) acc = mma<T>(fw[u][h], fx[u][h], acc);
   }
+  if (whole * TURN < k && wave == whole % W)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t c = whole * TURN + h * 4 * GR, left = k - c - (lane >> 4) * GR;
+      acc = mma<T>(frag(load_group(wp + c, left)), frag(load_group(xp + c, left)), acc);
+    }
   sums[wave][lane] = acc;
   __syncthreads();
   // thread: row t / 2, 8 columns from 8 (t % 2); lane (c / 4) 16 + row of a wave has columns c ... c + 3
@@ -825,7 +832,10 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0) {
   return best;
 }
 
-constexpr int FEW = 16;  // rows of x that few_rows_kernel takes
+// Whether few_rows_kernel takes the forward product: up to 16 rows of x, but 2 where the rows' groups begin
+// inside words (16 x 4096 x 4097 bf16 takes it 27 us and loose_tile 18, 4 rows 21, one row 16 us).
+constexpr int FEW = 16;
+bool is_few(int64_t m, int64_t k, int dtype) { return m <= (dtype != QNN_F32 && k % 2 ? 2 : FEW); }
 
 // The forward product's plan: rows that are no whole number of groups are padded (a launch and their bytes
 // there and back, 4 us and 4 TB/s) or taken as they are, whichever is the less.  What
@@ -945,7 +955,7 @@ int64_t padded_bytes(int64_t rows, int64_t cols, int dtype) {
 }
 
 int64_t fwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
-  if (m <= FEW) return 0;
+  if (is_few(m, k, dtype)) return 0;
   const Plan p = plan_y({m, n, k}, dtype);
   return (p.loose ? 0 : padded_bytes(m, k, dtype) + padded_bytes(n, k, dtype)) + p.split[0].bytes;
 }
@@ -1023,7 +1033,7 @@ int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     using T = decltype(t);
     hipStream_t s = (hipStream_t)stream;
     const Epilogue e = {bias, res, ldr, y, slope, act};
-    if (m <= FEW) {
+    if (is_few(m, k, dtype)) {
       hipLaunchKernelGGL((few_rows_kernel<T, 16>), dim3((unsigned)cdiv(n, 16)), dim3(1024), 0, s, (const T*)x, ldx,
                          (const T*)w, ldw, (int)m, n, k, e);
       QNN_LAUNCH_CHECK("few_rows_kernel");
@@ -1055,7 +1065,7 @@ int qnn_linear_act_plan(int64_t m, int64_t n, int64_t k, int dtype, int grads, i
   if (int rc = check(m, n, k, dtype)) return rc;
   QNN_REQUIRE(m > 0, "m: at least 1");
   QNN_REQUIRE(tile_m && tile_n && splits, "null pointer");
-  if (!grads && m <= FEW) {
+  if (!grads && is_few(m, k, dtype)) {
     *tile_m = *tile_n = FEW;
     splits[0] = splits[1] = 1;
     return QNN_OK;
