@@ -83,6 +83,12 @@ __device__ __forceinline__ void finish8(float (&z)[8], const float (&bias)[8], c
 // The XOR is made on the side of the load's source, since a direct load fills LDS in lane order.
 // Rows past the matrix and k past its end are loaded from an offset past the buffer's size, which
 // fills LDS with zeros; stages past the last are such loads too, so the counts of loads in flight hold.
+//
+// The 16 bytes of a direct load may begin at any word.  So rows of fp32 and rows of 16-bit types of an even
+// length and stride are loaded as they are, and only the elements that a group of theirs would bring from
+// past the matrix or from the next row come after the loop, one at a time (Product::tail): of
+// 1890 x 1470 x 11714 bf16 the forward pass takes 90 us and the backward one 138 where copies padded to whole
+// groups made them 111 and 152, 22 x 1895 x 10407 fp32 backward 53 for 96.
 constexpr uint32_t PAST = 0x80000000u;  // a buffer offset that is past every size below
 
 // Waits until at most N of this wave's loads and none of its LDS reads are under way, then for the other
@@ -124,7 +130,7 @@ struct Side {
   static __device__ __forceinline__ int turn(int row) { return -(row >> 2) & 3; }  // of a chunk's index, DENSE
   static __device__ __forceinline__ int spread(int k) {  // what a granule's index is XORed with, not DENSE
     if constexpr (ES == 2) return ((k & 3) | (k >> 3 & 1) << 2) & GMASK;
-    else return k >> 2 & 3;
+    else return k >> 2 & 3 & GMASK;
   }
 
   uint32_t off[LOADS];  // this lane's byte offsets from the tile's corner, PAST outside the rows
@@ -215,6 +221,21 @@ __device__ __forceinline__ f4 mma(f4 a, f4 b, f4 acc) {
   }
 }
 
+// The lane's fragment of the last `count` elements of k, from element k on, straight from memory.
+template <class T, bool DENSE>
+__device__ __forceinline__ f4 rest(const Operand& o, int64_t row, int64_t k, int count, int lane) {
+  constexpr int GR = GROUP<T>;
+  Vec<T, GR> v = {};
+  if (lane < 16) {  // the others' part of the stage is past the end
+    row = row + lane < o.rows ? row + lane : o.rows - 1;
+    const T* p = (const T*)o.p + (DENSE ? row * o.ld + k : k * o.ld + row);
+#pragma unroll
+    for (int e = 0; e < GR; ++e)
+      if (e < count) v.v[e] = p[DENSE ? e : e * o.ld];
+  }
+  return __builtin_bit_cast(f4, v);
+}
+
 // One product, as a launch's workgroups take it.  Its tiles' sums go through the epilogue, or (splits > 1)
 // as they are into part[split][m][ldp].
 struct Product {
@@ -224,6 +245,8 @@ struct Product {
   int splits;
   int blocks;        // tm tn splits
   int64_t span;      // elements of k in a split, a whole number of stages
+  int tail, edge;    // the last elements of k that direct loads must not take, at most GROUP<T>, in all tiles and
+                     // in those that reach the end of an operand's rows
   float* part;
   int64_t ldp;
   Epilogue e;
@@ -312,7 +335,10 @@ __device__ __forceinline__ void tile(const Product& t, int id) {
   int split, ti, tj;
   tile_of(t, id, split, ti, tj);
   const int64_t i0 = (int64_t)ti * C::BM, j0 = (int64_t)tj * C::BN, k0 = split * t.span;
-  int left = (int)(t.k - k0 < t.span ? t.k - k0 : t.span);
+  const bool at_edge = (!AD && i0 + C::BM > t.a.rows) || (!BD && j0 + C::BN > t.b.rows);
+  const int tail = t.tail ? t.tail : at_edge ? t.edge : 0;
+  const int64_t whole = t.k - tail;
+  int left = (int)(whole - k0 < t.span ? whole - k0 : t.span);
   const int stages = (left + KE - 1) / KE;
   const int ri = wave / C::WN * 16 * TM, rj = wave % C::WN * 16 * TN;  // this wave's corner in the tile
 
@@ -382,6 +408,16 @@ __device__ __forceinline__ void tile(const Product& t, int id) {
   if (s < stages) step(s, std::integral_constant<int, 0>{});
   meet<0>();
 
+  if (tail && split == t.splits - 1) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[0][j] = rest<T, BD>(t.b, j0 + rj + 16 * j, whole, tail, lane);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const f4 a = rest<T, AD>(t.a, i0 + ri + 16 * i, whole, tail, lane);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = mma<T>(fb[0][j], a, acc[i][j]);
+    }
+  }
   emit<T, C>(t, acc, lds, split, i0, j0, ri, rj, wave, lane);
 }
 
@@ -397,17 +433,18 @@ __device__ __forceinline__ void static_for(F&& f) {
   }
 }
 
-// The same for operands DENSE in k whose rows begin anywhere, which direct loads do not take: 16 bytes a
-// lane into registers, four stages ahead, and from there to LDS.  Rows past the matrix are its last one
+// The same for 16-bit operands DENSE in k whose rows begin inside words, which direct loads do not take: 16
+// bytes a lane into registers, four stages ahead, and from there to LDS.  Rows past the matrix are its last one
 // again (their sums are not written); the stage that is no whole one comes first, so that all others'
 // loads need no guard.  Against padded copies it saves their launch and twice the operands' bytes:
 // 203 x 5003 x 1535 fp16 24.0 -> 18.6 us (with 1536 and direct loads: 11.6), 64 x 1000 x 4001 bf16
-// 17.1 -> 12.2, 2000 x 301 x 5003 fp32 80 -> 63 (six or eight stages ahead are no faster than four).
+// 17.1 -> 12.2 (six or eight stages ahead are no faster than four).
 template <class T, class C>
 __device__ __forceinline__ void loose_tile(const Product& t, int id) {
   using A = Side<T, true, C::BM, C::W>;
   using B = Side<T, true, C::BN, C::W>;
   constexpr int TM = C::TM, TN = C::TN, KE = A::KE, GR = GROUP<T>, P = A::LOADS + B::LOADS, D = 4;
+  static_assert(sizeof(T) == 2, "rows of 32 bits begin at words");
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int split, ti, tj;
@@ -434,16 +471,14 @@ __device__ __forceinline__ void loose_tile(const Product& t, int id) {
   // begins inside a word is loaded from the element before it on (there is one from stage 1 on), and its last
   // element comes from the lane with the row's next group, which has it first in its own -- for the last
   // group of a stage that is the first one's lane, with the next stage; after the last stage `tail`.
-  constexpr bool SHIFT = sizeof(T) == 2;
-  const bool shift = SHIFT && (((uintptr_t)t.a.p | (uintptr_t)t.b.p | (t.a.ld | t.b.ld | head) << 1) & 2);  // some do
   int odd[P], next[P];  // bytes of a word before the group; the lane with the next one
   uint32_t tail[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) {
-    odd[j] = SHIFT ? (int)((uintptr_t)from[j] & 2) : 0;
+    odd[j] = (int)((uintptr_t)from[j] & 2);
     const int chunk = group[j] / GR, flip = chunk ^ (lane & 3);
     next[j] = ((lane & ~3) | ((chunk + 1 & 3) ^ flip)) * 4;
-    if constexpr (SHIFT) tail[j] = reinterpret_cast<const uint16_t*>(from[j])[all - 1 - head - group[j]];
+    tail[j] = reinterpret_cast<const uint16_t*>(from[j])[all - 1 - head - group[j]];
   }
   Words held[D][P];  // stage s in held[s % D]
   auto load = [&](int s, auto slot) {  // stage s >= 1 (past the last: that one again, which is not used)
@@ -457,16 +492,11 @@ __device__ __forceinline__ void loose_tile(const Product& t, int id) {
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       const uint32_t* v = held[S][j].v;
-      uint4 w = {v[0], v[1], v[2], v[3]};
-      if (shift) {
-        const uint32_t mine = group[j] == 0 ? held[(S + 1) % D][j].v[0] : v[0];
-        uint32_t last = (uint32_t)__builtin_amdgcn_ds_bpermute(next[j], (int)mine);
-        last = s == stages - 1 && group[j] == 3 * GR ? tail[j] : last;
-        w.x = __builtin_amdgcn_alignbyte(v[1], v[0], odd[j]);
-        w.y = __builtin_amdgcn_alignbyte(v[2], v[1], odd[j]);
-        w.z = __builtin_amdgcn_alignbyte(v[3], v[2], odd[j]);
-        w.w = __builtin_amdgcn_alignbyte(last, v[3], odd[j]);
-      }
+      const uint32_t mine = group[j] == 0 ? held[(S + 1) % D][j].v[0] : v[0];
+      uint32_t last = (uint32_t)__builtin_amdgcn_ds_bpermute(next[j], (int)mine);
+      last = s == stages - 1 && group[j] == 3 * GR ? tail[j] : last;
+      const uint4 w = {__builtin_amdgcn_alignbyte(v[1], v[0], odd[j]), __builtin_amdgcn_alignbyte(v[2], v[1], odd[j]),
+                       __builtin_amdgcn_alignbyte(v[3], v[2], odd[j]), __builtin_amdgcn_alignbyte(last, v[3], odd[j])};
       *reinterpret_cast<uint4*>(lds + (s & 3) * C::SLOT + to[j]) = w;
     }
   };
@@ -741,11 +771,14 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* part, int s
 //   Middle 128 x 128  0.26  0.97   5   (8 waves)
 //   Half   128 x 64   0.19  0.50   4
 //   Small  64 x 64    0.10  0.25   4   (0.13 alone on its CU: latency)
+//   Low    32 x 64     -    0.21  1.5  (2 waves; 0.29 alone; fp32, whose MFMAs take Small longer than its bytes
+//                                       where few of its rows are there: 32 x 4096 x 4096 backward 60 -> 45 us)
 // A larger tile does more MFMAs for each byte it loads; a smaller one fills the chip with fewer rows.
 using Big = Cfg<2, 4, 8, 4, 2>;
 using Middle = Cfg<2, 4, 4, 2, 2>;
 using Half = Cfg<2, 2, 4, 2, 2>;
 using Small = Cfg<2, 2, 2, 2, 4>;
+using Low = Cfg<1, 2, 2, 2, 4>;
 struct Shape {
   int bm, bn;
   float stage16, stage32, ends, alone;  // alone: what one by itself on a CU takes of its stage's time (16 bits)
@@ -753,7 +786,8 @@ struct Shape {
 constexpr Shape SHAPES[] = {{Big::BM, Big::BN, 0.72f, 0.0f, 10.0f, 1.0f},
                             {Middle::BM, Middle::BN, 0.26f, 0.97f, 5.0f, 1.0f},
                             {Half::BM, Half::BN, 0.19f, 0.50f, 4.0f, 1.0f},
-                            {Small::BM, Small::BN, 0.105f, 0.25f, 4.0f, 1.2f}};
+                            {Small::BM, Small::BN, 0.105f, 0.25f, 4.0f, 1.2f},
+                            {Low::BM, Low::BN, 0.0f, 0.21f, 1.5f, 1.4f}};
 
 int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
@@ -782,23 +816,23 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0) {
   const int64_t ke = 64 / type_bytes(dtype);
   Plan best = {};
   float least = INFINITY;
-  for (int c = dtype == QNN_F32 && from == 0 ? 1 : from; c < 4; ++c) {
+  for (int c = dtype == QNN_F32 && from == 0 ? 1 : from; c < (dtype == QNN_F32 ? 5 : 4); ++c) {
     const Shape& h = SHAPES[c];
-    const float stage = dtype == QNN_F32 ? h.stage32 : h.stage16, alone = dtype == QNN_F32 ? 1.0f : h.alone;
+    const float stage = dtype == QNN_F32 ? h.stage32 : h.stage16, alone = dtype == QNN_F32 && c < 4 ? 1.0f : h.alone;
     int64_t tiles[2], stages[2];
     for (int i = 0; i < count; ++i) {
       tiles[i] = cdiv(size[i].m, h.bm) * cdiv(size[i].n, h.bn);
       stages[i] = cdiv(size[i].k, ke);
     }
     // a split for each product: none, or as many as give it so many workgroups
-    constexpr int WANT[] = {0, 128, 256, 512};
-    for (int x = 0; x < (count > 1 ? 16 : 4); ++x) {
+    constexpr int WANT[] = {0, 128, 256, 512, 1024}, WANTS = 5;
+    for (int x = 0; x < (count > 1 ? WANTS * WANTS : WANTS); ++x) {
       int64_t each[2], n[2];
       float work = 0.0f, longest = 0.0f, shortest = INFINITY, us = 0.0f;
       int64_t blocks = 0;
       bool skip = false, split = false;
       for (int i = 0; i < count; ++i) {
-        const int want = WANT[i ? x / 4 : x % 4];
+        const int want = WANT[i ? x / WANTS : x % WANTS];
         int64_t s = want / tiles[i];
         if (s > stages[i] / 4) s = stages[i] / 4;
         if (s > MAX_SPLITS) s = MAX_SPLITS;
@@ -837,27 +871,26 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0) {
 constexpr int FEW = 16;
 bool is_few(int64_t m, int64_t k, int dtype) { return m <= (dtype != QNN_F32 && k % 2 ? 2 : FEW); }
 
-// The forward product's plan: rows that are no whole number of groups are padded (a launch and their bytes
-// there and back, 4 us and 4 TB/s) or taken as they are, whichever is the less.  What
-// loose_tile does besides takes it to 1.3 of the Small tile's estimate in 16-bit types, none in fp32.
-Plan plan_y(const Size& z, int dtype) {
+// The forward product's plan where rows (of 16 bits) begin inside words: padded (a launch and their bytes there
+// and back, 4 us and 4 TB/s) or taken as they are, whichever is the less.  What loose_tile does besides takes
+// it to 1.3 of the Small tile's estimate.
+Plan plan_loose(const Size& z, int dtype) {
   Plan p = plan_of(&z, 1, dtype);
-  if (z.k * type_bytes(dtype) % 16 == 0) return p;
-  const float padded = p.us + 4.0f + (float)((z.m + z.n) * z.k) * (float)type_bytes(dtype) * 0.5e-6f;
+  const float padded = p.us + 4.0f + (float)((z.m + z.n) * z.k) * 1e-6f;
   Plan q = plan_of(&z, 1, dtype, 3);
-  if (q.us * (dtype == QNN_F32 ? 1.0f : 1.3f) > padded) return p;
+  if (q.us * 1.3f > padded) return p;
   q.loose = true;
   return q;
 }
 
 // The plan's product i of c = a b^T; its sums' scratch is taken from room.
-int product_of(Product& p, const Plan& plan, int i, const Size& z, const Operand& a, const Operand& b,
-               const Epilogue& e, char*& room) {
+int product_of(Product& p, const Plan& plan, int i, const Size& z, const Operand& a, const Operand& b, int tail,
+               int edge, const Epilogue& e, char*& room) {
   const Shape& h = SHAPES[plan.shape];
   const Split& s = plan.split[i];
   const int64_t tm = cdiv(z.m, h.bm), tn = cdiv(z.n, h.bn);
   QNN_REQUIRE(tm * tn * s.n < (1LL << 30) && tn < (1LL << 27), "too many tiles for one call");
-  p = {a, b, z.m, z.n, z.k, (int)tm, (int)tn, s.n, (int)(tm * tn * s.n), s.span, (float*)room, s.ldp, e};
+  p = {a, b, z.m, z.n, z.k, (int)tm, (int)tn, s.n, (int)(tm * tn * s.n), s.span, tail, edge, (float*)room, s.ldp, e};
   room += s.bytes;
   return QNN_OK;
 }
@@ -879,6 +912,8 @@ int with_cfg(int shape, F&& f) {
   if constexpr (sizeof(T) == 2)
     if (shape == 0) return f(Big{});
   if (shape == 1) return f(Middle{});
+  if constexpr (sizeof(T) == 4)
+    if (shape == 4) return f(Low{});
   if (shape == 2) return f(Half{});
   return f(Small{});
 }
@@ -927,11 +962,18 @@ int launch_grads(int shape, const Product (&p)[2], hipStream_t s) {
   return rc ? rc : join<T>(p, 2, s);
 }
 
+// Whether direct loads take the matrix's rows as they are: their groups begin at words.  A row's last group may
+// then reach past the row.  In an operand DENSE in k those last elements are left to Product::tail.  Else what
+// such a group brings from the next row belongs to columns past the operand's end, which are not written, and
+// only the last row, after which there is nothing, is left to the tail (so a row has to hold a group).
+bool at_words(const void* p, int64_t ld, int64_t cols, int dtype) {
+  return dtype == QNN_F32 || cols % 8 == 0 || ((uintptr_t)p % 4 == 0 && ld % 2 == 0 && cols % 2 == 0);
+}
+
 // A matrix as the tiled product takes it: itself, or (noted in `pads`) padded into `room`, of which it
 // takes what it needs.
 template <class T>
 void on_boundaries(const void*& p, int64_t& ld, int64_t rows, int64_t cols, char*& room, Padding& pads) {
-  if (cols % GROUP<T> == 0) return;
   const int64_t per = cdiv(cols, GROUP<T>);
   pads.one[pads.count++] = {p, room, ld, rows, cols, per, cdiv(rows * per, 256)};
   p = room;
@@ -949,15 +991,24 @@ int pad(const Padding& pads, hipStream_t s) {
   return QNN_OK;
 }
 
+// The room for that, whatever the matrix's row stride.
 int64_t padded_bytes(int64_t rows, int64_t cols, int dtype) {
-  const int64_t size = type_bytes(dtype), g = 16 / size;
-  return cols % g == 0 ? 0 : up(rows * up(cols, g) * size, 256);
+  const int64_t size = type_bytes(dtype), group = 16 / size;
+  return cols % group == 0 ? 0 : up(rows * up(cols, group) * size, 256);
+}
+// where it is taken as it is if its rows begin at words
+int64_t loose_bytes(int64_t rows, int64_t cols, int dtype) {
+  return dtype == QNN_F32 && cols >= 4 ? 0 : padded_bytes(rows, cols, dtype);
 }
 
 int64_t fwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
   if (is_few(m, k, dtype)) return 0;
-  const Plan p = plan_y({m, n, k}, dtype);
-  return (p.loose ? 0 : padded_bytes(m, k, dtype) + padded_bytes(n, k, dtype)) + p.split[0].bytes;
+  const Size z = {m, n, k};
+  const int64_t words = plan_of(&z, 1, dtype).split[0].bytes;
+  if (dtype == QNN_F32 || k % 8 == 0) return words;
+  const Plan p = plan_loose(z, dtype);
+  const int64_t loose = (p.loose ? 0 : padded_bytes(m, k, dtype) + padded_bytes(n, k, dtype)) + p.split[0].bytes;
+  return words > loose ? words : loose;
 }
 
 // Strips of rows for dz's sums: one of 16 rows at a time for a few rows, which saves the launch that adds
@@ -977,7 +1028,7 @@ int64_t bwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
   if (m == 0) return 0;
   const Size grads[2] = {{m, k, n}, {n, k, m}};
   const Plan p = plan_of(grads, 2, dtype);
-  return padded_bytes(m, n, dtype) + padded_bytes(n, k, dtype) + padded_bytes(m, k, dtype) +
+  return padded_bytes(m, n, dtype) + loose_bytes(n, k, dtype) + loose_bytes(m, k, dtype) +
          up(strips_of(m, n).n * n * 4, 256) + p.split[0].bytes + p.split[1].bytes;
 }
 
@@ -1043,20 +1094,22 @@ int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     const void *px = x, *pw = w;
     int64_t lx = ldx, lw = ldw;
     const Size z = {m, n, k};
-    const Plan plan = plan_y(z, dtype);
-    if (!plan.loose) {
+    const bool words = at_words(x, ldx, k, dtype) && at_words(w, ldw, k, dtype);
+    const Plan plan = words ? plan_of(&z, 1, dtype) : plan_loose(z, dtype);
+    if (!words && !plan.loose) {
       Padding pads = {};
       on_boundaries<T>(px, lx, m, k, room, pads);
       on_boundaries<T>(pw, lw, n, k, room, pads);
       if (int rc = pad<T>(pads, s)) return rc;
     }
     Product p;
-    if (int rc = product_of(p, plan, 0, z, {px, lx, m}, {pw, lw, n}, e, room)) return rc;
-    if (plan.loose) {
-      hipLaunchKernelGGL((linear_y_loose_kernel<T, Small>), dim3((unsigned)p.blocks), dim3(Small::NT), Small::LDS, s, p);
-      QNN_LAUNCH_CHECK("linear_y_loose_kernel");
-      return join<T>(&p, 1, s);
-    }
+    if (int rc = product_of(p, plan, 0, z, {px, lx, m}, {pw, lw, n}, words ? (int)(k % GROUP<T>) : 0, 0, e, room)) return rc;
+    if constexpr (sizeof(T) == 2)
+      if (plan.loose) {
+        hipLaunchKernelGGL((linear_y_loose_kernel<T, Small>), dim3((unsigned)p.blocks), dim3(Small::NT), Small::LDS, s, p);
+        QNN_LAUNCH_CHECK("linear_y_loose_kernel");
+        return join<T>(&p, 1, s);
+      }
     return launch_y<T>(plan.shape, p, s);
   });
 }
@@ -1071,7 +1124,8 @@ int qnn_linear_act_plan(int64_t m, int64_t n, int64_t k, int dtype, int grads, i
     return QNN_OK;
   }
   const Size y = {m, n, k}, both[2] = {{m, k, n}, {n, k, m}};
-  const Plan p = grads ? plan_of(both, 2, dtype) : plan_y(y, dtype);
+  const bool words = dtype == QNN_F32 || k % 2 == 0;
+  const Plan p = grads ? plan_of(both, 2, dtype) : words ? plan_of(&y, 1, dtype) : plan_loose(y, dtype);
   *tile_m = SHAPES[p.shape].bm;
   *tile_n = SHAPES[p.shape].bn;
   splits[0] = p.split[0].n;
@@ -1146,23 +1200,33 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
       }
       return (int)QNN_OK;
     }
-    Padding pads = {};
-    on_boundaries<T>(g, ldg, m, n, room, pads);
-    const void *px = x, *pw = w;
-    int64_t lx = ldx, lw = ldw;
-    if (dx) on_boundaries<T>(pw, lw, n, k, room, pads);
-    if (dw) on_boundaries<T>(px, lx, m, k, room, pads);
-    if (int rc = pad<T>(pads, s)) return rc;
     // one plan whichever of the two is wanted, as the workspace's size goes by it
     const Size z[2] = {{m, k, n}, {n, k, m}};
     const Plan plan = plan_of(z, 2, dtype);
+    // w and x: taken as they are; g: too, where padding it costs more than dx' product loses by it (its rows' short
+    // pieces then lie across the memory's lines: 1890 x 1470 x 11715 bf16 91 us padded, 107 as it is)
+    constexpr int64_t group = GROUP<T>;
+    const bool ww = at_words(w, ldw, k, dtype) && k >= group, xw = at_words(x, ldx, k, dtype) && k >= group;
+    const bool pads_too = (dx && !ww) || (dw && !xw);
+    const float loss = dx ? plan.us * (dtype == QNN_F32 ? 0.04f : 0.1f) : 0.0f;
+    const bool gw = at_words(g, ldg, n, dtype) && n >= group &&
+                    (n % group == 0 || loss < (float)(m * n) * 0.5e-6f * sizeof(T) + (pads_too ? 0.0f : 4.0f));
+    Padding pads = {};
+    if (!gw) on_boundaries<T>(g, ldg, m, n, room, pads);
+    const void *px = x, *pw = w;
+    int64_t lx = ldx, lw = ldw;
+    if (dx && !ww) on_boundaries<T>(pw, lw, n, k, room, pads);
+    if (dw && !xw) on_boundaries<T>(px, lx, m, k, room, pads);
+    if (int rc = pad<T>(pads, s)) return rc;
+    const int over = gw ? (int)(n % group) : 0, all = (int)((n - 1) % group + 1);
+    const int dx_edge = ww && k % group ? all : 0, dw_edge = over || (xw && k % group) ? 1 : 0;
     Product p[2] = {};
     const Epilogue to_dx = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE};
     const Epilogue to_dw = {nullptr, nullptr, 0, dw, nullptr, QNN_ACT_NONE};
     if (dx)
-      if (int rc = product_of(p[0], plan, 0, z[0], {g, ldg, m}, {pw, lw, k}, to_dx, room)) return rc;
+      if (int rc = product_of(p[0], plan, 0, z[0], {g, ldg, m}, {pw, lw, k}, over, dx_edge, to_dx, room)) return rc;
     if (dw)
-      if (int rc = product_of(p[1], plan, 1, z[1], {g, ldg, n}, {px, lx, k}, to_dw, room)) return rc;
+      if (int rc = product_of(p[1], plan, 1, z[1], {g, ldg, n}, {px, lx, k}, 0, dw_edge, to_dw, room)) return rc;
     if (int rc = launch_grads<T>(plan.shape, p, s)) return rc;
     return (int)QNN_OK;
   });

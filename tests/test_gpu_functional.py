@@ -137,6 +137,44 @@ def test_linear_act_rows_that_begin_anywhere(F, dt, m, n, k):
 
 
 @pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(20, 70, 2), (20, 70, 6), (33, 66, 30), (65, 130, 46), (64, 6, 100), (17, 10, 12), (100, 1002, 94), (64, 100, 4002),
+                                   (130, 2002, 514), (1000, 1002, 258), (40, 34, 20002), (203, 1006, 1030), (510, 4082, 1026),
+                                   (700, 5102, 138), (1, 70, 4098), (18, 1000, 1002), (2002, 1470, 1034)])
+def test_linear_act_rows_that_begin_at_words(F, dt, m, n, k):
+    """Even lengths that are no whole groups, around whole stages, short and split reductions, edges on both sides."""
+    x, w, b, r, dy = linear_case(m, n, k, dt, m % 2 == 0, k % 4 == 2)
+    linear_check(F, x, w, b, r, dy, ("none", "gelu", "relu")[m % 3])
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("n,k", [(66, 72), (72, 66), (66, 70), (66, 67), (67, 66)])
+@pytest.mark.parametrize("m", [30, 200])
+def test_linear_act_infinities_at_the_ends_of_rows(F, dt, m, n, k):
+    """An infinity in a row's last element, next to the following row's first, stays in its row and column, and what lies
+    between the rows is not read."""
+    def matrix(rows, cols, gap, seed, at):
+        v = torch.full((rows, cols + gap), math.nan, dtype=dt, device="cuda")
+        v[:, :cols] = torch.randn(rows, cols, generator=gen(seed)).to(dt).cuda()
+        for i, j in at:
+            v[i, j] = math.inf
+        return v[:, :cols]
+    for gap in (0, 2, 3):
+        a, c = matrix(m, k, gap, 60, [(3, k - 1), (4, 0)]), matrix(n, k, gap, 61, [(9, k - 1), (12, 0)])
+        d = matrix(m, n, gap, 62, [(5, n - 1), (7, 0), (m - 1, n - 1)])
+        want = O.linear_act(a.cpu(), c.cpu(), None, None, "none", d.cpu())
+        a.requires_grad_(True), c.requires_grad_(True)
+        y = F.linear_act(a, c)
+        assert torch.isfinite(want["y"][0]).any() and not torch.isfinite(want["dw"][0]).all()
+        near(y, want["y"], f"{gap} y")
+        for q, v in zip(("dx", "dw"), torch.autograd.grad(y, (a, c), d)):
+            near(v, want[q], f"{gap} {q}")
+
+
+def test_linear_act_low_tiles_are_taken(F):
+    assert {plan(m, n, k, torch.float32, g)[0] for m, n, k in ((18, 1000, 1002), (20, 4096, 1000), (30, 10000, 2000), (510, 500, 512)) for g in (False, True)} >= {(32, 64)}
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
 def test_linear_act_around_few_rows(F, dt):
     for m in (2, 4, 8, 15, 16, 17, 18):
         for n, k in ((50, 1000), (33, 77), (16, 2050)):
