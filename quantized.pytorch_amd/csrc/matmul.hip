@@ -781,13 +781,15 @@ using Small = Cfg<2, 2, 2, 2, 4>;
 using Low = Cfg<1, 2, 2, 2, 4>;
 struct Shape {
   int bm, bn;
-  float stage16, stage32, ends, alone;  // alone: what one by itself on a CU takes of its stage's time (16 bits)
+  float stage16, stage32, ends;
+  float alone;   // what one by itself on a CU takes of its stage's time (16 bits, and Low)
+  float across;  // what each takes where the first operand's rows, DENSE, lie across 64-byte boundaries (16 bits)
 };
-constexpr Shape SHAPES[] = {{Big::BM, Big::BN, 0.72f, 0.0f, 10.0f, 1.0f},
-                            {Middle::BM, Middle::BN, 0.26f, 0.97f, 5.0f, 1.0f},
-                            {Half::BM, Half::BN, 0.19f, 0.50f, 4.0f, 1.0f},
-                            {Small::BM, Small::BN, 0.105f, 0.25f, 4.0f, 1.2f},
-                            {Low::BM, Low::BN, 0.0f, 0.21f, 1.5f, 1.4f}};
+constexpr Shape SHAPES[] = {{Big::BM, Big::BN, 0.72f, 0.0f, 10.0f, 1.0f, 1.0f},
+                            {Middle::BM, Middle::BN, 0.26f, 0.97f, 5.0f, 1.0f, 1.4f},
+                            {Half::BM, Half::BN, 0.19f, 0.50f, 4.0f, 1.0f, 1.6f},
+                            {Small::BM, Small::BN, 0.105f, 0.25f, 4.0f, 1.2f, 1.5f},
+                            {Low::BM, Low::BN, 0.0f, 0.21f, 1.5f, 1.4f, 1.0f}};
 
 int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
@@ -811,7 +813,7 @@ constexpr int MAX_SPLITS = 64;
 // The tile and the splits of k of the one or two products of a launch: the least of the times above for
 // the busiest of 256 CUs; splits cost a second launch (5.5 us with its host time) and their sums' way
 // through memory (at 4 TB/s).  Over the sizes that were swept (m, n 64 to 8192, k 64 to 8192) what it
-// picks for one product is within 10 % of the best pair, 20 % where the whole takes under 20 us.
+// picks for one product is mostly within 10 % of the best pair, 20 % where the whole takes under 20 us.
 Plan plan_of(const Size* size, int count, int dtype, int from = 0) {
   const int64_t ke = 64 / type_bytes(dtype);
   Plan best = {};
@@ -819,6 +821,7 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0) {
   for (int c = dtype == QNN_F32 && from == 0 ? 1 : from; c < (dtype == QNN_F32 ? 5 : 4); ++c) {
     const Shape& h = SHAPES[c];
     const float stage = dtype == QNN_F32 ? h.stage32 : h.stage16, alone = dtype == QNN_F32 && c < 4 ? 1.0f : h.alone;
+    const float across = dtype != QNN_F32 && size[0].k % 32 != 0 ? h.across : 1.0f;
     int64_t tiles[2], stages[2];
     for (int i = 0; i < count; ++i) {
       tiles[i] = cdiv(size[i].m, h.bm) * cdiv(size[i].n, h.bn);
@@ -841,9 +844,10 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0) {
         each[i] = cdiv(stages[i], s);
         n[i] = cdiv(stages[i], each[i]);
         blocks += tiles[i] * n[i];
-        work += (float)(tiles[i] * n[i]) * (float)each[i];
-        longest = fmaxf(longest, (float)each[i]);
-        shortest = fminf(shortest, (float)each[i]);
+        const float time = (float)each[i] * (i == 0 ? across : 1.0f);
+        work += (float)(tiles[i] * n[i]) * time;
+        longest = fmaxf(longest, time);
+        shortest = fminf(shortest, time);
         split = split || n[i] > 1;
         if (n[i] > 1) us += (float)(n[i] * size[i].m * size[i].n) * 2e-6f;
       }
@@ -867,9 +871,13 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0) {
 }
 
 // Whether few_rows_kernel takes the forward product: up to 16 rows of x, but 2 where the rows' groups begin
-// inside words (16 x 4096 x 4097 bf16 takes it 27 us and loose_tile 18, 4 rows 21, one row 16 us).
+// inside words (16 x 4096 x 4097 bf16 takes it 27 us and loose_tile 18, 4 rows 21, one row 16 us), and one
+// where w of 16-bit types is large (2 x 8192 x 8191 bf16 72 us and 33 in tiles, 8 x 8192 x 8192 28 and 23; but 9 x 4096 x 4096 8.8 and 10.1 us).
 constexpr int FEW = 16;
-bool is_few(int64_t m, int64_t k, int dtype) { return m <= (dtype != QNN_F32 && k % 2 ? 2 : FEW); }
+bool is_few(int64_t m, int64_t n, int64_t k, int dtype) {
+  if (dtype == QNN_F32) return m <= FEW;
+  return n * k > 20000000 ? m == 1 : m <= (k % 2 ? 2 : FEW);
+}
 
 // The forward product's plan where rows (of 16 bits) begin inside words: padded (a launch and their bytes there
 // and back, 4 us and 4 TB/s) or taken as they are, whichever is the less.  What loose_tile does besides takes
@@ -1002,7 +1010,7 @@ int64_t loose_bytes(int64_t rows, int64_t cols, int dtype) {
 }
 
 int64_t fwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
-  if (is_few(m, k, dtype)) return 0;
+  if (is_few(m, n, k, dtype)) return 0;
   const Size z = {m, n, k};
   const int64_t words = plan_of(&z, 1, dtype).split[0].bytes;
   if (dtype == QNN_F32 || k % 8 == 0) return words;
@@ -1084,7 +1092,7 @@ int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     using T = decltype(t);
     hipStream_t s = (hipStream_t)stream;
     const Epilogue e = {bias, res, ldr, y, slope, act};
-    if (is_few(m, k, dtype)) {
+    if (is_few(m, n, k, dtype)) {
       hipLaunchKernelGGL((few_rows_kernel<T, 16>), dim3((unsigned)cdiv(n, 16)), dim3(1024), 0, s, (const T*)x, ldx,
                          (const T*)w, ldw, (int)m, n, k, e);
       QNN_LAUNCH_CHECK("few_rows_kernel");
@@ -1118,7 +1126,7 @@ int qnn_linear_act_plan(int64_t m, int64_t n, int64_t k, int dtype, int grads, i
   if (int rc = check(m, n, k, dtype)) return rc;
   QNN_REQUIRE(m > 0, "m: at least 1");
   QNN_REQUIRE(tile_m && tile_n && splits, "null pointer");
-  if (!grads && is_few(m, k, dtype)) {
+  if (!grads && is_few(m, n, k, dtype)) {
     *tile_m = *tile_n = FEW;
     splits[0] = splits[1] = 1;
     return QNN_OK;
