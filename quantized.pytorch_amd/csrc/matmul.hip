@@ -814,14 +814,14 @@ constexpr int MAX_SPLITS = 64;
 // the busiest of 256 CUs; splits cost a second launch (5.5 us with its host time) and their sums' way
 // through memory (at 4 TB/s).  Over the sizes that were swept (m, n 64 to 8192, k 64 to 8192) what it
 // picks for one product is mostly within 10 % of the best pair, 20 % where the whole takes under 20 us.
-Plan plan_of(const Size* size, int count, int dtype, int from = 0) {
+Plan plan_of(const Size* size, int count, int dtype, int from = 0, bool dense = true) {
   const int64_t ke = 64 / type_bytes(dtype);
   Plan best = {};
   float least = INFINITY;
   for (int c = dtype == QNN_F32 && from == 0 ? 1 : from; c < (dtype == QNN_F32 ? 5 : 4); ++c) {
     const Shape& h = SHAPES[c];
     const float stage = dtype == QNN_F32 ? h.stage32 : h.stage16, alone = dtype == QNN_F32 && c < 4 ? 1.0f : h.alone;
-    const float across = dtype != QNN_F32 && size[0].k % 32 != 0 ? h.across : 1.0f;
+    const float across = dtype != QNN_F32 && dense && size[0].k % 32 != 0 ? h.across : 1.0f;
     int64_t tiles[2], stages[2];
     for (int i = 0; i < count; ++i) {
       tiles[i] = cdiv(size[i].m, h.bm) * cdiv(size[i].n, h.bn);
@@ -889,6 +889,20 @@ Plan plan_loose(const Size& z, int dtype) {
   if (q.us * 1.3f > padded) return p;
   q.loose = true;
   return q;
+}
+
+// The plans of dx and dw: one launch, or two where tiles of one shape would cost well more (5 x 11562 x 7871 fp32,
+// whose dx has 5 rows and dw 91 million elements: 203 us for 264).
+struct Grads {
+  Plan plan[2];  // one launch: the same one
+  bool apart;
+};
+Grads plan_grads(int64_t m, int64_t n, int64_t k, int dtype) {
+  const Size z[2] = {{m, k, n}, {n, k, m}};
+  Plan both = plan_of(z, 2, dtype), dx = plan_of(z, 1, dtype), dw = plan_of(z + 1, 1, dtype, 0, false);
+  if (dx.us + dw.us + 4.0f > 0.85f * both.us) return {{both, both}, false};
+  dw.split[1] = dw.split[0];
+  return {{dx, dw}, true};
 }
 
 // The plan's product i of c = a b^T; its sums' scratch is taken from room.
@@ -1034,10 +1048,9 @@ Strips strips_of(int64_t m, int64_t n) {
 
 int64_t bwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
   if (m == 0) return 0;
-  const Size grads[2] = {{m, k, n}, {n, k, m}};
-  const Plan p = plan_of(grads, 2, dtype);
+  const Grads p = plan_grads(m, n, k, dtype);
   return padded_bytes(m, n, dtype) + loose_bytes(n, k, dtype) + loose_bytes(m, k, dtype) +
-         up(strips_of(m, n).n * n * 4, 256) + p.split[0].bytes + p.split[1].bytes;
+         up(strips_of(m, n).n * n * 4, 256) + p.plan[0].split[0].bytes + p.plan[1].split[1].bytes;
 }
 
 constexpr int64_t LONGEST = 1LL << 21;  // of a row stride: offsets inside a tile's rows are 32 bits
@@ -1131,13 +1144,19 @@ int qnn_linear_act_plan(int64_t m, int64_t n, int64_t k, int dtype, int grads, i
     splits[0] = splits[1] = 1;
     return QNN_OK;
   }
-  const Size y = {m, n, k}, both[2] = {{m, k, n}, {n, k, m}};
+  const Size y = {m, n, k};
   const bool words = dtype == QNN_F32 || k % 2 == 0;
-  const Plan p = grads ? plan_of(both, 2, dtype) : words ? plan_of(&y, 1, dtype) : plan_loose(y, dtype);
-  *tile_m = SHAPES[p.shape].bm;
-  *tile_n = SHAPES[p.shape].bn;
-  splits[0] = p.split[0].n;
-  splits[1] = grads ? p.split[1].n : 1;
+  Plan p[2] = {};
+  if (grads) {
+    const Grads both = plan_grads(m, n, k, dtype);
+    p[0] = both.plan[0], p[1] = both.plan[1];
+  } else {
+    p[0] = words ? plan_of(&y, 1, dtype) : plan_loose(y, dtype);
+  }
+  *tile_m = SHAPES[p[0].shape].bm;
+  *tile_n = SHAPES[p[0].shape].bn;
+  splits[0] = p[0].split[0].n;
+  splits[1] = grads ? p[1].split[1].n : 1;
   return QNN_OK;
 }
 
@@ -1210,13 +1229,13 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
     }
     // one plan whichever of the two is wanted, as the workspace's size goes by it
     const Size z[2] = {{m, k, n}, {n, k, m}};
-    const Plan plan = plan_of(z, 2, dtype);
+    const Grads plan = plan_grads(m, n, k, dtype);
     // w and x: taken as they are; g: too, where padding it costs more than dx' product loses by it (its rows' short
     // pieces then lie across the memory's lines: 1890 x 1470 x 11715 bf16 91 us padded, 107 as it is)
     constexpr int64_t group = GROUP<T>;
     const bool ww = at_words(w, ldw, k, dtype) && k >= group, xw = at_words(x, ldx, k, dtype) && k >= group;
     const bool pads_too = (dx && !ww) || (dw && !xw);
-    const float loss = dx ? plan.us * (dtype == QNN_F32 ? 0.04f : 0.1f) : 0.0f;
+    const float loss = dx ? plan.plan[0].us * (dtype == QNN_F32 ? 0.04f : 0.1f) : 0.0f;
     const bool gw = at_words(g, ldg, n, dtype) && n >= group &&
                     (n % group == 0 || loss < (float)(m * n) * 0.5e-6f * sizeof(T) + (pads_too ? 0.0f : 4.0f));
     Padding pads = {};
@@ -1232,10 +1251,16 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
     const Epilogue to_dx = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE};
     const Epilogue to_dw = {nullptr, nullptr, 0, dw, nullptr, QNN_ACT_NONE};
     if (dx)
-      if (int rc = product_of(p[0], plan, 0, z[0], {g, ldg, m}, {pw, lw, k}, over, dx_edge, to_dx, room)) return rc;
+      if (int rc = product_of(p[0], plan.plan[0], 0, z[0], {g, ldg, m}, {pw, lw, k}, over, dx_edge, to_dx, room)) return rc;
     if (dw)
-      if (int rc = product_of(p[1], plan, 1, z[1], {g, ldg, n}, {px, lx, k}, 0, dw_edge, to_dw, room)) return rc;
-    if (int rc = launch_grads<T>(plan.shape, p, s)) return rc;
+      if (int rc = product_of(p[1], plan.plan[1], 1, z[1], {g, ldg, n}, {px, lx, k}, 0, dw_edge, to_dw, room)) return rc;
+    if (!plan.apart) return launch_grads<T>(plan.plan[0].shape, p, s);
+    for (int i = 0; i < 2; ++i) {
+      Product one[2] = {};
+      one[i] = p[i];
+      if (p[i].blocks > 0)
+        if (int rc = launch_grads<T>(plan.plan[i].shape, one, s)) return rc;
+    }
     return (int)QNN_OK;
   });
 }
