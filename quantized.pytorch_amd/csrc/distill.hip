@@ -8,6 +8,7 @@
 // into pieces whose (maximum, sum) pairs a second launch joins.  The gradient is dense but for the
 // teacher's classes: a workgroup writes its piece of the row as if there were none, and then the
 // classes that lie in it again, the first entry of a class with the sum of all of them.
+// 4096 x 131072 bf16, 64 entries a row: forward 221 us (4.9 TB/s), gradient 390 (5.5 TB/s).
 //
 // stats, four floats a row: the largest student logit, 1 / sum of e^((s - largest) / T), the largest
 // teacher logit, 1 / the teacher's sum (0: the row is not counted); then the number of counted rows.

@@ -1,5 +1,5 @@
 // Shared by the float operators (matmul.hip, layer_norm.hip, distill.hip): element types,
-// 16-byte groups of a row, reductions over a wave, the activations.
+// 16-byte groups of a row, the activations.
 #pragma once
 #include <math.h>
 
@@ -104,21 +104,12 @@ __device__ __forceinline__ void store_n(T* p, const float (&o)[N], int64_t left)
   }
 }
 
-__device__ __forceinline__ float wave_sum_f(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-
-// e^x by the hardware's 2^x; the product's rounding costs |x| 2^-24 of relative error.
-__device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
-
 // GELU z Phi(z) and its derivative Phi(z) + z phi(z) together, from one exponential.  With a = |z|, the
 // tail Phi(-a) = erfc(a / sqrt 2) / 2 = e^(-a^2 / 2) t P(t), t = 1 / (1 + c a), P fitted here to the
 // scaled complement e^(u^2) erfc(u), so that the far negative side keeps its relative precision too:
 //   y = max(z, 0) - a tail,  slope = d below 0 and 1 - d above, d = tail - a phi(a).
 // For results of 16 bits P has degree 5 (relative error 1.1e-6 to |z| = 6.5, past which y is under 1e-9;
-// fp16's half step is 2.4e-4); for fp32 degree 9 (3.6e-8 everywhere) and a^2 with its rounding error.
+// fp16's rounding is 4.9e-4 of the value); for fp32 degree 9 (3.6e-8 everywhere) and a^2 with its rounding error.
 // The two products with a take it clamped, which gives the limits at the infinities; a NaN stays one.
 template <bool FP32>
 __device__ __forceinline__ void gelu_f(float z, float& y, float& slope) {
@@ -155,7 +146,7 @@ __device__ __forceinline__ void gelu_f(float z, float& y, float& slope) {
 }
 
 // The derivative of GELU between the passes, for 16-bit types: fixed point of 1 / 28672 from 8192 (it lies
-// in [-0.13, 1.13]; 0 is a NaN), off by at most 1.8e-5 -- a fourteenth of fp16's half step at 1, where z
+// in [-0.13, 1.13]; 0 is a NaN), off by at most 1.8e-5 -- a fourteenth of fp16's half step below 1 (2^-12), where z
 // itself rounded to the type would add an error as large as that of the gradient's own rounding.
 constexpr float SLOPE_STEPS = 28672.0f;
 __device__ __forceinline__ int16_t slope_pack(float d) {

@@ -5,11 +5,13 @@
 //
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx, each once.  A row
 // lives in the registers of L lanes (G groups of 16 bytes a lane), so the two-step variance and the two
-// means of the backward pass cost no second read.  A workgroup takes rows in strides of the grid and
-// loads its next row before it works on the present one; the weights stay in registers from row to
-// row.  The backward pass sums dw and db on the way: a lane has the same columns in every row, so they
-// are sums in its registers, joined over a workgroup's rows in LDS, written as one partial row a
-// workgroup and added up by a second, small launch in a fixed order.
+// means of the backward pass cost no second read.  A workgroup takes rows in strides of the grid with
+// the next two on their way while it works on one; the weights stay in registers from row to row.
+// 16384 x 4096 bf16: forward 47 us (5.7 TB/s), backward 85 (4.7 TB/s) and 5.
+//
+// The backward pass sums dw and db on the way: a lane has the same columns in every row, so they are sums
+// in its registers, joined over a workgroup's rows in LDS, written as one partial row a workgroup and
+// added up by a second, small launch in a fixed order.
 #include "float_common.h"
 
 namespace qnn {

@@ -598,8 +598,9 @@ __global__ __launch_bounds__(256) void matmul_join_kernel(Joins j) {
 // y for up to 16 rows of x, both operands dense in k.  A workgroup has 16 outputs; its waves share
 // k between them in turns of 128 bytes a row, loads going straight into the fragments, and join
 // their sums in LDS in a fixed order.  Bound by the weight's way from HBM: one row of 16384 x 16384
-// bf16 in 109 us (4.9 TB/s), of 4096 x 4096 in 7.2; the launch's waves have most of it in flight at once.  Rows past either matrix are its last one again: their sums are not
-// written, and no load needs a guard but those of the last turn, where k ends inside it.
+// bf16 in 109 us (4.9 TB/s), of 4096 x 4096 in 7.2; the launch's waves have most of it in flight at once.
+// Rows past either matrix are its last one again: their sums are not written, and no load needs a guard but
+// those of the last turn, where k ends inside it.
 template <class T, int W>
 __global__ __launch_bounds__(64 * W) void few_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int m,
                                                           int64_t n, int64_t k, Epilogue e) {
@@ -871,8 +872,9 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0, bool dense = 
 }
 
 // Whether few_rows_kernel takes the forward product: up to 16 rows of x, but 2 where the rows' groups begin
-// inside words (16 x 4096 x 4097 bf16 takes it 27 us and loose_tile 18, 4 rows 21, one row 16 us), and one
-// where w of 16-bit types is large (2 x 8192 x 8191 bf16 72 us and 33 in tiles, 8 x 8192 x 8192 28 and 23; but 9 x 4096 x 4096 8.8 and 10.1 us).
+// inside words (4 x 4096 x 4097 bf16 takes it 21 us and loose_tile 18, one row 16), and one where w of 16-bit
+// types is large (2 x 8192 x 8191 bf16 72 us and 33 in tiles, 8 x 8192 x 8192 28 and 23; but 9 x 4096 x 4096
+// 8.8 and 10.1).
 constexpr int FEW = 16;
 bool is_few(int64_t m, int64_t n, int64_t k, int dtype) {
   if (dtype == QNN_F32) return m <= FEW;
@@ -1124,7 +1126,8 @@ int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
       if (int rc = pad<T>(pads, s)) return rc;
     }
     Product p;
-    if (int rc = product_of(p, plan, 0, z, {px, lx, m}, {pw, lw, n}, words ? (int)(k % GROUP<T>) : 0, 0, e, room)) return rc;
+    const int tail = words ? (int)(k % GROUP<T>) : 0;
+    if (int rc = product_of(p, plan, 0, z, {px, lx, m}, {pw, lw, n}, tail, 0, e, room)) return rc;
     if constexpr (sizeof(T) == 2)
       if (plan.loose) {
         hipLaunchKernelGGL((linear_y_loose_kernel<T, Small>), dim3((unsigned)p.blocks), dim3(Small::NT), Small::LDS, s, p);

@@ -143,7 +143,9 @@ def test_misaligned_rows_and_missing_work_are_refused():
     assert rc == 1 and b"boundaries" in msg
     rc, msg = _call("qnn_linear_act_fwd", P, 65, P, 64, None, None, 0, P, None, 20, 8, 64, 1, 0, P, 1 << 20, None)
     assert rc == 1 and b"boundaries" in msg
-    rc, msg = _call("qnn_linear_act_fwd", P, 63, P, 63, None, None, 0, P, None, 20, 8, 63, 1, 0, None, 0, None)
+    rc, msg = _call("qnn_linear_act_fwd", P, 8192, P, 8192, None, None, 0, P, None, 64, 64, 8192, 0, 0, None, 0, None)
+    assert rc == 1 and b"work" in msg
+    rc, msg = _call("qnn_linear_act_bwd", P, 9, None, P, 64, P, 64, None, P, P, None, 20, 9, 64, 1, 0, None, 0, None)
     assert rc == 1 and b"work" in msg
     rc, msg = _call("qnn_layer_norm_bwd", P, 8, P, 8, P, P, P, P, P, P, 4, 8, 0, 0, None, 0, None)
     assert rc == 1 and b"work" in msg
