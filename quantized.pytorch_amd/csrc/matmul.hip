@@ -557,11 +557,57 @@ __global__ __launch_bounds__(C::NT, C::EU) void linear_y_loose_kernel(Product y)
   loose_tile<T, C>(y, blockIdx.x);
 }
 
+// db of a few rows of dy beside the products (no activation: dz is dy), 64 columns a workgroup: one launch less
+// in front of them.
+struct ColumnSums {
+  const void* dy;
+  void* db;
+  int64_t ldy, m, n;
+  int blocks;  // 0: not wanted
+};
+template <class T, class C>
+__device__ __forceinline__ void column_sums(const ColumnSums& t, int id) {
+  constexpr int SUBS = C::NT / 8, U = 4;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  float(*sh)[64] = reinterpret_cast<float(*)[64]>(lds);
+  const int in = threadIdx.x & 7, sub = threadIdx.x >> 3;
+  const int64_t c = (int64_t)id * 64 + in * 8, left = t.n - c;
+  float sum[8] = {};
+  if (left > 0)
+    for (int64_t r = sub; r < t.m; r += U * SUBS) {
+      Vec<T, 8> g[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {  // (past the last row: that one again, which is not used)
+        const int64_t k = r + u * SUBS < t.m ? r + u * SUBS : t.m - 1;
+        g[u] = load_eight((const T*)t.dy + k * t.ldy + c, left);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += r + u * SUBS < t.m ? (float)g[u].v[i] : 0.0f;
+    }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sh[sub][in * 8 + i] = sum[i];
+  __syncthreads();
+  const int64_t col = (int64_t)id * 64 + threadIdx.x;
+  if (threadIdx.x < 64 && col < t.n) {
+    float s = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < SUBS; ++k) s += sh[k][threadIdx.x];
+    ((T*)t.db)[col] = (T)s;
+  }
+}
+
 // dx = dz w and dw = dz^T x in one launch, so that the one's last tiles and the other's first share the
 // chip.  The first's workgroups are counted up to a multiple of 8, which keeps the second's on the XCDs
 // that tile_of takes them to be on; a product with no workgroups is not wanted.
 template <class T, class C>
-__global__ __launch_bounds__(C::NT, C::EU) void linear_grads_kernel(Product dx, Product dw, int dw_first) {
+__global__ __launch_bounds__(C::NT, C::EU) void linear_grads_kernel(Product dx, Product dw, int dw_first,
+                                                                    ColumnSums db) {
+  if (const int rest = (int)gridDim.x - db.blocks; (int)blockIdx.x >= rest) {
+    column_sums<T, C>(db, blockIdx.x - rest);
+    return;
+  }
   const int lead = ((dw_first ? dw.blocks : dx.blocks) + 7) & ~7, id = blockIdx.x;
   const bool is_dw = (id < lead) == (dw_first != 0);
   const int at = id < lead ? id : id - lead;
@@ -900,11 +946,21 @@ struct Grads {
   bool apart;
 };
 Grads plan_grads(int64_t m, int64_t n, int64_t k, int dtype) {
+  // 3 us of host time, asked for twice a call: the last ones are kept
+  struct Kept {
+    int64_t m, n, k;
+    int dtype;
+    Grads g;
+  };
+  static thread_local Kept kept[32] = {};
+  Kept& slot = kept[(m * 31 + n * 7 + k + dtype) & 31];
+  if (slot.m == m && slot.n == n && slot.k == k && slot.dtype == dtype) return slot.g;
   const Size z[2] = {{m, k, n}, {n, k, m}};
   Plan both = plan_of(z, 2, dtype), dx = plan_of(z, 1, dtype), dw = plan_of(z + 1, 1, dtype, 0, false);
-  if (dx.us + dw.us + 4.0f > 0.85f * both.us) return {{both, both}, false};
-  dw.split[1] = dw.split[0];
-  return {{dx, dw}, true};
+  const bool apart = dx.us + dw.us + 4.0f < 0.85f * both.us;
+  if (apart) dw.split[1] = dw.split[0];
+  slot = {m, n, k, dtype, apart ? Grads{{dx, dw}, true} : Grads{{both, both}, false}};
+  return slot.g;
 }
 
 // The plan's product i of c = a b^T; its sums' scratch is taken from room.
@@ -972,14 +1028,14 @@ int launch_y(int shape, const Product& y, hipStream_t s) {
 
 // p: dx, dw (no blocks: not wanted); the one whose workgroups take longer goes first
 template <class T>
-int launch_grads(int shape, const Product (&p)[2], hipStream_t s) {
+int launch_grads(int shape, const Product (&p)[2], const ColumnSums& db, hipStream_t s) {
   const int rc = with_cfg<T>(shape, [&](auto cfg) {
     using C = decltype(cfg);
     static std::atomic<uint64_t> told{0};
     if (int rc = allow_lds((const void*)&linear_grads_kernel<T, C>, C::LDS, told)) return rc;
     const int first = p[1].blocks > 0 && (p[0].blocks == 0 || p[1].span > p[0].span) ? 1 : 0;
-    const unsigned blocks = (unsigned)up(p[first].blocks, 8) + (unsigned)p[1 - first].blocks;
-    hipLaunchKernelGGL((linear_grads_kernel<T, C>), dim3(blocks), dim3(C::NT), C::LDS, s, p[0], p[1], first);
+    const unsigned blocks = (unsigned)up(p[first].blocks, 8) + (unsigned)p[1 - first].blocks + (unsigned)db.blocks;
+    hipLaunchKernelGGL((linear_grads_kernel<T, C>), dim3(blocks), dim3(C::NT), C::LDS, s, p[0], p[1], first, db);
     QNN_LAUNCH_CHECK("linear_grads_kernel");
     return (int)QNN_OK;
   });
@@ -1196,7 +1252,9 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
     const Strips st = strips_of(m, n);
     float* part = db && st.n > 1 ? (float*)room : nullptr;
     room += up(st.n * n * 4, 256);
-    if (m > 0 && (act != QNN_ACT_NONE || db)) {
+    const Grads plan = m > 0 ? plan_grads(m, n, k, dtype) : Grads{};
+    const bool db_beside = db && act == QNN_ACT_NONE && st.n == 1 && (dx || dw) && !plan.apart;
+    if (m > 0 && (act != QNN_ACT_NONE || (db && !db_beside))) {
       QNN_REQUIRE(st.n * st.chunks < (1LL << 31), "too many rows for one call");
       auto launch_dz = [&](auto subs, auto of) {
         constexpr int SUBS = decltype(subs)::value, ACT = decltype(of)::value;
@@ -1230,9 +1288,7 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
       }
       return (int)QNN_OK;
     }
-    // one plan whichever of the two is wanted, as the workspace's size goes by it
     const Size z[2] = {{m, k, n}, {n, k, m}};
-    const Grads plan = plan_grads(m, n, k, dtype);
     // w and x: taken as they are; g: too, where padding it costs more than dx' product loses by it (its rows' short
     // pieces then lie across the memory's lines: 1890 x 1470 x 11715 bf16 91 us padded, 107 as it is)
     constexpr int64_t group = GROUP<T>;
@@ -1257,12 +1313,13 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
       if (int rc = product_of(p[0], plan.plan[0], 0, z[0], {g, ldg, m}, {pw, lw, k}, over, dx_edge, to_dx, room)) return rc;
     if (dw)
       if (int rc = product_of(p[1], plan.plan[1], 1, z[1], {g, ldg, n}, {px, lx, k}, 0, dw_edge, to_dw, room)) return rc;
-    if (!plan.apart) return launch_grads<T>(plan.plan[0].shape, p, s);
+    const ColumnSums sums = {dy, db, ldy, m, n, db_beside ? (int)cdiv(n, 64) : 0};
+    if (!plan.apart) return launch_grads<T>(plan.plan[0].shape, p, sums, s);
     for (int i = 0; i < 2; ++i) {
       Product one[2] = {};
       one[i] = p[i];
       if (p[i].blocks > 0)
-        if (int rc = launch_grads<T>(plan.plan[i].shape, one, s)) return rc;
+        if (int rc = launch_grads<T>(plan.plan[i].shape, one, {}, s)) return rc;
     }
     return (int)QNN_OK;
   });
