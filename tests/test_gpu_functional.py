@@ -743,3 +743,78 @@ def test_nothing_is_written_past_the_outputs(F, dt, m, n, k):
     _lib.call("qnn_topk_distill_bwd", p(x), k, p(t), 5, p(i), 5, a["stats"], p(grad), 0, a["ds"], m, k, 5, 1.0, 1, code, 0, 8, st)
     for q, (buf, size) in outs.items():
         assert (buf[size:] == 0x5A).all(), q
+
+
+# ------------------------------------------------------------------------------------ past 32 bits
+def large(*shape, seed):
+    """bf16 on the device, over 2^31 elements."""
+    assert math.prod(shape) > 2 ** 31
+    return torch.empty(shape, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(seed))
+
+
+def test_linear_act_long_batch(F):
+    m, n, k = 131080, 40, 16392
+    x = large(m, k, seed=1).requires_grad_(True)
+    w = (torch.randn(n, k, generator=gen(2)) / math.sqrt(k)).bfloat16().cuda().requires_grad_(True)
+    dy = torch.randn(m, n, generator=gen(3)).bfloat16().cuda()
+    y = F.linear_act(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    with torch.no_grad():
+        for at in (slice(0, 40), slice(m - 40, m)):
+            want = O.linear_act(x[at].cpu(), w.cpu(), None, None, "none", dy[at].cpu())
+            near(y[at], want["y"], "y")
+            near(dx[at], want["dx"], "dx")
+        value, size = 0.0, 0.0
+        for i in range(0, m, 8192):
+            a, b = dy[i:i + 8192].t().double(), x[i:i + 8192].double()
+            value, size = value + a @ b, size + a.abs() @ b.abs()
+        near(dw, O._out(value, (m + 1) * O.E * size, torch.bfloat16), "dw")
+
+
+@pytest.mark.parametrize("m", [1, 2, 20])
+def test_linear_act_large_weight(F, m):
+    n, k = 36000, 60000
+    x = torch.randn(m, k, generator=gen(4)).bfloat16().cuda().requires_grad_(True)
+    w = large(n, k, seed=5).requires_grad_(True)
+    dy = torch.randn(m, n, generator=gen(6)).bfloat16().cuda()
+    y = F.linear_act(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    with torch.no_grad():
+        for at in (slice(0, 40), slice(n - 40, n)):
+            want = O.linear_act(x.cpu(), w[at].cpu(), None, None, "none", dy[:, at].cpu())
+            near(y[:, at], want["y"], "y")
+            near(dw[at], want["dw"], "dw")
+        value, size = 0.0, 0.0
+        for i in range(0, n, 4096):
+            a, b = dy[:, i:i + 4096].double(), w[i:i + 4096].double()
+            value, size = value + a @ b, size + a.abs() @ b.abs()
+        near(dx, O._out(value, (n + 1) * O.E * size, torch.bfloat16), "dx")
+
+
+def test_layer_norm_long_batch(F):
+    rows, dim = 262200, 8192
+    x = large(rows, dim, seed=7).requires_grad_(True)
+    w, b = (torch.randn(dim, generator=gen(s)).cuda().requires_grad_(True) for s in (8, 9))
+    dy = large(rows, dim, seed=10)
+    y = F.layer_norm(x, w, b)
+    dx, = torch.autograd.grad(y, x, dy)
+    with torch.no_grad():
+        for at in (slice(0, 20), slice(rows - 20, rows)):
+            want = O.layer_norm(x[at].cpu(), w.cpu(), b.cpu(), 1e-5, dy[at].cpu())
+            near(y[at], want["y"], "y")
+            near(dx[at], want["dx"], "dx")
+
+
+def test_topk_distill_long_batch(F):
+    rows, vocab, top = 16400, 131072, 16
+    s = large(rows, vocab, seed=11).requires_grad_(True)
+    g = gen(12)
+    t, i = torch.randn(rows, top, generator=g), torch.randint(0, vocab, (rows, top), generator=g)
+    loss = F.topk_distill_loss(s, t.cuda(), i.cuda(), 2.0, "none")
+    grad = torch.randn(rows, generator=g)
+    ds, = torch.autograd.grad(loss, s, grad.cuda())
+    with torch.no_grad():
+        for at in (slice(0, 4), slice(rows - 4, rows)):
+            want = O.topk_distill(s[at].cpu(), t[at], i[at], 2.0, "none", grad[at])
+            near(loss[at], want["loss"], "loss")
+            near(ds[at], want["ds"], "ds")
