@@ -478,8 +478,9 @@ int qnn_linear_act_fwd_work(int64_t m, int64_t n, int64_t k, int dtype, int64_t*
 int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res,
                        int64_t ldr, void* y, void* slope, int64_t m, int64_t n, int64_t k, int dtype, int act,
                        void* work, int64_t work_bytes, qnn_stream_t stream);
-/* Introspection: the output tile that the forward product (grads == 0) or the two of the backward pass use,
- * and the splits of their reductions (splits[0], and for the backward pass dx's and dw's in turn). */
+/* Introspection: the output tile that the forward product (grads == 0) or dx's of the backward pass uses, of
+ * operands without gaps, and the splits of the reductions (splits[0], and for the backward pass dx's and dw's in
+ * turn). */
 int qnn_linear_act_plan(int64_t m, int64_t n, int64_t k, int dtype, int grads, int* tile_m, int* tile_n, int* splits);
 /* dz = dy * act'(z); dx[m][k] = dz w; dw[n][k] = dz^T x; db[n] = sum over m of dz; each of dx, dw, db is
  * nullable.  dz [m][n] (it is the residual's gradient too): required unless act is QNN_ACT_NONE, for
