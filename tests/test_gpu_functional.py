@@ -2,6 +2,7 @@
 sizes, strides and values where such kernels go wrong.  Every tolerance is the oracle's bound."""
 import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -690,8 +691,41 @@ def test_two_captured_training_steps(F):
                 assert torch.equal(p, q)
 
 
+def test_threads_at_once(F):
+    """Four threads on streams of their own, two sizes: what one alone gets."""
+    cases = []
+    for m, n, k in ((300, 500, 1000), (128, 1000, 512)):
+        x, w, b, r, dy = dev(*linear_case(m, n, k, torch.bfloat16, True, False))
+        t, i = torch.randn(m, 5, generator=gen(m)).cuda(), torch.randint(0, n, (m, 5), generator=gen(n)).cuda()
+        cases.append((x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True), t, i))
+
+    def step(x, w, b, t, i):
+        y = F.linear_act(F.layer_norm(x), w, b, activation="gelu")
+        return torch.autograd.grad(F.topk_distill_loss(y, t, i, 2.0), (x, w, b))
+
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def run(at):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[at] = step(*cases[at % 2])
+        stream.synchronize()
+
+    threads = [threading.Thread(target=run, args=(at,)) for at in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for at in range(4):
+        for p, q in zip(got[at], want[at % 2]):
+            assert torch.equal(p, q)
+
+
 @pytest.mark.parametrize("dt", TYPES, ids=IDS)
-@pytest.mark.parametrize("m,n,k", [(1, 33, 70), (5, 40, 64), (130, 67, 96), (70, 200, 130)])
+@pytest.mark.parametrize("m,n,k", [(1, 33, 70), (5, 40, 64), (130, 67, 96), (70, 200, 130), (34, 66, 98), (150, 1002, 514), (20, 6, 10)])
 def test_nothing_is_written_past_the_outputs(F, dt, m, n, k):
     """The C entries on buffers with a guard behind each output and behind the workspace."""
     from qnn import _lib
