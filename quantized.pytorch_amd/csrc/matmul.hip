@@ -121,12 +121,19 @@ struct Operand {
 };
 
 // R rows of an operand in a workgroup of W waves: its loads into LDS and its fragments from there.
-template <class T, bool DENSE, int R, int W>
+// SEG: of rows that begin at any 16 bytes (c chunks past a 64-byte boundary), a stage's slot holds what lies
+// between two such boundaries: chunk q of the stage is in that slot or, past its end, in the next one.  A load
+// of 64 bytes across a boundary takes the memory pipe twice as long: 1336 x 2072 x 3496 fp16 47 -> 37 us,
+// 6680 x 1256 x 5136 bf16 128 -> 107, 5556 x 9264 x 2896 328 -> 294.
+template <class T, bool DENSE, int R, int W, bool SEG = false>
 struct Side {
   static constexpr int ES = (int)sizeof(T), KE = 64 / ES, BYTES = R * 64, LOADS = R / 16 / W;
   static_assert(R % (16 * W) == 0, "a wave loads whole KiB");
   static constexpr int GRAN = 16 * ES, GMASK = R / 16 < 8 ? R / 16 - 1 : 7;  // bytes, and the XOR's bits
 
+  static __device__ __forceinline__ int past(const Operand& o, int64_t row) {
+    return SEG ? (int)((uintptr_t)((const T*)o.p + row * o.ld) >> 4 & 3) : 0;
+  }
   static __device__ __forceinline__ int turn(int row) { return -(row >> 2) & 3; }  // of a chunk's index, DENSE
   static __device__ __forceinline__ int spread(int k) {  // what a granule's index is XORed with, not DENSE
     if constexpr (ES == 2) return ((k & 3) | (k >> 3 & 1) << 2) & GMASK;
@@ -141,7 +148,7 @@ struct Side {
   // from row i0 and element k0 on
   __device__ __forceinline__ void begin(const Operand& o, int64_t i0, int64_t k0, int wave, int lane) {
     if constexpr (DENSE) {
-      base = (const char*)o.p + (i0 * o.ld + k0) * ES;
+      base = (const char*)o.p + (i0 * o.ld + k0) * ES - (SEG ? 64 : 0);
       step = 64;
     } else {
       base = (const char*)o.p + (k0 * o.ld + i0) * ES;
@@ -151,9 +158,9 @@ struct Side {
     for (int j = 0; j < LOADS; ++j) {
       const int at = (wave * LOADS + j) * 1024 + lane * 16;
       if constexpr (DENSE) {
-        const int row = at / 64, chunk = at / 16 % 4 ^ turn(row);
+        const int row = at / 64, chunk = (at / 16 % 4 ^ turn(row)) - past(o, i0 + row);
         kat[j] = chunk * 16 / ES;
-        off[j] = i0 + row < o.rows ? (uint32_t)(row * (int)o.ld * ES + chunk * 16) : PAST;
+        off[j] = i0 + row < o.rows ? (uint32_t)(row * (int)o.ld * ES + chunk * 16 + (SEG ? 64 : 0)) : PAST;
       } else {
         const int k = at / (R * ES), in = at % (R * ES);
         const int col = ((in / GRAN ^ spread(k)) * GRAN + in % GRAN) / ES;
@@ -163,18 +170,19 @@ struct Side {
     }
   }
   // load j of the next stage, of which `left` elements of k are there, into the slot at lds
-  __device__ __forceinline__ void load(char* lds, int j, int left, int wave) const {
+  // (first: the one in which k begins, where SEG has chunks before it)
+  __device__ __forceinline__ void load(char* lds, int j, int left, int wave, bool first) const {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass drops a kernel that names the resource type, without a word
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_t)(lds + (wave * LOADS + j) * 1024), 16,
-                                             kat[j] < left ? off[j] : PAST, 0, 0, 0);
+                                             kat[j] < left && !(SEG && first && kat[j] < 0) ? off[j] : PAST, 0, 0, 0);
 #endif
   }
   // fragment f (rows 16 f ... of the wave's, which begin at row r0)
-  static __device__ __forceinline__ int place(int r0, int lane) {
+  static __device__ __forceinline__ int place(int r0, int lane, int c) {
     if constexpr (DENSE) {
       const int row = lane & 15;
-      return (r0 + row) * 64 + ((lane >> 4) ^ turn(row)) * 16;
+      return (r0 + row) * 64 + ((((lane >> 4) + c) & 3) ^ turn(row)) * 16;
     } else if constexpr (ES == 2) {
       return ((lane >> 4) * 8 + (lane >> 2 & 3)) * R * ES + (lane & 3) * 8;
     } else {
@@ -325,10 +333,10 @@ __device__ __forceinline__ void emit(const Product& t, const f4 (&acc)[C::TM][C:
 }
 
 // Workgroup `id` of the product's.
-template <class T, bool AD, bool BD, class C>
+template <class T, bool AD, bool BD, class C, bool SEG>
 __device__ __forceinline__ void tile(const Product& t, int id) {
-  using A = Side<T, AD, C::BM, C::W>;
-  using B = Side<T, BD, C::BN, C::W>;
+  using A = Side<T, AD, C::BM, C::W, SEG && AD>;
+  using B = Side<T, BD, C::BN, C::W, SEG && BD>;
   constexpr int TM = C::TM, TN = C::TN, KE = A::KE, P = A::LOADS + B::LOADS;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -346,37 +354,40 @@ __device__ __forceinline__ void tile(const Product& t, int id) {
   B sb;
   sa.begin(t.a, i0, k0, wave, lane);
   sb.begin(t.b, j0, k0, wave, lane);
-  auto load = [&](int slot, int j) {  // load j of P of the next stage
-    if (j < A::LOADS) sa.load(lds + slot * C::SLOT, j, left, wave);
-    else sb.load(lds + slot * C::SLOT + A::BYTES, j - A::LOADS, left, wave);
+  auto load = [&](int slot, int j, bool first = false) {  // load j of P of the next stage
+    if (j < A::LOADS) sa.load(lds + slot * C::SLOT, j, left, wave, first);
+    else sb.load(lds + slot * C::SLOT + A::BYTES, j - A::LOADS, left, wave, first);
     if (j == P - 1) {
       sa.base += sa.step;
       sb.base += sb.step;
       left -= KE;
     }
   };
-  const int pa = A::place(ri, lane), pb = B::place(rj, lane);
+  // the same for all of a lane's rows, which are 16 apart
+  const int ca = A::past(t.a, i0 + (lane & 15)), cb = B::past(t.b, j0 + (lane & 15));
+  const int pa = A::place(ri, lane, ca), pb = B::place(rj, lane, cb);
+  const bool na = (lane >> 4) + ca > 3, nb = (lane >> 4) + cb > 3;  // in the next slot
   f4 fa[2][TM], fb[2][TN], acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-  auto fetch = [&](int slot, int to, int f) {  // fragment f of TN + TM
-    char* s = lds + slot * C::SLOT;
-    if (f < TN) fb[to][f] = B::fragment(s + A::BYTES, pb, rj, f, lane);
-    else fa[to][f - TN] = A::fragment(s, pa, ri, f - TN, lane);
+  auto fetch = [&](int s, int to, int f) {  // fragment f of TN + TM of stage s
+    const int here = (s & 3) * C::SLOT, next = ((s + 1) & 3) * C::SLOT;
+    if (f < TN) fb[to][f] = B::fragment(lds + (SEG && BD && nb ? next : here) + A::BYTES, pb, rj, f, lane);
+    else fa[to][f - TN] = A::fragment(lds + (SEG && AD && na ? next : here), pa, ri, f - TN, lane);
   };
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int j = 0; j < P; ++j) load(s, j);
-  meet<3 * P>();
+    for (int j = 0; j < P; ++j) load(s, j, s == 0 && k0 == 0);
+  meet<(SEG ? 2 : 3) * P>();
 #pragma unroll
   for (int f = 0; f < TM + TN; ++f) fetch(0, 0, f);
   // step s: stage s is in registers, s + 1 to s + 3 in LDS or on their way
   auto step = [&](int s, auto cur) {
     constexpr int C0 = decltype(cur)::value;
-    meet<2 * P>();  // stage s + 1 has landed, and stage s has left its slot
+    meet<(SEG ? 1 : 2) * P>();  // stage s + 1 has landed (SEG: s + 2), and stage s has left its slot
     // rows of MFMAs with the loads of stage s + 4 and the reads of stage s + 1 between them, in this
     // order: left to itself the compiler puts the reads last, where the next step waits for them
     constexpr int BUSY = TM > 2 ? TM - 2 : 1, READS = (TM + TN + BUSY - 1) / BUSY, LOADS = (P + BUSY - 1) / BUSY;
@@ -385,7 +396,7 @@ __device__ __forceinline__ void tile(const Product& t, int id) {
 #pragma unroll
       for (int j = i * LOADS; j < (i + 1) * LOADS && j < P; ++j) load(s & 3, j);
 #pragma unroll
-      for (int f = i * READS; f < (i + 1) * READS && f < TM + TN; ++f) fetch((s + 1) & 3, C0 ^ 1, f);
+      for (int f = i * READS; f < (i + 1) * READS && f < TM + TN; ++f) fetch(s + 1, C0 ^ 1, f);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -500,7 +511,7 @@ __device__ __forceinline__ void loose_tile(const Product& t, int id) {
       *reinterpret_cast<uint4*>(lds + (s & 3) * C::SLOT + to[j]) = w;
     }
   };
-  const int pa = A::place(ri, lane), pb = B::place(rj, lane);
+  const int pa = A::place(ri, lane, 0), pb = B::place(rj, lane, 0);
   f4 fa[2][TM], fb[2][TN], acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -547,9 +558,9 @@ __device__ __forceinline__ void loose_tile(const Product& t, int id) {
   emit<T, C>(t, acc, lds, split, i0, j0, ri, rj, wave, lane);
 }
 
-template <class T, class C>
+template <class T, class C, bool SEG>
 __global__ __launch_bounds__(C::NT, C::EU) void linear_y_kernel(Product y) {
-  tile<T, true, true, C>(y, blockIdx.x);
+  tile<T, true, true, C, SEG>(y, blockIdx.x);
 }
 
 template <class T, class C>
@@ -601,7 +612,7 @@ __device__ __forceinline__ void column_sums(const ColumnSums& t, int id) {
 // dx = dz w and dw = dz^T x in one launch, so that the one's last tiles and the other's first share the
 // chip.  The first's workgroups are counted up to a multiple of 8, which keeps the second's on the XCDs
 // that tile_of takes them to be on; a product with no workgroups is not wanted.
-template <class T, class C>
+template <class T, class C, bool SEG>
 __global__ __launch_bounds__(C::NT, C::EU) void linear_grads_kernel(Product dx, Product dw, int dw_first,
                                                                     ColumnSums db) {
   if (const int rest = (int)gridDim.x - db.blocks; (int)blockIdx.x >= rest) {
@@ -612,8 +623,8 @@ __global__ __launch_bounds__(C::NT, C::EU) void linear_grads_kernel(Product dx, 
   const bool is_dw = (id < lead) == (dw_first != 0);
   const int at = id < lead ? id : id - lead;
   if (at >= (is_dw ? dw.blocks : dx.blocks)) return;
-  if (is_dw) tile<T, false, false, C>(dw, at);
-  else tile<T, true, false, C>(dx, at);
+  if (is_dw) tile<T, false, false, C, false>(dw, at);
+  else tile<T, true, false, C, SEG>(dx, at);
 }
 
 // The splits' sums of up to two products, in their order, through the epilogue: 8 columns a thread.
@@ -830,13 +841,14 @@ struct Shape {
   int bm, bn;
   float stage16, stage32, ends;
   float alone;   // what one by itself on a CU takes of its stage's time (16 bits, and Low)
-  float across;  // what each takes where the first operand's rows, DENSE, lie across 64-byte boundaries (16 bits)
+  // what each takes where the first operand's rows, DENSE, begin off 64-byte boundaries (16 bits): at 16 bytes, elsewhere
+  float off16, off;
 };
-constexpr Shape SHAPES[] = {{Big::BM, Big::BN, 0.72f, 0.0f, 10.0f, 1.0f, 1.0f},
-                            {Middle::BM, Middle::BN, 0.26f, 0.97f, 5.0f, 1.0f, 1.4f},
-                            {Half::BM, Half::BN, 0.19f, 0.50f, 4.0f, 1.0f, 1.6f},
-                            {Small::BM, Small::BN, 0.105f, 0.25f, 4.0f, 1.2f, 1.5f},
-                            {Low::BM, Low::BN, 0.0f, 0.21f, 1.5f, 1.4f, 1.0f}};
+constexpr Shape SHAPES[] = {{Big::BM, Big::BN, 0.72f, 0.0f, 10.0f, 1.0f, 1.0f, 1.0f},
+                            {Middle::BM, Middle::BN, 0.26f, 0.97f, 5.0f, 1.0f, 1.15f, 1.4f},
+                            {Half::BM, Half::BN, 0.19f, 0.50f, 4.0f, 1.0f, 1.5f, 1.6f},
+                            {Small::BM, Small::BN, 0.105f, 0.25f, 4.0f, 1.2f, 1.5f, 1.5f},
+                            {Low::BM, Low::BN, 0.0f, 0.21f, 1.5f, 1.4f, 1.0f, 1.0f}};
 
 int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
@@ -869,7 +881,8 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0, bool dense = 
   for (int c = dtype == QNN_F32 && from == 0 ? 1 : from; c < (dtype == QNN_F32 ? 5 : 4); ++c) {
     const Shape& h = SHAPES[c];
     const float stage = dtype == QNN_F32 ? h.stage32 : h.stage16, alone = dtype == QNN_F32 && c < 4 ? 1.0f : h.alone;
-    const float across = dtype != QNN_F32 && dense && size[0].k % 32 != 0 ? h.across : 1.0f;
+    const bool on = dtype == QNN_F32 || !dense || size[0].k % 32 == 0;
+    const float off = on ? 1.0f : size[0].k % 8 == 0 ? h.off16 : h.off;
     int64_t tiles[2], stages[2];
     for (int i = 0; i < count; ++i) {
       tiles[i] = cdiv(size[i].m, h.bm) * cdiv(size[i].n, h.bn);
@@ -892,7 +905,7 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0, bool dense = 
         each[i] = cdiv(stages[i], s);
         n[i] = cdiv(stages[i], each[i]);
         blocks += tiles[i] * n[i];
-        const float time = (float)each[i] * (i == 0 ? across : 1.0f);
+        const float time = (float)each[i] * (i == 0 ? off : 1.0f);
         work += (float)(tiles[i] * n[i]) * time;
         longest = fmaxf(longest, time);
         shortest = fminf(shortest, time);
@@ -1015,15 +1028,34 @@ int join(const Product* p, int count, hipStream_t s) {
   return QNN_OK;
 }
 
+// Whether the rows of an operand DENSE in k are taken between 64-byte boundaries (Side's SEG).
+template <class T>
+bool in_segments(const Operand& o) {
+  const int64_t ld = o.ld * (int64_t)sizeof(T);
+  return sizeof(T) == 2 && (uintptr_t)o.p % 16 == 0 && ld % 16 == 0 && ((uintptr_t)o.p % 64 != 0 || ld % 64 != 0);
+}
+// (Not in Small tiles: they are where latency counts, and SEG has one stage less on its way: 1000 x 1000 x 1000
+// fp16 8.0 us in segments, 6.9 without, 24 x 12568 x 7368 bf16 49 and 34.)
+template <class T, class C, class F>
+int with_segments(bool seg, F&& f) {
+  if constexpr (sizeof(T) == 2 && !std::is_same_v<C, Small>)
+    if (seg) return f(std::true_type{});
+  return f(std::false_type{});
+}
+
 template <class T>
 int launch_y(int shape, const Product& y, hipStream_t s) {
+  const bool seg = y.tail == 0 && (in_segments<T>(y.a) || in_segments<T>(y.b));
   const int rc = with_cfg<T>(shape, [&](auto cfg) {
     using C = decltype(cfg);
-    static std::atomic<uint64_t> told{0};
-    if (int rc = allow_lds((const void*)&linear_y_kernel<T, C>, C::LDS, told)) return rc;
-    hipLaunchKernelGGL((linear_y_kernel<T, C>), dim3((unsigned)y.blocks), dim3(C::NT), C::LDS, s, y);
-    QNN_LAUNCH_CHECK("linear_y_kernel");
-    return (int)QNN_OK;
+    return with_segments<T, C>(seg, [&](auto in) {
+      constexpr bool SEG = decltype(in)::value;
+      static std::atomic<uint64_t> told{0};
+      if (int rc = allow_lds((const void*)&linear_y_kernel<T, C, SEG>, C::LDS, told)) return rc;
+      hipLaunchKernelGGL((linear_y_kernel<T, C, SEG>), dim3((unsigned)y.blocks), dim3(C::NT), C::LDS, s, y);
+      QNN_LAUNCH_CHECK("linear_y_kernel");
+      return (int)QNN_OK;
+    });
   });
   return rc ? rc : join<T>(&y, 1, s);
 }
@@ -1031,15 +1063,19 @@ int launch_y(int shape, const Product& y, hipStream_t s) {
 // p: dx, dw (no blocks: not wanted); the one whose workgroups take longer goes first
 template <class T>
 int launch_grads(int shape, const Product (&p)[2], const ColumnSums& db, hipStream_t s) {
+  const bool seg = p[0].blocks > 0 && p[0].tail == 0 && in_segments<T>(p[0].a);
+  const int first = p[1].blocks > 0 && (p[0].blocks == 0 || p[1].span > p[0].span) ? 1 : 0;
+  const unsigned blocks = (unsigned)up(p[first].blocks, 8) + (unsigned)p[1 - first].blocks + (unsigned)db.blocks;
   const int rc = with_cfg<T>(shape, [&](auto cfg) {
     using C = decltype(cfg);
-    static std::atomic<uint64_t> told{0};
-    if (int rc = allow_lds((const void*)&linear_grads_kernel<T, C>, C::LDS, told)) return rc;
-    const int first = p[1].blocks > 0 && (p[0].blocks == 0 || p[1].span > p[0].span) ? 1 : 0;
-    const unsigned blocks = (unsigned)up(p[first].blocks, 8) + (unsigned)p[1 - first].blocks + (unsigned)db.blocks;
-    hipLaunchKernelGGL((linear_grads_kernel<T, C>), dim3(blocks), dim3(C::NT), C::LDS, s, p[0], p[1], first, db);
-    QNN_LAUNCH_CHECK("linear_grads_kernel");
-    return (int)QNN_OK;
+    return with_segments<T, C>(seg, [&](auto in) {
+      constexpr bool SEG = decltype(in)::value;
+      static std::atomic<uint64_t> told{0};
+      if (int rc = allow_lds((const void*)&linear_grads_kernel<T, C, SEG>, C::LDS, told)) return rc;
+      hipLaunchKernelGGL((linear_grads_kernel<T, C, SEG>), dim3(blocks), dim3(C::NT), C::LDS, s, p[0], p[1], first, db);
+      QNN_LAUNCH_CHECK("linear_grads_kernel");
+      return (int)QNN_OK;
+    });
   });
   return rc ? rc : join<T>(p, 2, s);
 }

@@ -171,6 +171,27 @@ def test_linear_act_infinities_at_the_ends_of_rows(F, dt, m, n, k):
             near(v, want[q], f"{gap} {q}")
 
 
+@pytest.mark.parametrize("dt", TYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("m,n,k", [(1336, 700, 1000), (4090, 3900, 72), (300, 200, 4008), (410, 2720, 1016), (260, 300, 8), (140, 1000, 20024),
+                                   (2100, 2050, 1032)])
+def test_linear_act_rows_off_64_byte_boundaries(F, dt, m, n, k):
+    """Rows that begin at every 16 bytes between two such boundaries, by their stride and by their first one, with NaN
+    between them; products whole and split."""
+    def matrix(rows, cols, before, after, seed):
+        v = torch.full((rows, before + cols + after), math.nan, dtype=dt, device="cuda")
+        v[:, before:before + cols] = torch.randn(rows, cols, generator=gen(seed)).to(dt).cuda() / (1 if seed else math.sqrt(cols))
+        return v[:, before:before + cols]
+    for before, after in ((0, 0), (8, 8), (24, 64 - (24 + k) % 32), (16, 24)):
+        print(m, n, k, dt, before, plan(m, n, k, dt, False), plan(m, n, k, dt, True), flush=True)
+        x, w, dy = matrix(m, k, before, after, 1), matrix(n, k, after, before, 0), matrix(m, n, 8, 8, 2)
+        want = O.linear_act(x, w, None, None, "none", dy)
+        x.requires_grad_(True), w.requires_grad_(True)
+        y = F.linear_act(x, w)
+        near(y, want["y"], "y")
+        for q, v in zip(("dx", "dw"), torch.autograd.grad(y, (x, w), dy)):
+            near(v, want[q], q)
+
+
 def test_linear_act_low_tiles_are_taken(F):
     assert {plan(m, n, k, torch.float32, g)[0] for m, n, k in ((18, 1000, 1002), (20, 4096, 1000), (30, 10000, 2000), (510, 500, 512)) for g in (False, True)} >= {(32, 64)}
 
