@@ -21,16 +21,18 @@ __all__ = ["top_logits", "step"]
 
 def top_logits(teacher, images, top):
     """The `top` largest logits of each row of teacher(images) and their classes (int32), in eval mode
-    and without gradients; the teacher's mode is left as it was."""
+    and without gradients; the teacher and each of its modules are left in the mode that they were in."""
     if top < 1:
         raise ValueError(f"qnn: top_logits keeps at least one logit, got top={top}")
-    training = teacher.training
+    training = [(m, m.training) for m in teacher.modules()]
     teacher.eval()
     try:
         with torch.no_grad():
             values, classes = torch.topk(teacher(images), top, dim=-1)
     finally:
-        teacher.train(training)
+        teacher.train(training[0][1])
+        for m, mode in training:  # train() gives every module the teacher's own mode, frozen ones too
+            m.training = mode
     return values, classes.int()
 
 
