@@ -8,6 +8,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -61,10 +62,16 @@ void ok(int status, const char* entry) {
 bool is_float(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 int code_of(at::ScalarType t) { return t == at::kFloat ? QNN_F32 : t == at::kBFloat16 ? QNN_BF16 : QNN_F16; }
 
-Tensor tensor_of(py::handle h, const char* op, const char* name) {
+// The argument as a tensor.  What the kernels would lose without a word is refused: the tangent of a dual tensor
+// (of a `constant` it is dropped as its gradient is), and the call itself under torch.jit.trace, which would
+// record nothing but the empty output.
+Tensor tensor_of(py::handle h, const char* op, const char* name, bool constant = false) {
   TORCH_CHECK_TYPE(THPVariable_Check(h.ptr()), "qnn: ", op, " expects a tensor for ", name, ", got ",
                    Py_TYPE(h.ptr())->tp_name);
   Tensor t = THPVariable_Unpack(h.ptr());
+  TORCH_CHECK(constant || !t._fw_grad(/*level=*/0).defined(), "qnn: ", op, " has no forward-mode derivative (", name,
+              " is a dual tensor with a tangent)");
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), "qnn: ", op, " cannot be recorded by torch.jit.trace");
   TORCH_CHECK(t.is_cuda(), "qnn: ", op, " runs on the MI355X path only (ROCm device tensor required for ", name,
               ", got ", t.device(), ")");
   return t;
@@ -374,7 +381,7 @@ constexpr int64_t MAX_TOP = 1024;
 
 Tensor topk_distill_loss(py::handle hs, py::handle ht, py::handle hi, double temp, int64_t reduction) {
   constexpr const char* op = "topk_distill_loss";
-  const Tensor s = tensor_of(hs, op, "logits"), t = tensor_of(ht, op, "teacher_logits").detach(),
+  const Tensor s = tensor_of(hs, op, "logits"), t = tensor_of(ht, op, "teacher_logits", true).detach(),
                i = tensor_of(hi, op, "teacher_index");
   TORCH_CHECK_TYPE(is_float(s.scalar_type()) && is_float(t.scalar_type()),
                    "qnn: topk_distill_loss expects logits and teacher_logits of float32, bfloat16 or float16, got ",

@@ -14,7 +14,8 @@ on the current stream of their tensors' device and allocate their workspaces the
 they may be captured into a graph (`torch.cuda.graph`), each graph with workspaces of its own.  To
 capture a backward pass take `torch.autograd.grad` inside the capture and let no eager autograd graph
 of the same leaves live across it (torch ties a leaf's gradient to the stream that met it first).
-Results are the same from run to run.  Gradients of gradients are not offered.
+Results are the same from run to run.  Gradients of gradients and forward-mode derivatives are not
+offered: a dual tensor with a tangent raises `RuntimeError`, and so does a call under `torch.jit.trace`.
 
 The checks, allocations and autograd nodes are a CPython extension (`csrc/functional.cpp`, built beside
 the library), since the calls are short.

@@ -1,0 +1,43 @@
+"""qnn.functional on the device where autograd hands it more than plain tensors."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def F(gpu):
+    from qnn import functional
+    return functional
+
+
+def calls(F):
+    """Each operator with its differentiable arguments: (name, function of them, arguments)."""
+    x, w, v, b, r = (torch.randn(*s, device="cuda") for s in ((2, 4), (3, 4), (4,), (3,), (2, 3)))
+    i = torch.zeros(2, 4, dtype=torch.long, device="cuda")
+    return (("linear_act", lambda *a: F.linear_act(*a), [x, w, b, r]), ("layer_norm", lambda *a: F.layer_norm(*a), [x, v, v.clone()]),
+            ("topk_distill_loss", lambda s: F.topk_distill_loss(s, x, i), [x]))
+
+
+def test_tangents_and_traces_are_refused(F):
+    for name, f, args in calls(F):
+        want = f(*args)
+        with forward_ad.dual_level():
+            for at, a in enumerate(args):
+                dual = forward_ad.make_dual(a, torch.ones_like(a))
+                with pytest.raises(RuntimeError, match=f"{name} has no forward-mode derivative"):
+                    f(*args[:at], dual, *args[at + 1:])
+            assert torch.equal(f(*args), want)
+        with pytest.raises(RuntimeError, match=f"{name} cannot be recorded"):
+            torch.jit.trace(f, tuple(args))
+        assert torch.equal(f(*args), want)
+
+
+def test_a_dual_teacher_is_a_constant(F):
+    """As one that requires a gradient is."""
+    s, t, i = torch.randn(2, 9, device="cuda"), torch.randn(2, 4, device="cuda"), torch.arange(8, device="cuda").view(2, 4)
+    want = F.topk_distill_loss(s, t, i)
+    with forward_ad.dual_level():
+        got = F.topk_distill_loss(s, forward_ad.make_dual(t, torch.ones_like(t)), i)
+        assert torch.equal(got, want) and forward_ad.unpack_dual(got).tangent is None
