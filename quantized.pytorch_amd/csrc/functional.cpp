@@ -86,7 +86,8 @@ void same_device(const Tensor& t, const Tensor& first, const char* op, const cha
 }
 
 // t as a matrix of dense rows along its last dimension: itself, a view or a copy.  For the products rows
-// also begin on 16-byte boundaries (or follow one another without a gap), strides within LONGEST.
+// also begin on 16-byte boundaries (or follow one another without a gap), strides within LONGEST.  A lazily negated
+// view (of a conjugate's imaginary part) is copied: what lies in memory is not its value.
 constexpr int64_t LONGEST = 1 << 21;  // of a row stride that the products take
 struct Rows {
   Tensor t;
@@ -98,7 +99,7 @@ Rows rows_of(const Tensor& given, bool products = false) {
   int64_t ld = t.size(0) <= 1 ? n : t.stride(0);
   const bool fits = !products || (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && ld <= LONGEST &&
                                   (ld * t.element_size() % 16 == 0 || ld == n));
-  if ((t.stride(1) != 1 && n > 1) || ld < n || !fits) {
+  if ((t.stride(1) != 1 && n > 1) || ld < n || !fits || t.is_neg()) {
     t = t.clone(at::MemoryFormat::Contiguous);
     ld = n;
   }
@@ -106,7 +107,7 @@ Rows rows_of(const Tensor& given, bool products = false) {
 }
 Tensor vector_of(const OptTensor& t) {
   if (!t) return Tensor();
-  return t->is_contiguous() ? *t : t->contiguous();
+  return t->is_contiguous() && !t->is_neg() ? *t : t->clone(at::MemoryFormat::Contiguous);
 }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -365,7 +366,7 @@ struct TopKDistill : torch::autograd::Function<TopKDistill> {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(saved[0].device());
       const Rows s2 = rows_of(saved[0]), t2 = rows_of(saved[1]), i2 = rows_of(saved[2]);
-      const Tensor g = grads[0].contiguous();
+      const Tensor g = grads[0].contiguous().resolve_neg();
       out[0] = at::empty(ctx->saved_data["s"].toIntVector(), saved[0].options().requires_grad(false));
       ok(api.topk_distill_bwd(ptr(s2.t), s2.ld, ptr(t2.t), t2.ld, ptr(i2.t), i2.ld, saved[3].data_ptr<float>(),
                               g.data_ptr<float>(), reduction == NONE, ptr(out[0]), s2.t.size(0), s2.t.size(1),

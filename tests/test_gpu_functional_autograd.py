@@ -41,3 +41,25 @@ def test_a_dual_teacher_is_a_constant(F):
     with forward_ad.dual_level():
         got = F.topk_distill_loss(s, forward_ad.make_dual(t, torch.ones_like(t)), i)
         assert torch.equal(got, want) and forward_ad.unpack_dual(got).tangent is None
+
+
+def test_negated_views(F):
+    """A view with torch's negative bit (the imaginary part of a conjugate) gives what its values do, forward and backward:
+    the kernels took what lies in memory."""
+    negated = torch._neg_view
+    cases = calls(F) + (("one feature", lambda x, w: F.linear_act(x, w), [torch.randn(3, 1, device="cuda"), torch.randn(2, 1, device="cuda")]),
+                        ("rows of losses", lambda s: F.topk_distill_loss(s, s.detach(), torch.zeros_like(s, dtype=torch.int32), reduction="none"),
+                         [torch.randn(5, 6, device="cuda")]))
+    for name, f, args in cases:
+        plain = [(-a).requires_grad_(True) for a in args]
+        views = [negated(a.clone()).requires_grad_(True) for a in args]
+        assert all(v.is_neg() and torch.equal(v, p) for v, p in zip(views, plain))
+        with torch.no_grad():
+            assert torch.equal(f(*views), f(*plain)), name
+        y, want = f(*views), f(*plain)
+        assert torch.equal(y, want), name
+        dy = torch.randn_like(want)
+        for p, q in zip(torch.autograd.grad(y, views, negated(-dy)), torch.autograd.grad(want, plain, dy)):
+            assert torch.equal(p, q), name
+    part = torch.randn(4, 6, dtype=torch.cfloat, device="cuda").conj().imag
+    assert part.is_neg() and torch.equal(F.layer_norm(part), F.layer_norm(part.resolve_neg()))
