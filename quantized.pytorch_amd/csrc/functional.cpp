@@ -120,11 +120,19 @@ qnn_stream_t stream_of(const Tensor& t) {
 bool wants(const Tensor& t) { return t.requires_grad(); }
 bool wants(const OptTensor& t) { return t && t->requires_grad(); }
 
-// Gradients of gradients are not offered: under create_graph the gradients carry a node that says so.
-variable_list once(const variable_list& given, variable_list grads, const char* op) {
+// Gradients of gradients are not offered: under create_graph, gradients carry a node that says so where the gradient
+// that came in is asked for one.  Where it is not they are constants, and a warning says what is missing of them if
+// they depend (`depend`) on inputs that do require a gradient.
+variable_list once(const variable_list& given, variable_list grads, const char* op, bool depend) {
+  if (!at::GradMode::is_enabled()) return grads;
   bool any = false;
   for (const auto& g : given) any = any || (g.defined() && g.requires_grad());
-  if (!at::GradMode::is_enabled() || !any) return grads;
+  if (!any) {
+    if (depend)
+      TORCH_WARN("qnn: gradients of ", op, "'s gradients are not offered: those made here under create_graph are "
+                 "constants, and what is computed from them sends nothing back to ", op, "'s inputs");
+    return grads;
+  }
   for (auto& g : grads)
     if (g.defined()) g = g.detach().requires_grad_(true);
   return (*std::make_shared<torch::autograd::DelayedError>(
@@ -204,7 +212,8 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
       }
       if (need_r) out[3] = act != QNN_ACT_NONE ? dz : dy;
     }
-    return once(grads, std::move(out), "linear_act");
+    // without GELU the gradients are products of dy with the other operand
+    return once(grads, std::move(out), "linear_act", act == QNN_ACT_GELU || (need_x && need_w));
   }
 };
 
@@ -288,7 +297,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                             ptr(out[1]), ptr(out[2]), rows, dim, code, wcode, ptr(work), bytes, stream_of(dy)),
          "qnn_layer_norm_bwd");
     }
-    return once(grads, std::move(out), "layer_norm");
+    return once(grads, std::move(out), "layer_norm", need_x);
   }
 };
 
@@ -374,7 +383,7 @@ struct TopKDistill : torch::autograd::Function<TopKDistill> {
                               code_of(t2.t.scalar_type()), (int)i2.t.element_size(), stream_of(s2.t)),
          "qnn_topk_distill_bwd");
     }
-    return once(grads, std::move(out), "topk_distill_loss");
+    return once(grads, std::move(out), "topk_distill_loss", true);
   }
 };
 

@@ -16,6 +16,8 @@ capture a backward pass take `torch.autograd.grad` inside the capture and let no
 of the same leaves live across it (torch ties a leaf's gradient to the stream that met it first).
 Results are the same from run to run.  Gradients of gradients and forward-mode derivatives are not
 offered: a dual tensor with a tangent raises `RuntimeError`, and so does a call under `torch.jit.trace`.
+Gradients made under `create_graph` raise it when they are differentiated further by way of the gradient
+that came in; if that does not require one they are constants, with a warning.
 
 The checks, allocations and autograd nodes are a CPython extension (`csrc/functional.cpp`, built beside
 the library), since the calls are short.

@@ -1,4 +1,6 @@
 """qnn.functional on the device where autograd hands it more than plain tensors."""
+import warnings
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -63,3 +65,26 @@ def test_negated_views(F):
             assert torch.equal(p, q), name
     part = torch.randn(4, 6, dtype=torch.cfloat, device="cuda").conj().imag
     assert part.is_neg() and torch.equal(F.layer_norm(part), F.layer_norm(part.resolve_neg()))
+
+
+def test_constant_gradients_under_create_graph_warn(F):
+    """A penalty on such a gradient sends nothing back, which was not said; where the gradient depends on nothing that
+    requires one, and without create_graph, there is nothing to say."""
+    def grad(y, *leaves, **kw):
+        with warnings.catch_warnings(record=True) as seen:
+            warnings.simplefilter("always")
+            got = torch.autograd.grad(y, leaves, torch.ones_like(y), **kw)
+        assert not any(g.requires_grad for g in got)
+        return [str(w.message) for w in seen if "create_graph" in str(w.message)]
+
+    for name, f, args in calls(F):
+        leaves = [a.clone().requires_grad_(True) for a in args]
+        said = grad(f(*leaves), *leaves, create_graph=True)
+        assert len(said) == 1 and name in said[0], said
+        assert not grad(f(*leaves), *leaves)
+    (_, _, (x, w, b, _)), (_, _, (_, v, _)), _ = calls(F)
+    leaf = lambda a: a.clone().requires_grad_(True)
+    for y, of in ((F.linear_act(leaf(x), w), 0), (F.linear_act(x, leaf(w), activation="relu"), 0), (F.linear_act(x, w, leaf(b)), 0),
+                  (F.layer_norm(x, leaf(v)), 0), (F.linear_act(x, leaf(w), activation="gelu"), 1), (F.layer_norm(leaf(x)), 1)):
+        node = y.grad_fn.next_functions
+        assert len(grad(y, *(n.variable for n, _ in node if n is not None), create_graph=True)) == of
