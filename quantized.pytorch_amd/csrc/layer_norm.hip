@@ -248,33 +248,136 @@ __global__ __launch_bounds__(S::NT) void layer_norm_bwd_kernel(const T* __restri
   }
 }
 
-// dw and db from `parts` partial rows: 64 columns a workgroup, 16 threads a column
+// A sum is at most 1024 additions deep at any size that fits the card: CHAIN of a lane's own terms one after another, the
+// rows of a workgroup, JOINED partial rows, and the sums of those.
+constexpr int CHAIN = 512, JOINED = 256;
+
+// dw and db from `parts` partial rows: 64 columns a workgroup at a time, 16 threads a column
 template <class W>
 __global__ __launch_bounds__(1024) void layer_norm_join_kernel(const float* __restrict__ part, int parts, int dim,
                                                                W* dw, W* db) {
   __shared__ float sh[16][64];
   const int lane = threadIdx.x & 63, k = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;  // over dw's columns, then db's
-  float s = 0.0f;
-  if (c < 2 * (int64_t)dim) {
+  for (int64_t c0 = (int64_t)blockIdx.x * 64; c0 < 2 * (int64_t)dim; c0 += (int64_t)gridDim.x * 64) {
+    const int64_t c = c0 + lane;  // over dw's columns, then db's
+    float s = 0.0f;
+    if (c < 2 * (int64_t)dim)
+      for (int p0 = k; p0 < parts; p0 += 16 * JOINED) {
+        const int p1 = p0 + 16 * JOINED < parts ? p0 + 16 * JOINED : parts;
+        float t = 0.0f;
 #pragma unroll 8
-    for (int p = k; p < parts; p += 16) s += part[(int64_t)p * 2 * dim + c];
-  }
-  sh[k][lane] = s;
-  __syncthreads();
-  if (k == 0 && c < 2 * (int64_t)dim) {
+        for (int p = p0; p < p1; p += 16) t += part[(int64_t)p * 2 * dim + c];
+        s += t;
+      }
+    sh[k][lane] = s;
+    __syncthreads();
+    if (k == 0 && c < 2 * (int64_t)dim) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) s += sh[i][lane];
-    if (c < dim) {
-      if (dw) dw[c] = (W)s;
-    } else if (db) {
-      db[c - dim] = (W)s;
+      for (int i = 1; i < 16; ++i) s += sh[i][lane];
+      if (c < dim) {
+        if (dw) dw[c] = (W)s;
+      } else if (db) {
+        db[c - dim] = (W)s;
+      }
     }
+    __syncthreads();
   }
 }
 
-// ---- rows too long for registers (or shorter than a group): a workgroup a row, read again (from L2) for each step
+// ---- rows shorter than a group: a row a thread
+constexpr int NARROW = 256;
+
+template <class T>
+__device__ __forceinline__ void load_narrow(float (&v)[GROUP<T>], const T* p, int dim) {
+#pragma unroll
+  for (int i = 0; i < GROUP<T>; ++i) v[i] = i < dim ? (float)p[i] : 0.0f;
+}
+
+template <class T, class W>
+__global__ __launch_bounds__(NARROW) void layer_norm_fwd_narrow_kernel(const T* x, int64_t ldx, const W* w, const W* b,
+                                                                       T* y, float* mean, float* rstd, int64_t rows,
+                                                                       int dim, float eps) {
+  constexpr int GR = GROUP<T>;
+  float wv[GR], bv[GR];
+#pragma unroll
+  for (int i = 0; i < GR; ++i) {
+    wv[i] = w && i < dim ? (float)w[i] : 1.0f;
+    bv[i] = b && i < dim ? (float)b[i] : 0.0f;
+  }
+  for (int64_t r = (int64_t)blockIdx.x * NARROW + threadIdx.x; r < rows; r += (int64_t)gridDim.x * NARROW) {
+    float v[GR], s = 0.0f, q = 0.0f;
+    load_narrow<T>(v, x + r * ldx, dim);
+#pragma unroll
+    for (int i = 0; i < GR; ++i) s += v[i];
+    const float mu = s / (float)dim;
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+      const float d = i < dim ? v[i] - mu : 0.0f;
+      q = fmaf(d, d, q);
+    }
+    const float rs = 1.0f / sqrtf(q / (float)dim + eps);
+#pragma unroll
+    for (int i = 0; i < GR; ++i)
+      if (i < dim) y[r * dim + i] = (T)fmaf((v[i] - mu) * rs, wv[i], bv[i]);
+    if (mean) mean[r] = mu;
+    if (rstd) rstd[r] = rs;
+  }
+}
+
+// dx, and this workgroup's sums of dw and db into part as in layer_norm_bwd_kernel (each null: not wanted)
+template <class T, class W>
+__global__ __launch_bounds__(NARROW) void layer_norm_bwd_narrow_kernel(const T* dy, int64_t ldy, const T* x,
+                                                                       int64_t ldx, const W* w, const float* mean,
+                                                                       const float* rstd, T* dx, float* part,
+                                                                       int64_t rows, int dim) {
+  constexpr int GR = GROUP<T>;
+  __shared__ float sh[NARROW / 64][2][GR];
+  float wv[GR], sum[2][GR] = {};
+#pragma unroll
+  for (int i = 0; i < GR; ++i) wv[i] = w && i < dim ? (float)w[i] : 1.0f;
+  for (int64_t r = (int64_t)blockIdx.x * NARROW + threadIdx.x; r < rows; r += (int64_t)gridDim.x * NARROW) {
+    float v[GR], d[GR], s = 0.0f, q = 0.0f;
+    load_narrow<T>(v, x + r * ldx, dim);
+    load_narrow<T>(d, dy + r * ldy, dim);
+    const float mu = mean[r], rs = rstd[r];
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+      v[i] = i < dim ? (v[i] - mu) * rs : 0.0f;
+      sum[0][i] = fmaf(d[i], v[i], sum[0][i]);
+      sum[1][i] += d[i];
+      d[i] *= wv[i];
+      s += d[i];
+      q = fmaf(d[i], v[i], q);
+    }
+    const float sg = s / (float)dim, sx = q / (float)dim;
+    if (dx)
+#pragma unroll
+      for (int i = 0; i < GR; ++i)
+        if (i < dim) dx[r * dim + i] = (T)(rs * (d[i] - sg - v[i] * sx));
+  }
+  if (!part) return;
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) sum[which][i] += __shfl_xor(sum[which][i], o, 64);
+      if ((threadIdx.x & 63) == 0) sh[threadIdx.x / 64][which][i] = sum[which][i];
+    }
+  __syncthreads();
+  const int which = threadIdx.x / GR, i = threadIdx.x % GR;
+  if (which < 2 && i < dim) {
+    float s = sh[0][which][i];
+#pragma unroll
+    for (int k = 1; k < NARROW / 64; ++k) s += sh[k][which][i];
+    part[((int64_t)blockIdx.x * 2 + which) * dim + i] = s;
+  }
+}
+
+// ---- rows too long for registers: a workgroup a row, read again (from L2) for each step
 constexpr int LONG = 1024;
+// columns over which a thread adds one after another: CHAIN of its own
+constexpr int64_t RUN = (int64_t)LONG * CHAIN;
 
 template <class T, class W>
 __global__ __launch_bounds__(LONG) void layer_norm_fwd_long_kernel(const T* x, int64_t ldx, const W* w, const W* b,
@@ -286,20 +389,30 @@ __global__ __launch_bounds__(LONG) void layer_norm_fwd_long_kernel(const T* x, i
   const T* xr = x + r * ldx;
   int turn = 0;
   float s[1] = {0.0f}, q[1] = {0.0f}, v[GR];
-  for (int64_t c = threadIdx.x * GR; c < dim; c += LONG * GR) {
-    load_n<T, GR>(v, xr + c, dim - c);
+  for (int64_t c0 = 0; c0 < dim; c0 += RUN) {
+    const int64_t end = c0 + RUN < dim ? c0 + RUN : dim;
+    float t = 0.0f;
+    for (int64_t c = c0 + threadIdx.x * GR; c < end; c += LONG * GR) {
+      load_n<T, GR>(v, xr + c, dim - c);
 #pragma unroll
-    for (int i = 0; i < GR; ++i) s[0] += v[i];
+      for (int i = 0; i < GR; ++i) t += v[i];
+    }
+    s[0] += t;
   }
   row_sums<LONG>(s, sh, turn);
   const float mu = s[0] / (float)dim;
-  for (int64_t c = threadIdx.x * GR; c < dim; c += LONG * GR) {
-    load_n<T, GR>(v, xr + c, dim - c);
+  for (int64_t c0 = 0; c0 < dim; c0 += RUN) {
+    const int64_t end = c0 + RUN < dim ? c0 + RUN : dim;
+    float t = 0.0f;
+    for (int64_t c = c0 + threadIdx.x * GR; c < end; c += LONG * GR) {
+      load_n<T, GR>(v, xr + c, dim - c);
 #pragma unroll
-    for (int i = 0; i < GR; ++i) {
-      const float d = c + i < dim ? v[i] - mu : 0.0f;
-      q[0] = fmaf(d, d, q[0]);
+      for (int i = 0; i < GR; ++i) {
+        const float d = c + i < dim ? v[i] - mu : 0.0f;
+        t = fmaf(d, d, t);
+      }
     }
+    q[0] += t;
   }
   row_sums<LONG>(q, sh, turn);
   const float rs = 1.0f / sqrtf(q[0] / (float)dim + eps);
@@ -338,13 +451,19 @@ __global__ __launch_bounds__(LONG) void layer_norm_dx_long_kernel(const T* dy, i
       if (w) g[i] *= wv[i];
     }
   };
-  for (int64_t c = threadIdx.x * GR; c < dim; c += LONG * GR) {
-    load(c);
+  for (int64_t c0 = 0; c0 < dim; c0 += RUN) {
+    const int64_t end = c0 + RUN < dim ? c0 + RUN : dim;
+    float t0 = 0.0f, t1 = 0.0f;
+    for (int64_t c = c0 + threadIdx.x * GR; c < end; c += LONG * GR) {
+      load(c);
 #pragma unroll
-    for (int i = 0; i < GR; ++i) {
-      s[0] += g[i];
-      s[1] = fmaf(g[i], v[i], s[1]);
+      for (int i = 0; i < GR; ++i) {
+        t0 += g[i];
+        t1 = fmaf(g[i], v[i], t1);
+      }
     }
+    s[0] += t0;
+    s[1] += t1;
   }
   row_sums<LONG>(s, sh, turn);
   const float sg = s[0] / (float)dim, sx = s[1] / (float)dim;
@@ -407,13 +526,23 @@ bool with_shape(int64_t dim, F&& f) {
   return true;
 }
 
-constexpr int MAX_PARTS = 512;  // partial rows of dw and db: two workgroups of 256 a CU
+// Partial rows of dw and db: two workgroups of 256 a CU, and as many as keep a lane's sums within CHAIN rows.
+constexpr int MAX_PARTS = 512;
 
-// workgroups of a launch over all rows
-template <class S>
-unsigned row_blocks(int64_t rows, int64_t most) {
-  const int64_t n = cdiv(rows, S::ROWS);
+// workgroups of a launch over all rows, `each` of them at a time in one
+unsigned row_blocks(int64_t rows, int64_t each, int64_t most) {
+  const int64_t n = cdiv(rows, each);
   return (unsigned)(n < most ? n : most);
+}
+int64_t row_parts(int64_t rows, int64_t each, int64_t most = MAX_PARTS) {
+  const int64_t chains = cdiv(rows, each * CHAIN);
+  return row_blocks(rows, each, chains > most ? chains : most);
+}
+template <class T>
+int64_t parts_of(int64_t rows, int64_t dim) {
+  int64_t parts = 0;
+  if (with_shape<T>(dim, [&](auto shape) { parts = row_parts(rows, decltype(shape)::ROWS); })) return parts;
+  return dim < GROUP<T> ? row_parts(rows, NARROW) : row_parts(rows, 1, 64);
 }
 
 int check(int64_t rows, int64_t dim, int64_t ld) {
@@ -423,8 +552,12 @@ int check(int64_t rows, int64_t dim, int64_t ld) {
   return QNN_OK;
 }
 
-int64_t work_bytes_of(int64_t rows, int64_t dim) {
-  return (rows < MAX_PARTS ? rows : MAX_PARTS) * 2 * dim * (int64_t)sizeof(float);
+// Rows too long for registers are a workgroup each, and a launch has fewer than 2^32 threads.
+template <class T>
+int check_long(int64_t rows, int64_t dim) {
+  QNN_REQUIRE(cdiv(dim, GROUP<T>) <= 4096 || rows < (1LL << 32) / LONG,
+              "too many rows for one call: under 2^22 of more than 4096 groups of 16 bytes");
+  return QNN_OK;
 }
 
 }  // namespace
@@ -445,12 +578,17 @@ int qnn_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b,
     using T = decltype(t);
     using W = decltype(tw);
     hipStream_t s = (hipStream_t)stream;
+    if (int rc = check_long<T>(rows, dim)) return rc;
     const bool held = with_shape<T>(dim, [&](auto shape) {
       using S = decltype(shape);
-      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, S>), dim3(row_blocks<S>(rows, S::NT > 256 ? 512 : 1024)), dim3(S::NT), 0, s,
-                         (const T*)x, ldx, (const W*)w, (const W*)b, (T*)y, mean, rstd, rows, (int)dim, eps);
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W, S>), dim3(row_blocks(rows, S::ROWS, S::NT > 256 ? 512 : 1024)),
+                         dim3(S::NT), 0, s, (const T*)x, ldx, (const W*)w, (const W*)b, (T*)y, mean, rstd, rows,
+                         (int)dim, eps);
     });
-    if (!held)
+    if (!held && dim < GROUP<T>)
+      hipLaunchKernelGGL((layer_norm_fwd_narrow_kernel<T, W>), dim3(row_blocks(rows, NARROW, 2048)), dim3(NARROW), 0, s,
+                         (const T*)x, ldx, (const W*)w, (const W*)b, (T*)y, mean, rstd, rows, (int)dim, eps);
+    else if (!held)
       hipLaunchKernelGGL((layer_norm_fwd_long_kernel<T, W>), dim3((unsigned)rows), dim3(LONG), 0, s, (const T*)x, ldx,
                          (const W*)w, (const W*)b, (T*)y, mean, rstd, dim, eps);
     QNN_LAUNCH_CHECK("qnn_layer_norm_fwd");
@@ -461,8 +599,10 @@ int qnn_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b,
 int qnn_layer_norm_bwd_work(int64_t rows, int64_t dim, int dtype, int64_t* bytes) {
   if (int rc = check(rows, dim, dim)) return rc;
   QNN_REQUIRE(bytes, "null pointer");
-  *bytes = work_bytes_of(rows, dim);
-  return QNN_OK;
+  return with_type(dtype, [&](auto t) {
+    *bytes = parts_of<decltype(t)>(rows, dim) * 2 * dim * (int64_t)sizeof(float);
+    return (int)QNN_OK;
+  });
 }
 
 int qnn_layer_norm_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* w, const float* mean,
@@ -472,33 +612,37 @@ int qnn_layer_norm_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, 
   if (int rc = check(rows, dim, ldy)) return rc;
   QNN_REQUIRE(rows == 0 || (dy && x && mean && rstd), "null pointer");
   const bool sums = dw || db;
-  QNN_REQUIRE(!sums || rows == 0 || (work && work_bytes >= work_bytes_of(rows, dim)),
-              "work: at least what qnn_layer_norm_bwd_work says");
   return with_types(dtype, wdtype, [&](auto t, auto tw) {
     using T = decltype(t);
     using W = decltype(tw);
     hipStream_t s = (hipStream_t)stream;
+    const int64_t parts = parts_of<T>(rows, dim);
+    QNN_REQUIRE(!sums || rows == 0 || (work && work_bytes >= parts * 2 * dim * (int64_t)sizeof(float)),
+                "work: at least what qnn_layer_norm_bwd_work says");
+    if (int rc = check_long<T>(rows, dim)) return rc;
     float* part = sums ? (float*)work : nullptr;
-    unsigned parts = 0;
     if (rows > 0 && (dx || sums)) {
       const bool held = with_shape<T>(dim, [&](auto shape) {
         using S = decltype(shape);
-        parts = row_blocks<S>(rows, MAX_PARTS);
-        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, S>), dim3(parts), dim3(S::NT), 0, s, (const T*)dy, ldy,
-                           (const T*)x, ldx, (const W*)w, mean, rstd, (T*)dx, part, rows, (int)dim);
+        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, W, S>), dim3((unsigned)parts), dim3(S::NT), 0, s, (const T*)dy,
+                           ldy, (const T*)x, ldx, (const W*)w, mean, rstd, (T*)dx, part, rows, (int)dim);
       });
-      if (!held && dx)
-        hipLaunchKernelGGL((layer_norm_dx_long_kernel<T, W>), dim3((unsigned)rows), dim3(LONG), 0, s, (const T*)dy,
-                           ldy, (const T*)x, ldx, (const W*)w, mean, rstd, (T*)dx, dim);
-      if (!held && sums) {
-        parts = (unsigned)(rows < 64 ? rows : 64);
-        hipLaunchKernelGGL((layer_norm_dw_long_kernel<T>), dim3((unsigned)cdiv(dim, 256 * GROUP<T>), parts), dim3(256),
-                           0, s, (const T*)dy, ldy, (const T*)x, ldx, mean, rstd, part, rows, dim);
+      if (!held && dim < GROUP<T>) {
+        hipLaunchKernelGGL((layer_norm_bwd_narrow_kernel<T, W>), dim3((unsigned)parts), dim3(NARROW), 0, s,
+                           (const T*)dy, ldy, (const T*)x, ldx, (const W*)w, mean, rstd, (T*)dx, part, rows, (int)dim);
+      } else if (!held) {
+        if (dx)
+          hipLaunchKernelGGL((layer_norm_dx_long_kernel<T, W>), dim3((unsigned)rows), dim3(LONG), 0, s, (const T*)dy,
+                             ldy, (const T*)x, ldx, (const W*)w, mean, rstd, (T*)dx, dim);
+        if (sums)
+          hipLaunchKernelGGL((layer_norm_dw_long_kernel<T>),
+                             dim3((unsigned)cdiv(dim, 256 * GROUP<T>), (unsigned)parts), dim3(256), 0, s,
+                             (const T*)dy, ldy, (const T*)x, ldx, mean, rstd, part, rows, dim);
       }
       QNN_LAUNCH_CHECK("qnn_layer_norm_bwd");
     }
     if (sums) {
-      hipLaunchKernelGGL((layer_norm_join_kernel<W>), dim3((unsigned)cdiv(2 * dim, 64)), dim3(1024), 0, s, part,
+      hipLaunchKernelGGL((layer_norm_join_kernel<W>), dim3(row_blocks(2 * dim, 64, 1 << 20)), dim3(1024), 0, s, part,
                          (int)parts, (int)dim, (W*)dw, (W*)db);
       QNN_LAUNCH_CHECK("qnn_layer_norm_bwd");
     }

@@ -1,0 +1,40 @@
+"""The sizes at which the float operators' launches end, at the C entries and without a device: what would need 2^32 threads
+or more is refused before anything is launched, and sums over many rows get the partial sums that keep them short."""
+import ctypes
+
+import pytest
+
+
+def call(name, *args):
+    from qnn import _lib
+    return getattr(_lib.load(), name)(*args), _lib.load().qnn_last_error()
+
+
+P = ctypes.c_void_p(4096)  # an address that no check reads
+SIZES = {0: 4, 1: 2, 2: 2}  # QNN_F32, QNN_BF16, QNN_F16
+
+
+@pytest.mark.parametrize("code", SIZES)
+def test_layer_norm_rows_longer_than_registers(code):
+    dim = 4096 * 16 // SIZES[code] + 1
+    for rows in (1 << 22, (1 << 31) - 1):
+        rc, msg = call("qnn_layer_norm_fwd", P, dim, None, None, P, None, None, rows, dim, 1e-5, code, code, None)
+        assert rc == 1 and b"too many rows" in msg
+        rc, msg = call("qnn_layer_norm_bwd", P, dim, P, dim, None, P, P, P, P, P, rows, dim, code, code, P, 1 << 62, None)
+        assert rc == 1 and b"too many rows" in msg
+
+
+@pytest.mark.parametrize("code", SIZES)
+@pytest.mark.parametrize("dim", [1, 3, 8, 16, 100, 1000, 8192, 70000])
+def test_layer_norm_partial_rows(code, dim):
+    """At least one for each 512 rows that a lane adds (256 rows side by side where a row is a thread's, 16 where 16 lanes
+    have it), few of them where rows are few, and never more than rows."""
+    n = ctypes.c_int64(-1)
+    group = 16 // SIZES[code]
+    side = 256 if dim < group else 16 if dim <= 16 * group else 4 if dim <= 128 * group else 1
+    for rows in (0, 1, 500, 100000, 1 << 22, (1 << 31) - 1):
+        assert call("qnn_layer_norm_bwd_work", rows, dim, code, ctypes.byref(n))[0] == 0
+        parts, rest = divmod(n.value, 8 * dim)
+        assert rest == 0 and rows <= 512 * side * parts and parts <= rows
+        assert parts <= max(512, -(-rows // (512 * side)))
+    assert call("qnn_layer_norm_bwd_work", 5, dim, 3, ctypes.byref(n))[0] == 1

@@ -1,0 +1,80 @@
+"""The float operators at sizes where launches, offsets and sums reach their limits: rows in the millions, rows of a few
+elements, rows of millions.  The definition is computed in float64 on the device."""
+import math
+
+import pytest
+import torch
+
+from oracle import float_oracle as O
+from test_gpu_functional import IDS, TYPES, gen, near
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def F(gpu):
+    from qnn import functional
+    return functional
+
+
+def normal(*shape, seed, dt=torch.float32):
+    return torch.randn(shape, generator=torch.Generator("cuda").manual_seed(seed), device="cuda").to(dt)
+
+
+# ------------------------------------------------------------------------------------ layer_norm
+def norm_check(F, x, w, b, dy, eps=1e-5):
+    want = O.layer_norm(x, w, b, eps, dy)
+    with torch.no_grad():
+        near(F.layer_norm(x, w, b, eps), want["y"], "y (no grad)")
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    y = F.layer_norm(*leaves, eps)
+    near(y, want["y"], "y")
+    for q, v in zip(("dx", "dw", "db"), torch.autograd.grad(y, leaves, dy)):
+        near(v, want[q], q)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("dim", range(1, 8))
+def test_layer_norm_rows_shorter_than_a_group(F, dt, dim):
+    """A row a thread: around a wave, a workgroup and a turn of the launch, with weights of either type and strided rows."""
+    for n, rows in enumerate((1, 63, 65, 255, 257, 131071, 131073, 600000)):
+        x, dy = normal(rows, dim, seed=n, dt=dt), normal(rows, dim, seed=n + 50, dt=dt)
+        for wt in {dt, torch.float32}:
+            norm_check(F, x.detach(), 1 + normal(dim, seed=7).to(wt) / 4, normal(dim, seed=8).to(wt), dy)
+    x, dy = (normal(700, dim + 3, seed=s, dt=dt)[::2, 1:1 + dim] for s in (3, 4))
+    norm_check(F, x.detach(), normal(dim, seed=7), normal(dim, seed=8), dy)
+    # one gradient alone
+    x, w = normal(300, dim, seed=1, dt=dt), normal(dim, seed=7, dt=dt)
+    want = O.layer_norm(x, w, w, 1e-5, dy[:300])
+    for at, q in enumerate(("dx", "dw", "db")):
+        leaves = [x.clone(), w.clone(), w.clone()]
+        leaf = leaves[at].requires_grad_(True)
+        near(torch.autograd.grad(F.layer_norm(*leaves), leaf, dy[:300])[0], want[q], q)
+
+
+@pytest.mark.parametrize("dt,dim", [(torch.bfloat16, 4), (torch.float16, 7), (torch.float32, 3)], ids=["bf16-4", "fp16-7", "fp32-3"])
+def test_layer_norm_millions_of_short_rows(F, dt, dim):
+    rows = 4_200_000
+    norm_check(F, normal(rows, dim, seed=1, dt=dt), 1 + normal(dim, seed=2) / 4, normal(dim, seed=3), normal(rows, dim, seed=4, dt=dt))
+
+
+@pytest.mark.parametrize("rows,dim", [(4_000_000, 3), (1 << 26, 4), (3_000_000, 520), (300_000_000, 4)])
+def test_layer_norm_sums_over_many_rows(F, rows, dim):
+    """dw and db of equal terms, where a long chain of fp32 additions drifts: the rows are all the same one."""
+    x = torch.arange(dim, device="cuda", dtype=torch.float32).expand(rows, dim).contiguous()
+    dy = torch.full((rows, dim), 1.1, device="cuda")
+    w, b = torch.ones(dim, device="cuda", requires_grad=True), torch.zeros(dim, device="cuda", requires_grad=True)
+    want = O.layer_norm(x[:1], w.detach(), b.detach(), 1e-5, dy[:1])
+    dw, db = torch.autograd.grad(F.layer_norm(x, w, b), (w, b), dy)
+    chain = (O.CHAIN + 2) * O.E
+    for q, got in (("dw", dw), ("db", db)):
+        value, err = want[q]
+        near(got, (rows * value, rows * (err + chain * value.abs())), q)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("rows,dim", [(2, 600_001), (1, (1 << 25) + 3)])
+def test_layer_norm_rows_of_millions(F, dt, rows, dim):
+    """Equal terms again, in y and dx: a large mean and a constant gradient."""
+    x = (3 + normal(rows, dim, seed=1)).to(dt)
+    norm_check(F, x, 1 + normal(dim, seed=2, dt=dt) / 4, normal(dim, seed=3, dt=dt), torch.full((rows, dim), 1.1, dtype=dt, device="cuda"))
