@@ -42,6 +42,12 @@ struct Entries {
     const int64_t at = r * ldi + e;
     return index_bytes == 8 ? ((const int64_t*)index)[at] : (int64_t)((const int32_t*)index)[at];
   }
+  Entries from(int64_t r) const {  // row r on
+    Entries e = *this;
+    e.t = (const char*)t + r * ldt * type_bytes(tdtype);
+    e.index = (const char*)index + r * ldi * index_bytes;
+    return e;
+  }
 };
 
 // A running (maximum, sum of e^((x - maximum) / T)); k = log2(e) / T.  While the maximum is -inf the
@@ -251,8 +257,9 @@ struct Grad {
 
 template <class T, int L>
 __global__ __launch_bounds__((Grad<T, L>::THREADS)) void distill_grad_kernel(const T* s, int64_t lds, Entries en,
-                                                                             const float* stats, const float* grad,
-                                                                             int grad_rows, T* ds, int64_t rows,
+                                                                             const float* stats, const float* count,
+                                                                             const float* grad, int grad_rows, T* ds,
+                                                                             int64_t rows,
                                                                              int64_t vocab, int pieces, float temp,
                                                                              int mean) {
   constexpr int GR = GROUP<T>, ROWS = Grad<T, L>::ROWS;
@@ -271,7 +278,7 @@ __global__ __launch_bounds__((Grad<T, L>::THREADS)) void distill_grad_kernel(con
     const float4 st = *reinterpret_cast<const float4*>(stats + 4 * r);
     m = st.x, inv = st.y, ti = st.w;
     g = temp * (grad_rows ? grad[r] : grad[0]);
-    if (mean) g /= fmaxf(stats[4 * rows], 1.0f);
+    if (mean) g /= fmaxf(count[0], 1.0f);
     if (lane < 64) {  // the row's first wave picks the entries of this piece, in their order
       int n = 0;
       for (int e0 = 0; e0 < en.top; e0 += 64) {
@@ -335,6 +342,9 @@ int splits_of(int64_t rows, int64_t vocab, int dtype) {
   return (int)(n > MAX_SPLITS ? MAX_SPLITS : n);
 }
 
+// Rows in a launch of `blocks` workgroups of `threads` for each `each` rows: a launch has fewer than 2^32 threads.
+int64_t slice_of(int64_t each, int64_t blocks, int threads) { return ((1LL << 32) - 1) / threads / blocks * each; }
+
 int check(const void* s, int64_t lds, const void* t, int64_t ldt, const void* index, int64_t ldi, int64_t rows,
           int64_t vocab, int64_t top, float temp, int tdtype, int index_bytes, const float* stats) {
   QNN_REQUIRE(rows >= 0 && rows < (1LL << 31), "rows: 0 to 2^31 - 1");
@@ -393,12 +403,18 @@ int qnn_topk_distill_fwd(const void* s, int64_t lds, const void* t, int64_t ldt,
         hipLaunchKernelGGL((distill_split_rows_kernel<T, false>), dim3((unsigned)cdiv(rows, NT / 64)), dim3(NT), 0, st,
                            (const T*)s, lds, en, rows, vocab, temp, splits, (const Run*)work, row_loss, stats, loss,
                            mean);
-    } else if (vocab * (int64_t)sizeof(T) <= WAVE_BYTES) {
-      hipLaunchKernelGGL((distill_rows_kernel<T, 64>), dim3((unsigned)cdiv(rows, NT / 64)), dim3(NT), 0, st,
-                         (const T*)s, lds, en, rows, vocab, temp, row_loss, stats);
     } else {
-      hipLaunchKernelGGL((distill_rows_kernel<T, WIDE>), dim3((unsigned)rows), dim3(WIDE), 0, st, (const T*)s, lds, en,
-                         rows, vocab, temp, row_loss, stats);
+      auto launch = [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value, THREADS = L > NT ? L : NT, ROWS = THREADS / L;
+        const int64_t slice = slice_of(ROWS, 1, THREADS);
+        for (int64_t r = 0; r < rows; r += slice) {
+          const int64_t n = rows - r < slice ? rows - r : slice;
+          hipLaunchKernelGGL((distill_rows_kernel<T, L>), dim3((unsigned)cdiv(n, ROWS)), dim3(THREADS), 0, st,
+                             (const T*)s + r * lds, lds, en.from(r), n, vocab, temp, row_loss + r, stats + 4 * r);
+        }
+      };
+      if (vocab * (int64_t)sizeof(T) <= WAVE_BYTES) launch(std::integral_constant<int, 64>{});
+      else launch(std::integral_constant<int, WIDE>{});
     }
     QNN_LAUNCH_CHECK("qnn_topk_distill_fwd");
     return (int)QNN_OK;
@@ -423,15 +439,16 @@ int qnn_topk_distill_bwd(const void* s, int64_t lds, const void* t, int64_t ldt,
     auto launch = [&](auto lanes) {
       constexpr int L = decltype(lanes)::value;
       using G = Grad<T, L>;
-      const int64_t pieces = cdiv(vocab, G::PIECE), blocks = cdiv(rows, G::ROWS) * pieces;
-      QNN_REQUIRE(blocks < (1LL << 31), "too many logits for one call");
-      hipLaunchKernelGGL((distill_grad_kernel<T, L>), dim3((unsigned)blocks), dim3(G::THREADS), 0, (hipStream_t)stream,
-                         (const T*)s, lds, en, stats, grad, grad_rows, (T*)ds, rows, vocab, (int)pieces, temp, mean);
-      return (int)QNN_OK;
+      const int64_t pieces = cdiv(vocab, G::PIECE), slice = slice_of(G::ROWS, pieces, G::THREADS);
+      for (int64_t r = 0; r < rows; r += slice) {
+        const int64_t n = rows - r < slice ? rows - r : slice;
+        hipLaunchKernelGGL((distill_grad_kernel<T, L>), dim3((unsigned)(cdiv(n, G::ROWS) * pieces)), dim3(G::THREADS), 0,
+                           (hipStream_t)stream, (const T*)s + r * lds, lds, en.from(r), stats + 4 * r, stats + 4 * rows,
+                           grad_rows ? grad + r : grad, grad_rows, (T*)ds + r * vocab, n, vocab, (int)pieces, temp, mean);
+      }
     };
-    const int rc = vocab * (int64_t)sizeof(T) <= WAVE_BYTES ? launch(std::integral_constant<int, 64>{})
-                                                            : launch(std::integral_constant<int, WIDE>{});
-    if (rc) return rc;
+    if (vocab * (int64_t)sizeof(T) <= WAVE_BYTES) launch(std::integral_constant<int, 64>{});
+    else launch(std::integral_constant<int, WIDE>{});
     QNN_LAUNCH_CHECK("qnn_topk_distill_bwd");
     return (int)QNN_OK;
   });

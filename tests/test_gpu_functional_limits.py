@@ -78,3 +78,29 @@ def test_layer_norm_rows_of_millions(F, dt, rows, dim):
     """Equal terms again, in y and dx: a large mean and a constant gradient."""
     x = (3 + normal(rows, dim, seed=1)).to(dt)
     norm_check(F, x, 1 + normal(dim, seed=2, dt=dt) / 4, normal(dim, seed=3, dt=dt), torch.full((rows, dim), 1.1, dtype=dt, device="cuda"))
+
+
+# ----------------------------------------------------------------------------- topk_distill_loss
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_topk_distill_more_rows_than_a_launch_holds(F, reduction):
+    """70 million rows of three classes: the rows around the launches' borders, and the mean."""
+    rows, vocab = 70_000_000, 3
+    s = normal(rows, vocab, seed=1, dt=torch.float16).requires_grad_(True)
+    t = normal(rows, 2, seed=2, dt=torch.bfloat16)
+    i = torch.randint(-1, vocab, (rows, 2), generator=torch.Generator("cuda").manual_seed(3), device="cuda", dtype=torch.int32)
+    loss = F.topk_distill_loss(s, t, i, 2.0, reduction)
+    grad = normal(rows, seed=4) if reduction == "none" else torch.ones((), device="cuda")
+    ds, = torch.autograd.grad(loss, s, grad)
+    counted = int((i >= 0).any(1).sum())
+    border = ((1 << 32) - 1) // 256 * 4
+    for at in (0, border - 300, border, rows - 300):
+        at = slice(at, at + 300)
+        part = grad[at] if reduction == "none" else torch.full((300,), 1 / counted)
+        want = O.topk_distill(s[at].detach().cpu(), t[at].cpu(), i[at].cpu(), 2.0, "none", part)
+        near(ds[at], (want["ds"][0], want["ds"][1] + 2 * O.E * want["ds"][0].abs()), "ds")
+        if reduction == "none":
+            near(loss[at], want["loss"], "loss")
+    if reduction == "mean":
+        with torch.no_grad():
+            each = F.topk_distill_loss(s, t, i, 2.0, "none").double()
+        assert abs(loss.item() - each.sum().item() / counted) <= 2 * O.E * each.abs().sum().item() / counted
