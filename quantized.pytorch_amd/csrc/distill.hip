@@ -57,42 +57,53 @@ struct Run {
 };
 __device__ __forceinline__ float from(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// This lane's run over s[lo, hi): groups (lo + lane GROUP), L GROUP apart, U of them in flight.
+__device__ __forceinline__ Run joined(Run a, Run b, float k) {
+  const float m = fmaxf(a.m, b.m), f = from(m);
+  return {m, a.s * __builtin_amdgcn_exp2f((a.m - f) * k) + b.s * __builtin_amdgcn_exp2f((b.m - f) * k)};
+}
+
+// This lane's run over s[lo, hi): groups (lo + lane GROUP), L GROUP apart, U of them in flight.  A sum of more than
+// CHAIN terms is the sum of such sums.
 template <class T, int L>
 __device__ __forceinline__ Run run_over(const T* s, int64_t lo, int64_t hi, int lane, float k) {
-  constexpr int GR = GROUP<T>, U = 4;
-  Run a = {-INFINITY, 0.0f};
-  auto add = [&](const float* v, int n) {
-    float m = a.m;
+  constexpr int GR = GROUP<T>, U = 4, CHAIN = 512;
+  Run all = {-INFINITY, 0.0f};
+  for (int64_t end; lo < hi; lo = end) {
+    end = hi - lo > (int64_t)CHAIN * L ? lo + (int64_t)CHAIN * L : hi;
+    Run a = {-INFINITY, 0.0f};
+    auto add = [&](const float* v, int n) {
+      float m = a.m;
 #pragma unroll
-    for (int i = 0; i < n; ++i) m = fmaxf(m, v[i]);
-    const float f = from(m);
-    float t = a.s * __builtin_amdgcn_exp2f((a.m - f) * k);
+      for (int i = 0; i < n; ++i) m = fmaxf(m, v[i]);
+      const float f = from(m);
+      float t = a.s * __builtin_amdgcn_exp2f((a.m - f) * k);
 #pragma unroll
-    for (int i = 0; i < n; ++i) t += __builtin_amdgcn_exp2f((v[i] - f) * k);
-    a = {m, t};
-  };
-  int64_t c = lo + lane * GR;
-  for (; c + (U - 1) * L * GR + GR <= hi; c += U * L * GR) {
-    Vec<T, GR> raw[U];
+      for (int i = 0; i < n; ++i) t += __builtin_amdgcn_exp2f((v[i] - f) * k);
+      a = {m, t};
+    };
+    int64_t c = lo + lane * GR;
+    for (; c + (U - 1) * L * GR + GR <= end; c += U * L * GR) {
+      Vec<T, GR> raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = load_group(s + c + u * L * GR, GR);
+      for (int u = 0; u < U; ++u) raw[u] = load_group(s + c + u * L * GR, GR);
 #pragma unroll
-    for (int u = 0; u < U; u += 2) {
-      float v[2 * GR];
+      for (int u = 0; u < U; u += 2) {
+        float v[2 * GR];
 #pragma unroll
-      for (int i = 0; i < GR; ++i) v[i] = (float)raw[u].v[i], v[GR + i] = (float)raw[u + 1].v[i];
-      add(v, 2 * GR);
+        for (int i = 0; i < GR; ++i) v[i] = (float)raw[u].v[i], v[GR + i] = (float)raw[u + 1].v[i];
+        add(v, 2 * GR);
+      }
     }
-  }
-  for (; c < hi; c += L * GR) {
-    const Vec<T, GR> raw = load_group(s + c, hi - c);
-    float v[GR];
+    for (; c < end; c += L * GR) {
+      const Vec<T, GR> raw = load_group(s + c, end - c);
+      float v[GR];
 #pragma unroll
-    for (int i = 0; i < GR; ++i) v[i] = c + i < hi ? (float)raw.v[i] : -INFINITY;
-    add(v, GR);
+      for (int i = 0; i < GR; ++i) v[i] = c + i < end ? (float)raw.v[i] : -INFINITY;
+      add(v, GR);
+    }
+    all = joined(all, a, k);
   }
-  return a;
+  return all;
 }
 
 // ---- reductions over the L lanes of a row (L 64, or a workgroup)

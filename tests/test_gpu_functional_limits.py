@@ -104,3 +104,47 @@ def test_topk_distill_more_rows_than_a_launch_holds(F, reduction):
         with torch.no_grad():
             each = F.topk_distill_loss(s, t, i, 2.0, "none").double()
         assert abs(loss.item() - each.sum().item() / counted) <= 2 * O.E * each.abs().sum().item() / counted
+
+
+def test_topk_distill_sums_over_a_large_vocabulary(F):
+    """Terms 1 and e^-0.1 in turn in each of 64 pieces of a row, where a long chain of additions drifts: q from the definition."""
+    vocab = (1 << 31) - 1
+    s = torch.zeros(1, vocab, device="cuda")
+    s[0, 1::2] = -0.1
+    term = math.exp(s[0, 1].item())
+    s.requires_grad_(True)
+    t, i = torch.zeros(1, 1, device="cuda"), torch.zeros(1, 1, dtype=torch.long, device="cuda")
+    loss = F.topk_distill_loss(s, t, i)
+    ds, = torch.autograd.grad(loss, s)
+    total = (vocab + 1) // 2 + vocab // 2 * term
+    eps = (1.5 * 1 + 2 + O.CHAIN) * O.E
+    assert abs(loss.item() - math.log(total)) <= eps * (2 + math.log(total))
+    for part, value in ((ds[0, 2::2], 1 / total), (ds[0, 1::2], term / total)):
+        low, high = part.aminmax()
+        assert abs(low.item() / value - 1) <= eps and abs(high.item() / value - 1) <= eps
+    assert abs(ds[0, 0].item() + 1 - 1 / total) <= eps
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("rows,vocab", [(1025, 262_144), (1025, 262_147), (1025, 600_001), (1, 20_000_003)])
+def test_topk_distill_rows_of_several_sums(F, dt, rows, vocab):
+    """A lane's sums join into others at 262144 classes of a row that one workgroup has; largest logits early and late."""
+    s = normal(rows, vocab, seed=1, dt=dt)
+    s[-1, :9] += 20
+    s[0, -9:] += 20
+    if rows > 2:
+        s[1, vocab // 2:], s[2, :vocab // 2] = -math.inf, -math.inf
+    s.requires_grad_(True)
+    t, i = normal(rows, 5, seed=2), torch.randint(0, vocab, (rows, 5), generator=gen(3)).cuda()
+    if rows > 2:
+        i[1] %= vocab // 2
+        i[2] = i[2] % (vocab // 2) + vocab // 2
+    loss = F.topk_distill_loss(s, t, i, 1.0, "none")
+    grad = normal(rows, seed=5)
+    ds, = torch.autograd.grad(loss, s, grad)
+    for at in (0, 1, 2, rows - 1):
+        if at < rows:
+            at = slice(at, at + 1)
+            want = O.topk_distill(s[at].detach().cpu(), t[at].cpu(), i[at].cpu(), 1.0, "none", grad[at])
+            near(loss[at], want["loss"], "loss")
+            near(ds[at], want["ds"], "ds")
