@@ -1120,7 +1120,7 @@ int64_t loose_bytes(int64_t rows, int64_t cols, int dtype) {
 }
 
 int64_t fwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
-  if (is_few(m, n, k, dtype)) return 0;
+  if (m == 0 || is_few(m, n, k, dtype)) return 0;
   const Size z = {m, n, k};
   const int64_t words = plan_of(&z, 1, dtype).split[0].bytes;
   if (dtype == QNN_F32 || k % 8 == 0) return words;

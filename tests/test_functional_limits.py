@@ -38,3 +38,13 @@ def test_layer_norm_partial_rows(code, dim):
         assert rest == 0 and rows <= 512 * side * parts and parts <= rows
         assert parts <= max(512, -(-rows // (512 * side)))
     assert call("qnn_layer_norm_bwd_work", 5, dim, 3, ctypes.byref(n))[0] == 1
+
+
+@pytest.mark.parametrize("code", SIZES)
+@pytest.mark.parametrize("n,k", [(1, 1), (64, 64), (4096, 8192), (4099, 8191), (1 << 21, 1 << 21)])
+def test_linear_act_work_of_no_rows(code, n, k):
+    """None; for a large weight of a 16-bit type the plan of no tiles divided by their number, which ended the process."""
+    size = ctypes.c_int64(-1)
+    for name in ("qnn_linear_act_fwd_work", "qnn_linear_act_bwd_work"):
+        assert call(name, 0, n, k, code, ctypes.byref(size))[0] == 0 and size.value == 0
+        size.value = -1

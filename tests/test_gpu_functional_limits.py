@@ -148,3 +148,17 @@ def test_topk_distill_rows_of_several_sums(F, dt, rows, vocab):
             want = O.topk_distill(s[at].detach().cpu(), t[at].cpu(), i[at].cpu(), 1.0, "none", grad[at])
             near(loss[at], want["loss"], "loss")
             near(ds[at], want["ds"], "ds")
+
+
+# ------------------------------------------------------------------------------------ linear_act
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_linear_act_empty_batch_of_a_large_weight(F, dt):
+    """No rows through a weight of over 20 million elements, forward and backward: zeros for the gradients."""
+    w, b = normal(4096, 8192, seed=1, dt=dt).requires_grad_(True), normal(4096, seed=2, dt=dt).requires_grad_(True)
+    for shape in ((0, 8192), (3, 0, 8192)):
+        for act in ("none", "relu", "gelu"):
+            x = torch.zeros(*shape, device="cuda", dtype=dt).requires_grad_(True)
+            y = F.linear_act(x, w, b, None, act)
+            assert y.shape == (*shape[:-1], 4096)
+            dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.zeros_like(y))
+            assert dx.shape == x.shape and not dw.any() and not db.any()
