@@ -740,8 +740,7 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(Padding p) {
 
 template <class T>
 __global__ __launch_bounds__(256) void zero_kernel(T* p, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) p[i] = (T)0.0f;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = (T)0.0f;
 }
 
 // -------------------------------------------------------------------------- dz, and the bias's gradient
@@ -838,17 +837,17 @@ using Half = Cfg<2, 2, 4, 2, 2>;
 using Small = Cfg<2, 2, 2, 2, 4>;
 using Low = Cfg<1, 2, 2, 2, 4>;
 struct Shape {
-  int bm, bn;
+  int bm, bn, threads;
   float stage16, stage32, ends;
   float alone;   // what one by itself on a CU takes of its stage's time (16 bits, and Low)
   // what each takes where the first operand's rows, DENSE, begin off 64-byte boundaries (16 bits): at 16 bytes, elsewhere
   float off16, off;
 };
-constexpr Shape SHAPES[] = {{Big::BM, Big::BN, 0.72f, 0.0f, 10.0f, 1.0f, 1.0f, 1.0f},
-                            {Middle::BM, Middle::BN, 0.26f, 0.97f, 5.0f, 1.0f, 1.15f, 1.4f},
-                            {Half::BM, Half::BN, 0.19f, 0.50f, 4.0f, 1.0f, 1.5f, 1.6f},
-                            {Small::BM, Small::BN, 0.105f, 0.25f, 4.0f, 1.2f, 1.5f, 1.5f},
-                            {Low::BM, Low::BN, 0.0f, 0.21f, 1.5f, 1.4f, 1.0f, 1.0f}};
+constexpr Shape SHAPES[] = {{Big::BM, Big::BN, Big::NT, 0.72f, 0.0f, 10.0f, 1.0f, 1.0f, 1.0f},
+                            {Middle::BM, Middle::BN, Middle::NT, 0.26f, 0.97f, 5.0f, 1.0f, 1.15f, 1.4f},
+                            {Half::BM, Half::BN, Half::NT, 0.19f, 0.50f, 4.0f, 1.0f, 1.5f, 1.6f},
+                            {Small::BM, Small::BN, Small::NT, 0.105f, 0.25f, 4.0f, 1.2f, 1.5f, 1.5f},
+                            {Low::BM, Low::BN, Low::NT, 0.0f, 0.21f, 1.5f, 1.4f, 1.0f, 1.0f}};
 
 int64_t up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
@@ -893,7 +892,7 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0, bool dense = 
     for (int x = 0; x < (count > 1 ? WANTS * WANTS : WANTS); ++x) {
       int64_t each[2], n[2];
       float work = 0.0f, longest = 0.0f, shortest = INFINITY, us = 0.0f;
-      int64_t blocks = 0;
+      int64_t blocks = 0, grid = 0;
       bool skip = false, split = false;
       for (int i = 0; i < count; ++i) {
         const int want = WANT[i ? x / WANTS : x % WANTS];
@@ -905,6 +904,7 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0, bool dense = 
         each[i] = cdiv(stages[i], s);
         n[i] = cdiv(stages[i], each[i]);
         blocks += tiles[i] * n[i];
+        grid += up(tiles[i] * n[i], 8);
         const float time = (float)each[i] * (i == 0 ? off : 1.0f);
         work += (float)(tiles[i] * n[i]) * time;
         longest = fmaxf(longest, time);
@@ -917,6 +917,7 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0, bool dense = 
       // in whole turns of the longest, or evenly but for the end, where the shortest ones are
       const float most = fmaxf(longest * alone, fminf(turns * longest, work / 256.0f + 0.6f * shortest));
       us += most * stage + (0.6f * turns + 0.4f) * h.ends + (split ? 5.5f : 0.0f);
+      if (grid >= (1LL << 32) / h.threads) us += 1e30f;  // more threads than a launch takes: refused if no tile has fewer
       if (us < least) {
         least = us;
         best.us = us;
@@ -978,13 +979,20 @@ Grads plan_grads(int64_t m, int64_t n, int64_t k, int dtype) {
   return slot.g;
 }
 
+int check_grid(int64_t blocks, int threads) {
+  QNN_REQUIRE(blocks < (1LL << 32) / threads, "too many rows for one call: a launch has fewer than 2^32 threads");
+  return QNN_OK;
+}
+
 // The plan's product i of c = a b^T; its sums' scratch is taken from room.
 int product_of(Product& p, const Plan& plan, int i, const Size& z, const Operand& a, const Operand& b, int tail,
                int edge, const Epilogue& e, char*& room) {
   const Shape& h = SHAPES[plan.shape];
   const Split& s = plan.split[i];
   const int64_t tm = cdiv(z.m, h.bm), tn = cdiv(z.n, h.bn);
-  QNN_REQUIRE(tm * tn * s.n < (1LL << 30) && tn < (1LL << 27), "too many tiles for one call");
+  if (int rc = check_grid(up(tm * tn * s.n, 8), h.threads)) return rc;  // (up: as launch_grads counts the first's)
+  if (s.n > 1)
+    if (int rc = check_grid(2 * cdiv(z.m * (s.ldp / 8), 256), 256)) return rc;  // join, of two such products at most
   p = {a, b, z.m, z.n, z.k, (int)tm, (int)tn, s.n, (int)(tm * tn * s.n), s.span, tail, edge, (float*)room, s.ldp, e};
   room += s.bytes;
   return QNN_OK;
@@ -1022,7 +1030,6 @@ int join(const Product* p, int count, hipStream_t s) {
   }
   const int64_t blocks = j.blocks[0] + j.blocks[1];
   if (blocks == 0) return QNN_OK;
-  QNN_REQUIRE(blocks < (1LL << 31), "too many rows for one call");
   hipLaunchKernelGGL((matmul_join_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, j);
   QNN_LAUNCH_CHECK("matmul_join_kernel");
   return QNN_OK;
@@ -1061,11 +1068,18 @@ int launch_y(int shape, const Product& y, hipStream_t s) {
 }
 
 // p: dx, dw (no blocks: not wanted); the one whose workgroups take longer goes first
+int first_of(const Product (&p)[2]) {
+  return p[1].blocks > 0 && (p[0].blocks == 0 || p[1].span > p[0].span) ? 1 : 0;
+}
+int64_t grid_of(const Product (&p)[2], const ColumnSums& db) {
+  const int first = first_of(p);
+  return up(p[first].blocks, 8) + p[1 - first].blocks + db.blocks;
+}
 template <class T>
 int launch_grads(int shape, const Product (&p)[2], const ColumnSums& db, hipStream_t s) {
   const bool seg = p[0].blocks > 0 && p[0].tail == 0 && in_segments<T>(p[0].a);
-  const int first = p[1].blocks > 0 && (p[0].blocks == 0 || p[1].span > p[0].span) ? 1 : 0;
-  const unsigned blocks = (unsigned)up(p[first].blocks, 8) + (unsigned)p[1 - first].blocks + (unsigned)db.blocks;
+  const int first = first_of(p);
+  const unsigned blocks = (unsigned)grid_of(p, db);
   const int rc = with_cfg<T>(shape, [&](auto cfg) {
     using C = decltype(cfg);
     return with_segments<T, C>(seg, [&](auto in) {
@@ -1098,12 +1112,15 @@ void on_boundaries(const void*& p, int64_t& ld, int64_t rows, int64_t cols, char
   ld = per * GROUP<T>;
   room += up(rows * ld * (int64_t)sizeof(T), 256);
 }
-template <class T>
-int pad(const Padding& pads, hipStream_t s) {
+int64_t grid_of(const Padding& pads) {
   int64_t blocks = 0;
   for (int i = 0; i < pads.count; ++i) blocks += pads.one[i].blocks;
+  return blocks;
+}
+template <class T>
+int pad(const Padding& pads, hipStream_t s) {
+  const int64_t blocks = grid_of(pads);
   if (blocks == 0) return QNN_OK;
-  QNN_REQUIRE(blocks < (1LL << 31), "a matrix too large for one call");
   hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, pads);
   QNN_LAUNCH_CHECK("pad_rows_kernel");
   return QNN_OK;
@@ -1213,15 +1230,16 @@ int qnn_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     const Size z = {m, n, k};
     const bool words = at_words(x, ldx, k, dtype) && at_words(w, ldw, k, dtype);
     const Plan plan = words ? plan_of(&z, 1, dtype) : plan_loose(z, dtype);
+    Padding pads = {};
     if (!words && !plan.loose) {
-      Padding pads = {};
       on_boundaries<T>(px, lx, m, k, room, pads);
       on_boundaries<T>(pw, lw, n, k, room, pads);
-      if (int rc = pad<T>(pads, s)) return rc;
     }
     Product p;
     const int tail = words ? (int)(k % GROUP<T>) : 0;
     if (int rc = product_of(p, plan, 0, z, {px, lx, m}, {pw, lw, n}, tail, 0, e, room)) return rc;
+    if (int rc = check_grid(grid_of(pads), 256)) return rc;
+    if (int rc = pad<T>(pads, s)) return rc;
     if constexpr (sizeof(T) == 2)
       if (plan.loose) {
         hipLaunchKernelGGL((linear_y_loose_kernel<T, Small>), dim3((unsigned)p.blocks), dim3(Small::NT), Small::LDS, s, p);
@@ -1292,8 +1310,42 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
     room += up(st.n * n * 4, 256);
     const Grads plan = m > 0 ? plan_grads(m, n, k, dtype) : Grads{};
     const bool db_beside = db && act == QNN_ACT_NONE && st.n == 1 && (dx || dw) && !plan.apart;
+    if (act != QNN_ACT_NONE) {
+      g = dz;
+      ldg = n;
+    }
+    Padding pads = {};
+    Product p[2] = {};
+    const ColumnSums sums = {dy, db, ldy, m, n, db_beside ? (int)cdiv(n, 64) : 0};
+    if (m > 0 && (dx || dw)) {
+      const Size z[2] = {{m, k, n}, {n, k, m}};
+      // w and x: taken as they are; g: too, where padding it costs more than dx' product loses by it (its rows' short
+      // pieces then lie across the memory's lines: 1890 x 1470 x 11715 bf16 91 us padded, 107 as it is)
+      constexpr int64_t group = GROUP<T>;
+      const bool ww = at_words(w, ldw, k, dtype) && k >= group, xw = at_words(x, ldx, k, dtype) && k >= group;
+      const bool pads_too = (dx && !ww) || (dw && !xw);
+      const float loss = dx ? plan.plan[0].us * (dtype == QNN_F32 ? 0.04f : 0.1f) : 0.0f;
+      const bool gw = at_words(g, ldg, n, dtype) && n >= group &&
+                      (n % group == 0 || loss < (float)(m * n) * 0.5e-6f * sizeof(T) + (pads_too ? 0.0f : 4.0f));
+      if (!gw) on_boundaries<T>(g, ldg, m, n, room, pads);
+      const void *px = x, *pw = w;
+      int64_t lx = ldx, lw = ldw;
+      if (dx && !ww) on_boundaries<T>(pw, lw, n, k, room, pads);
+      if (dw && !xw) on_boundaries<T>(px, lx, m, k, room, pads);
+      const int over = gw ? (int)(n % group) : 0, all = (int)((n - 1) % group + 1);
+      const int dx_edge = ww && k % group ? all : 0, dw_edge = over || (xw && k % group) ? 1 : 0;
+      const Epilogue to_dx = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE};
+      const Epilogue to_dw = {nullptr, nullptr, 0, dw, nullptr, QNN_ACT_NONE};
+      if (dx)
+        if (int rc = product_of(p[0], plan.plan[0], 0, z[0], {g, ldg, m}, {pw, lw, k}, over, dx_edge, to_dx, room)) return rc;
+      if (dw)
+        if (int rc = product_of(p[1], plan.plan[1], 1, z[1], {g, ldg, n}, {px, lx, k}, 0, dw_edge, to_dw, room)) return rc;
+      if (int rc = check_grid(grid_of(pads), 256)) return rc;
+      if (!plan.apart)
+        if (int rc = check_grid(grid_of(p, sums), SHAPES[plan.plan[0].shape].threads)) return rc;
+    }
+    // all of the call's launches can be made
     if (m > 0 && (act != QNN_ACT_NONE || (db && !db_beside))) {
-      QNN_REQUIRE(st.n * st.chunks < (1LL << 31), "too many rows for one call");
       auto launch_dz = [&](auto subs, auto of) {
         constexpr int SUBS = decltype(subs)::value, ACT = decltype(of)::value;
         hipLaunchKernelGGL((linear_dz_kernel<T, SUBS, ACT>), dim3((unsigned)(st.n * st.chunks)), dim3(64 * SUBS), 0, s,
@@ -1308,10 +1360,6 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
       else if (act == QNN_ACT_GELU) with_subs(std::integral_constant<int, QNN_ACT_GELU>{});
       else with_subs(std::integral_constant<int, QNN_ACT_NONE>{});
       QNN_LAUNCH_CHECK("linear_dz_kernel");
-      if (act != QNN_ACT_NONE) {
-        g = dz;
-        ldg = n;
-      }
     }
     if (db && st.n != 1) {  // (no strip: zeros)
       hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)cdiv(n, 64)), dim3(256), 0, s, part, (int)st.n, (T*)db,
@@ -1321,37 +1369,14 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
     if (!dx && !dw) return (int)QNN_OK;
     if (m == 0) {  // an empty sum
       if (dw) {
-        hipLaunchKernelGGL((zero_kernel<T>), dim3((unsigned)cdiv(n * k, 256)), dim3(256), 0, s, (T*)dw, n * k);
+        const int64_t blocks = cdiv(n * k, 256);
+        hipLaunchKernelGGL((zero_kernel<T>), dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20)), dim3(256), 0, s,
+                           (T*)dw, n * k);
         QNN_LAUNCH_CHECK("zero_kernel");
       }
       return (int)QNN_OK;
     }
-    const Size z[2] = {{m, k, n}, {n, k, m}};
-    // w and x: taken as they are; g: too, where padding it costs more than dx' product loses by it (its rows' short
-    // pieces then lie across the memory's lines: 1890 x 1470 x 11715 bf16 91 us padded, 107 as it is)
-    constexpr int64_t group = GROUP<T>;
-    const bool ww = at_words(w, ldw, k, dtype) && k >= group, xw = at_words(x, ldx, k, dtype) && k >= group;
-    const bool pads_too = (dx && !ww) || (dw && !xw);
-    const float loss = dx ? plan.plan[0].us * (dtype == QNN_F32 ? 0.04f : 0.1f) : 0.0f;
-    const bool gw = at_words(g, ldg, n, dtype) && n >= group &&
-                    (n % group == 0 || loss < (float)(m * n) * 0.5e-6f * sizeof(T) + (pads_too ? 0.0f : 4.0f));
-    Padding pads = {};
-    if (!gw) on_boundaries<T>(g, ldg, m, n, room, pads);
-    const void *px = x, *pw = w;
-    int64_t lx = ldx, lw = ldw;
-    if (dx && !ww) on_boundaries<T>(pw, lw, n, k, room, pads);
-    if (dw && !xw) on_boundaries<T>(px, lx, m, k, room, pads);
     if (int rc = pad<T>(pads, s)) return rc;
-    const int over = gw ? (int)(n % group) : 0, all = (int)((n - 1) % group + 1);
-    const int dx_edge = ww && k % group ? all : 0, dw_edge = over || (xw && k % group) ? 1 : 0;
-    Product p[2] = {};
-    const Epilogue to_dx = {nullptr, nullptr, 0, dx, nullptr, QNN_ACT_NONE};
-    const Epilogue to_dw = {nullptr, nullptr, 0, dw, nullptr, QNN_ACT_NONE};
-    if (dx)
-      if (int rc = product_of(p[0], plan.plan[0], 0, z[0], {g, ldg, m}, {pw, lw, k}, over, dx_edge, to_dx, room)) return rc;
-    if (dw)
-      if (int rc = product_of(p[1], plan.plan[1], 1, z[1], {g, ldg, n}, {px, lx, k}, 0, dw_edge, to_dw, room)) return rc;
-    const ColumnSums sums = {dy, db, ldy, m, n, db_beside ? (int)cdiv(n, 64) : 0};
     if (!plan.apart) return launch_grads<T>(plan.plan[0].shape, p, sums, s);
     for (int i = 0; i < 2; ++i) {
       Product one[2] = {};

@@ -48,3 +48,42 @@ def test_linear_act_work_of_no_rows(code, n, k):
     for name in ("qnn_linear_act_fwd_work", "qnn_linear_act_bwd_work"):
         assert call(name, 0, n, k, code, ctypes.byref(size))[0] == 0 and size.value == 0
         size.value = -1
+
+
+THREADS = {(256, 256): 512, (128, 128): 512, (128, 64): 256, (64, 64): 256, (32, 64): 128}
+
+
+@pytest.mark.parametrize("code", SIZES)
+@pytest.mark.parametrize("n,k", [(8, 8), (1, 8), (8, 1), (64, 64), (65, 24), (7, 3), (31, 31)])
+def test_linear_act_tiles_fit_a_launch(code, n, k):
+    """To two thousand million rows the plan takes tiles whose launch can be made."""
+    tm, tn, sp = ctypes.c_int(), ctypes.c_int(), (ctypes.c_int * 2)()
+    for m in (1 << 29, (1 << 30) - 1, 1 << 30, 2_000_000_000):
+        if m * (n + k) * SIZES[code] > 1 << 38:  # what no card holds
+            continue
+        for grads in (0, 1):
+            assert call("qnn_linear_act_plan", m, n, k, code, grads, ctypes.byref(tm), ctypes.byref(tn), sp)[0] == 0
+            tiles = lambda rows, cols: -(-rows // tm.value) * -(-cols // tn.value)
+            blocks = tiles(m, k) * sp[0] + tiles(n, k) * sp[1] if grads else tiles(m, n) * sp[0]
+            assert blocks * THREADS[tm.value, tn.value] < 1 << 32, (m, grads, tm.value, tn.value)
+
+
+@pytest.mark.parametrize("code", SIZES)
+@pytest.mark.parametrize("n,k", [(2048, 8), (8, 2048), (2048, 2048), (2047, 31)])
+def test_linear_act_tiles_past_a_launch(code, n, k):
+    m = (1 << 31) - 1
+    if n > 8:
+        rc, msg = call("qnn_linear_act_fwd", P, k, P, k, None, None, 0, P, None, m, n, k, code, 0, P, 1 << 62, None)
+        assert rc == 1 and b"too many rows" in msg
+    if k > 8:
+        for act in (0, 2):  # (GELU: before its dz is launched)
+            rc, msg = call("qnn_linear_act_bwd", P, n, P, P, k, P, k, P, P, P, P, m, n, k, code, act, P, 1 << 62, None)
+            assert rc == 1 and b"too many rows" in msg
+
+
+@pytest.mark.parametrize("code", [1, 2])
+def test_linear_act_padding_past_a_launch(code):
+    """Rows that are padded: 2^32 groups of 16 bytes are too many."""
+    n, k = 64, 1031
+    rc, msg = call("qnn_linear_act_bwd", P, n, None, P, k, P, k, None, None, P, None, 1 << 25, n, k, code, 0, P, 1 << 62, None)
+    assert rc == 1 and b"too many rows" in msg

@@ -162,3 +162,36 @@ def test_linear_act_empty_batch_of_a_large_weight(F, dt):
             assert y.shape == (*shape[:-1], 4096)
             dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.zeros_like(y))
             assert dx.shape == x.shape and not dw.any() and not db.any()
+
+
+def test_linear_act_no_rows_and_the_largest_weight(F):
+    """The gradient of a weight of over 2^32 elements from no rows: zeros, all of them."""
+    n = k = 65544
+    x = torch.zeros(0, k, device="cuda", dtype=torch.bfloat16)
+    w = torch.empty(n, k, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    y = F.linear_act(x, w)
+    torch.full((n, k), math.nan, device="cuda", dtype=torch.bfloat16)  # (what the allocator may hand out again)
+    dw, = torch.autograd.grad(y, w, torch.zeros_like(y))
+    assert dw.shape == w.shape and not dw.any()
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_linear_act_most_rows_of_a_launch(F, dt):
+    """Tall matrices of one column: single products, rounded once."""
+    m = 2_000_000_001
+    x = torch.empty(m, 1, device="cuda", dtype=dt).normal_(generator=torch.Generator("cuda").manual_seed(1)).requires_grad_(True)
+    w = torch.tensor([[0.7]], device="cuda", dtype=dt)
+    y = F.linear_act(x, w)
+    with torch.no_grad():
+        assert torch.equal(y, x * w)
+    dx, = torch.autograd.grad(y, x, y.detach())
+    with torch.no_grad():
+        assert torch.equal(dx, y * w)
+
+
+def test_linear_act_refuses_more(F):
+    x = torch.zeros((1 << 31) - 1, 1, device="cuda", dtype=torch.float16)
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(RuntimeError, match="too many rows"):
+        F.linear_act(x, torch.ones(1, 1, device="cuda", dtype=torch.float16))
+    assert torch.cuda.memory_allocated() <= before
