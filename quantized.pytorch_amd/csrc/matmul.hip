@@ -806,7 +806,9 @@ __global__ __launch_bounds__(64 * SUBS) void linear_dz_kernel(const T* __restric
   }
 }
 
-// db from the strips' sums: 64 columns a workgroup, 4 threads a column
+// db from the strips' sums: 64 columns a workgroup, 4 threads a column, which add up to JOINED strips one after another
+// and then those sums
+constexpr int JOINED = 256;
 template <class T>
 __global__ __launch_bounds__(256) void linear_db_kernel(const float* part, int strips, T* db, int64_t n) {
   __shared__ float sh[4][64];
@@ -814,8 +816,13 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* part, int s
   const int64_t c = (int64_t)blockIdx.x * 64 + lane;
   float s = 0.0f;
   if (c < n)
+    for (int p0 = sub; p0 < strips; p0 += 4 * JOINED) {
+      const int p1 = p0 + 4 * JOINED < strips ? p0 + 4 * JOINED : strips;
+      float t = 0.0f;
 #pragma unroll 8
-    for (int p = sub; p < strips; p += 4) s += part[p * n + c];
+      for (int p = p0; p < p1; p += 4) t += part[p * n + c];
+      s += t;
+    }
   sh[sub][lane] = s;
   __syncthreads();
   if (sub == 0 && c < n) db[c] = (T)(sh[0][lane] + sh[1][lane] + sh[2][lane] + sh[3][lane]);
@@ -1147,7 +1154,7 @@ int64_t fwd_bytes(int64_t m, int64_t n, int64_t k, int dtype) {
 }
 
 // Strips of rows for dz's sums: one of 16 rows at a time for a few rows, which saves the launch that adds
-// the strips up; else enough workgroups of 4 to fill the chip.
+// the strips up; else enough workgroups of 4 to fill the chip, and as many as leave a lane 512 rows to add.
 struct Strips {
   int chunks;
   int64_t n, rows;  // strips, and rows in each
@@ -1155,7 +1162,8 @@ struct Strips {
 Strips strips_of(int64_t m, int64_t n) {
   const int64_t chunks = cdiv(n, 512);
   if (m <= 256) return {(int)chunks, m > 0, m};
-  const int64_t want = cdiv(1024, chunks), most = cdiv(m, 16), s = want < most ? want : most, rows = cdiv(m, s);
+  const int64_t want = cdiv(1024, chunks), most = cdiv(m, 16), s = want < most ? want : most;
+  const int64_t rows = cdiv(m, s) < 4 * 512 ? cdiv(m, s) : 4 * 512;
   return {(int)chunks, cdiv(m, rows), rows};
 }
 

@@ -87,3 +87,15 @@ def test_linear_act_padding_past_a_launch(code):
     n, k = 64, 1031
     rc, msg = call("qnn_linear_act_bwd", P, n, None, P, k, P, k, None, None, P, None, 1 << 25, n, k, code, 0, P, 1 << 62, None)
     assert rc == 1 and b"too many rows" in msg
+
+
+@pytest.mark.parametrize("code", SIZES)
+@pytest.mark.parametrize("n", [1, 8, 600, 100000])
+def test_linear_act_strips_of_rows(code, n):
+    """The bias's gradient has a partial row for each 2048 rows at least: 512 that a lane adds."""
+    size = ctypes.c_int64(-1)
+    for m in (1000, 3_000_000, 1 << 26, (1 << 31) - 1):
+        if m * n > 1 << 37:
+            continue
+        assert call("qnn_linear_act_bwd_work", m, n, 8, code, ctypes.byref(size))[0] == 0
+        assert size.value >= -(-m // 2048) * n * 4 * (m > 256)

@@ -195,3 +195,20 @@ def test_linear_act_refuses_more(F):
     with pytest.raises(RuntimeError, match="too many rows"):
         F.linear_act(x, torch.ones(1, 1, device="cuda", dtype=torch.float16))
     assert torch.cuda.memory_allocated() <= before
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n", [(1 << 26, 8), (3_000_000, 600), (70_000, 30_011), (300_000_000, 2), (4097, 65)])
+def test_linear_act_bias_gradient_over_many_rows(F, dt, m, n):
+    """Equal terms, where a long chain of fp32 additions drifts."""
+    x, b = torch.zeros(m, 1, device="cuda", dtype=dt), torch.zeros(n, device="cuda", dtype=dt).requires_grad_(True)
+    dy = torch.full((m, n), 1.1e-3, device="cuda", dtype=dt)
+    one = dy[0, 0].item()
+    for act, slope, err in (("none", 1.0, 0.0), ("relu", 1.0, 0.0)) if m * n > 1 << 27 else (("none", 1.0, 0.0), ("relu", 1.0, 0.0), ("gelu", 0.5, 2.0 ** -14)):
+        bias = b if act != "relu" else torch.ones_like(b).requires_grad_(True)
+        y = F.linear_act(x, torch.zeros(n, 1, device="cuda", dtype=dt), bias, None, act)
+        db, = torch.autograd.grad(y, bias, dy)
+        value = torch.full((n,), m * one * slope, dtype=torch.float64)
+        value, err = O._out(value, ((O.CHAIN + 2) * O.E + err) * value, dt)
+        # (sums past fp16's largest, 65504: 2^26 and 3e8 terms of 1.1e-3 round to infinity)
+        near(db, (torch.where(value > torch.finfo(dt).max, float("inf"), value), err), act)
