@@ -459,7 +459,8 @@ int qnn_chain_epilogue(const uint8_t* bncode, int n, int ho, int wo, int c, cons
  *
  * The operators of a student's training step that are not quantized (qnn/functional.py).  Matrices
  * are row-major with a row stride ("ld", in elements, at least the row's length); the last index is
- * dense.  Sums, statistics and states are held in fp32 whatever the type; each output is rounded
+ * dense.  Sums, statistics and states are held in fp32 whatever the type, but for what 16-bit types keep
+ * of an activation's derivative (slope below) and the gradient dz, which is an output too; each output is rounded
  * once.  Nothing is kept between calls: `work` is scratch of at least the size that the matching
  * *_work call gives (16-byte aligned), free for other use once the call's kernels have run.  Every
  * result is the same from run to run (no floating-point atomics).  No output overlaps an input. */
@@ -470,7 +471,8 @@ enum { QNN_ACT_NONE = 0, QNN_ACT_RELU = 1, QNN_ACT_GELU = 2 };
  * the int8 epilogue: the residual first, then the activation.  GELU is z Phi(z).  All of one type.
  * slope (nullable): act'(z) for qnn_linear_act_bwd --
  *   ReLU  [m][ceil(n / 8)] bytes, bit c & 7 of byte c / 8: z is not <= 0;
- *   GELU  [m][n], fp32 for QNN_F32, else uint16 fixed point, 8192 + 28672 act'(z) (0: NaN).
+ *   GELU  [m][n], fp32 for QNN_F32; 16 bits for QNN_BF16, fp16 of 2^15 act'(z), off by 2^-11 of act'(z) (to 2^-29), and
+ *         for QNN_F16, 24096 + 40192 s (0: NaN) with s = sign(act') |act'(z)|^(1/4), off by 5e-5 |act'(z)|^(3/4).
  * 1 <= n, k and the row strides <= 2^21, m < 2^31; m == 0 is a no-op.  Rows of x, w (and dy, dz) that are
  * whole 16-byte groups begin on 16-byte boundaries.  Replaces nothing of the reference (its layers are
  * F.linear on fake-quantized operands, quantize.py:423-430); stands beside qnn_qconv2d_fwd. */

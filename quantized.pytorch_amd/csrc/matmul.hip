@@ -57,7 +57,7 @@ __device__ __forceinline__ void finish8(float (&z)[8], const float (&bias)[8], c
       } else {
         Vec<int16_t, 8> q;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q.v[i] = slope_pack(d[i]);
+        for (int i = 0; i < 8; ++i) q.v[i] = slope_pack<T>(d[i]);
         store_group((int16_t*)e.slope + row * n + col, q, left);
       }
     }
@@ -782,7 +782,7 @@ __global__ __launch_bounds__(64 * SUBS) void linear_dz_kernel(const T* __restric
           v[i] = (float)g[u].v[i];
           if constexpr (ACT == QNN_ACT_RELU) v[i] = d[u].v[0] >> i & 1 ? v[i] : 0.0f;
           else if constexpr (ACT == QNN_ACT_GELU && sizeof(T) == 4) v[i] *= d[u].v[i];
-          else if constexpr (ACT == QNN_ACT_GELU) v[i] *= slope_unpack(d[u].v[i]);
+          else if constexpr (ACT == QNN_ACT_GELU) v[i] *= slope_unpack<T>(d[u].v[i]);
           v[i] = (float)(T)v[i];  // db is the sum of dz as it is written
           sum[i] += v[i];
         }

@@ -62,8 +62,10 @@ def linear_act(x, weight, bias=None, residual=None, activation="none"):
     x [..., in], weight [out, in], bias [out], residual [..., out] (the output's shape; expand it for
     a broadcast one), all of one type; activation "none", "relu" or "gelu" (the erf form), applied
     after the residual as in the int8 layers' epilogue.  Under autograd gradients flow to all four;
-    between the passes a bit an element is kept for ReLU, and the slope for GELU (16 bits, 32 in
-    float32).  The gradient of z is rounded to the type once, before the two products it enters."""
+    between the passes a bit an element is kept for ReLU, and the slope d for GELU: 32 bits in float32,
+    in bfloat16 and float16 16 bits that are off by 2^-11 of d, and by 5e-5 |d|^(3/4), an eighth and
+    (from |d| = 1e-4 on) at most the whole of the type's half step.  The gradient of z is rounded to the
+    type once, before the two products it enters."""
     act = _ACTS.get(activation)
     if act is None:
         raise ValueError(f"qnn: linear_act activation must be one of {sorted(_ACTS)}, got {activation!r}")
