@@ -511,6 +511,8 @@ int qnn_layer_norm_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, 
  * of t / temp over the entries that are there, q the softmax of s / temp over the vocabulary:
  *   row_loss[r] = temp^2 sum_e p_e (log p_e - log q_index[e])      (an entry with p_e = 0 adds 0)
  *   ds[r][j]    = g temp (q_j - sum over e with index[e] == j of p_e)
+ * (temp^2 KL of p and q where the classes are distinct; a class that is named twice adds each of its entries, which
+ * takes temp^2 sum_e p_e log(P / p_e) off the KL with their sum P at the class, whatever the student.)
  * A row without entries, or whose teacher logits are all -inf, is not counted: loss 0, gradient 0.
  * row_loss [rows]; stats [4 rows + 4] fp32, what the backward takes; loss (nullable): one fp32,
  * the sum of the counted rows' losses, over their number when mean != 0 (0 rows counted: 0).

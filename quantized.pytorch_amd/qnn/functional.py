@@ -114,15 +114,18 @@ class LayerNorm(nn.LayerNorm):
 
 # ----------------------------------------------------------------------------- topk_distill_loss
 def topk_distill_loss(logits, teacher_logits, teacher_index, temperature=1.0, reduction="mean"):
-    """temperature^2 KL(p || q) between a teacher known by its top logits and a student.
+    """temperature^2 sum_e p_e (log p_e - log q_index[e]) between a teacher known by its top logits
+    and a student: temperature^2 KL(p || q) where a row's classes are distinct.
 
     logits [..., vocab]; teacher_logits [..., top] (any of the three types) at the classes
     teacher_index [..., top] (int64 or int32), top <= 1024.  p is the softmax of teacher_logits /
     temperature over a row's entries, q that of logits / temperature over the vocabulary.  An entry
-    with a negative index is absent (padding); a class that is named twice has the sum of its
-    entries; an index past the vocabulary, or a teacher logit that is NaN, makes its row's loss and
-    gradient NaN.  A row without
-    entries (or whose teacher logits are all -inf) is not counted: loss 0, gradient 0.
+    with a negative index is absent (padding).  A class that is named twice takes part with each of
+    its entries: the gradient is that of the KL whose P at the class is the sum of them, and the
+    value is that KL plus temperature^2 sum_e p_e log(p_e / P_index[e]), a constant of the teacher,
+    which is 0 without such classes and else negative.  An index past the vocabulary, or a teacher
+    logit that is NaN, makes its row's loss and gradient NaN.  A row without entries (or whose
+    teacher logits are all -inf) is not counted: loss 0, gradient 0.
 
     The loss is float32: the mean over the counted rows (0 if there is none), their sum, or with
     "none" the rows' losses [...].  Gradients flow to logits alone, in their type; the teacher is a
