@@ -461,7 +461,8 @@ int qnn_chain_epilogue(const uint8_t* bncode, int n, int ho, int wo, int c, cons
  * are row-major with a row stride ("ld", in elements, at least the row's length); the last index is
  * dense.  Sums, statistics and states are held in fp32 whatever the type, but for what 16-bit types keep
  * of an activation's derivative (slope below) and the gradient dz, which is an output too; each output is rounded
- * once.  Nothing is kept between calls: `work` is scratch of at least the size that the matching
+ * once.  Nothing is kept between calls (but a thread's last 32 plans of the backward product, tiles and splits by the
+ * sizes and the type alone): `work` is scratch of at least the size that the matching
  * *_work call gives (16-byte aligned), free for other use once the call's kernels have run.  Every
  * result is the same from run to run (no floating-point atomics).  No output overlaps an input. */
 enum { QNN_F32 = 0, QNN_BF16 = 1, QNN_F16 = 2 };
@@ -473,7 +474,9 @@ enum { QNN_ACT_NONE = 0, QNN_ACT_RELU = 1, QNN_ACT_GELU = 2 };
  *   ReLU  [m][ceil(n / 8)] bytes, bit c & 7 of byte c / 8: z is not <= 0;
  *   GELU  [m][n], fp32 for QNN_F32; 16 bits for QNN_BF16, fp16 of 2^15 act'(z), off by 2^-11 of act'(z) (to 2^-29), and
  *         for QNN_F16, 24096 + 40192 s (0: NaN) with s = sign(act') |act'(z)|^(1/4), off by 5e-5 |act'(z)|^(3/4).
- * 1 <= n, k and the row strides <= 2^21, m < 2^31; m == 0 is a no-op.  Rows of x, w (and dy, dz) that are
+ * 1 <= n, k and the row strides <= 2^21, m < 2^31; m == 0 is a no-op.  Refused is what no launch holds, whose
+ * threads are fewer than 2^32: from 2^31 - 128 rows on (and fewer of outputs that the card's memory would not hold), and
+ * 2^32 groups of 16 bytes in matrices whose rows have to be padded.  Rows of x, w (and dy, dz) that are
  * whole 16-byte groups begin on 16-byte boundaries.  Replaces nothing of the reference (its layers are
  * F.linear on fake-quantized operands, quantize.py:423-430); stands beside qnn_qconv2d_fwd. */
 int qnn_linear_act_fwd_work(int64_t m, int64_t n, int64_t k, int dtype, int64_t* bytes);
@@ -495,7 +498,8 @@ int qnn_linear_act_bwd(const void* dy, int64_t ldy, const void* slope, const voi
 
 /* y = (x - mean) rstd w + b over the last dim, mean and the biased variance of each row in two steps
  * (the deviations, not the squares' difference), rstd = 1 / sqrt(var + eps).  w, b nullable (1, 0), of
- * type wdtype: dtype or QNN_F32.  mean, rstd [rows] fp32, nullable: what the backward takes. */
+ * type wdtype: dtype or QNN_F32.  mean, rstd [rows] fp32, nullable: what the backward takes.  rows < 2^31, but
+ * < 2^22 of rows over 64 KiB (what a launch holds). */
 int qnn_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, float* mean, float* rstd,
                        int64_t rows, int64_t dim, float eps, int dtype, int wdtype, qnn_stream_t stream);
 /* g = dy w, xh = (x - mean) rstd: dx = rstd (g - mean(g) - xh mean(g xh)), dw = sum over rows of dy xh,

@@ -11,7 +11,9 @@ import math
 import torch
 
 E = 2.0 ** -24
-CHAIN = 1024  # no kernel adds more than this many terms one after another, beside the products' chains
+# No kernel adds more than this many terms one after another, beside the products' chains: lanes stop at 512, and the sums of
+# those are added in a few levels (rows of a layer norm up to 2^29 elements, everything else at any size).
+CHAIN = 1024
 
 
 def _u(dtype):

@@ -9,9 +9,18 @@
 // the next two on their way while it works on one; the weights stay in registers from row to row.
 // 16384 x 4096 bf16: forward 47 us (5.7 TB/s), backward 85 (4.7 TB/s) and 5.
 //
+// Wide rows ask for more registers than there are.  Backward over 8192 columns spills 164 to 1052 bytes a lane, forward
+// over 2048 groups (16384 columns of 16 bits, 8192 of fp32) 20 to 444; 4097 to 8192 columns of 16 bits leave the
+// backward pass one wave a SIMD.  1000 x 8192 bf16 forward 12 us and backward 22, 1000 x
+// 16384 18 and 70 (of which the bytes are 13 and 20), 1000 x 12288 fp32 26 and 112 (20 and 30), 1000 x 32768 bf16
+// 97 and 358 (27 and 40).
+//
 // The backward pass sums dw and db on the way: a lane has the same columns in every row, so they are sums
 // in its registers, joined over a workgroup's rows in LDS, written as one partial row a workgroup and
-// added up by a second, small launch in a fixed order.
+// added up by a second, small launch in a fixed order.  Where a workgroup has one row of few (up to 512), the
+// partial rows are more than the data: 512 x 4096 bf16 33.6 MB beside 12.6, 12.5 us and 4.8 (the bytes: 2.6).
+//
+// Rows shorter than a group are a thread's each: 4.2 million x 4 bf16 24 us and 63 (the bytes: 14 and 21).
 #include "float_common.h"
 
 namespace qnn {
@@ -526,7 +535,8 @@ bool with_shape(int64_t dim, F&& f) {
   return true;
 }
 
-// Partial rows of dw and db: two workgroups of 256 a CU, and as many as keep a lane's sums within CHAIN rows.
+// Partial rows of dw and db: two workgroups of 256 a CU (where their registers let two of them in, see above), and as
+// many as keep a lane's sums within CHAIN rows.
 constexpr int MAX_PARTS = 512;
 
 // workgroups of a launch over all rows, `each` of them at a time in one

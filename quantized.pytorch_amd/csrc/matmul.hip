@@ -942,7 +942,8 @@ Plan plan_of(const Size* size, int count, int dtype, int from = 0, bool dense = 
 // Whether few_rows_kernel takes the forward product: up to 16 rows of x, but 2 where the rows' groups begin
 // inside words (4 x 4096 x 4097 bf16 takes it 21 us and loose_tile 18, one row 16), and one where w of 16-bit
 // types is large (2 x 8192 x 8191 bf16 72 us and 33 in tiles, 8 x 8192 x 8192 28 and 23; but 9 x 4096 x 4096
-// 8.8 and 10.1).
+// 8.8 and 10.1).  "Large" is 20 million elements, between those two weights of 17 and 67; where between them the sides
+// cross was not measured.
 constexpr int FEW = 16;
 bool is_few(int64_t m, int64_t n, int64_t k, int dtype) {
   if (dtype == QNN_F32) return m <= FEW;
