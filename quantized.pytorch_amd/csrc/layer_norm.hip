@@ -257,8 +257,8 @@ __global__ __launch_bounds__(S::NT) void layer_norm_bwd_kernel(const T* __restri
   }
 }
 
-// A sum is at most 1024 additions deep at any size that fits the card: CHAIN of a lane's own terms one after another, the
-// rows of a workgroup, JOINED partial rows, and the sums of those.
+// A sum is at most 1024 additions deep (of rows to 2^27 columns): CHAIN of a lane's own terms one after another, the rows
+// of a workgroup, JOINED partial rows, and the sums of those.
 constexpr int CHAIN = 512, JOINED = 256;
 
 // dw and db from `parts` partial rows: 64 columns a workgroup at a time, 16 threads a column
